@@ -1057,8 +1057,12 @@ int b200_get_rows(int src_type, const void* src, const int64_t sne[4], const siz
     using namespace b200;
     if (!src || !idx || !dst || !dev_err || !shape_ok(sne, snb) || !shape_ok(ine, inb) || ine[3] != 1)
         return B200_E_INVALID;
-    if (src_type != 0 && src_type != 1) return B200_E_UNSUPPORTED;   // F32, F16
+    if (src_type != 0 && src_type != 1 && src_type != 2 && src_type != 8)
+        return B200_E_UNSUPPORTED;   // F32, F16, Q4_0, Q8_0
     if (ine[1] > sne[2] || ine[2] > sne[3]) return B200_E_INVALID;
+    if (src_type > 1)
+        return get_rows_quant_impl(src_type, src, sne, snb, idx, ine, inb, dst, dev_err,
+                                   static_cast<cudaStream_t>(stream));
     const int64_t n = sne[0] * ine[0] * ine[1] * ine[2];
     const int64_t rows = ine[0] * ine[1] * ine[2];
     if (rows > 0 && rows < (1ll << 31) && sne[0] >= 64) {

@@ -50,6 +50,9 @@ int mul_mat_vec_tiles(int wtype, const void* w_packed, int64_t N, int64_t K, con
                       int64_t M, float* dst, int64_t ldd, void* workspace, size_t workspace_bytes, int* dev_err,
                       cudaStream_t st);
 bool weight_type_supported(int type, int64_t K);
+// b200_get_rows over a Q4_0 (2) / Q8_0 (8) table (kv_cache.cu); pointers, shapes and idx checked before.
+int get_rows_quant_impl(int src_type, const void* src, const int64_t sne[4], const size_t snb[4], const int32_t* idx,
+                        const int64_t ine[4], const size_t inb[4], float* dst, int* dev_err, cudaStream_t st);
 // dst_bases / n_dst / col0: the output columns [col0, col0 + N) of every one of n_dst [M][ldd]
 // buffers (a device array of pointers, other GPUs' included) instead of dst
 int mul_mat_impl(int wtype, const void* w_packed, int64_t N, int64_t K, const float* src1, int64_t lda, int64_t M,

@@ -13,6 +13,7 @@ LIB_PATH = os.path.join(PKG, "lib", "libggml-b200.so")
 
 # ggml_type numbering
 F32, F16, Q8_0, Q4_K, Q6_K, I32, BF16 = 0, 1, 8, 12, 14, 26, 30
+I64 = 27
 Q4_0 = 2
 TYPE_NAMES = {F32: "f32", F16: "f16", Q8_0: "q8_0", Q4_K: "q4_K", Q6_K: "q6_K", I32: "i32", BF16: "bf16"}
 BLOCK = {F32: (1, 4), F16: (1, 2), BF16: (1, 2), Q4_0: (32, 18), Q8_0: (32, 34), Q4_K: (256, 144), Q6_K: (256, 210)}
@@ -330,6 +331,13 @@ _SIGS.update({
     "b200_peer_wait_limit_ns": (_c.c_uint64, []),
 })
 _SIGS.update({
+    "b200_rope_multi": (_int, [_int, _vp, _vp, _vp, _vp, _int, _int, _vp, _f, _f, _f, _vp, _vp]),
+    "b200_set_rows": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp]),
+    "b200_flash_attn_kvq_workspace_size": (_sz, [_i64] * 6),
+    "b200_flash_attn_kvq": (_int, [_int, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _vp, _f,
+                                   _f, _vp, _sz, _vp, _vp]),
+})
+_SIGS.update({
     "ggml_backend_b200_builder_new": (_vp, []),
     "ggml_backend_b200_builder_free": (None, [_vp]),
     "ggml_backend_b200_builder_reset": (None, [_vp]),
@@ -592,6 +600,136 @@ def mul_mat_id_ffn(wtype_gate_up, gate, up, wtype_down, down, H, F, n_expert, x,
                                      _ptr(x), x_nb1, x_nb2, ne11, _ptr(ids), ids_nb0, ids_nb1, n_used, n_tokens,
                                      _ptr(dst), d_nb1, d_nb2, _ptr(workspace),
                                      workspace.numel() * workspace.element_size(), _ptr(dev_err), _stream(stream))
+
+
+ROPE_MROPE, ROPE_VISION, ROPE_IMROPE = 8, 24, 40
+_I64x4, _SZx4, _I32x4 = ctypes.c_int64 * 4, ctypes.c_size_t * 4, ctypes.c_int32 * 4
+_ROW_TYPES = {"torch.float32": F32, "torch.float16": F16, "torch.int32": I32, "torch.int64": I64}
+
+
+def _type_of(t, what):
+    ty = _ROW_TYPES.get(str(t.dtype))
+    if ty is None:
+        raise B200Error(f"{what}: dtype {t.dtype} is not supported")
+    return ty
+
+
+def _on(t, what, *others):
+    """The current device must hold every tensor of a call (kernels launch on the current device)."""
+    import torch
+    dev = torch.cuda.current_device()
+    for x in (t,) + others:
+        if x is not None and (not x.is_cuda or x.device.index != dev):
+            raise B200Error(f"{what}: a tensor is on {x.device}, the current device is cuda:{dev}")
+
+
+def _dims(t):
+    """ggml's ne / nb (bytes) of a torch tensor of 1 to 4 dims, outermost first."""
+    sh, st, es = t.shape, t.stride(), t.element_size()
+    n = len(sh)
+    ne, nb = [1, 1, 1, 1], [es, es, es, es]
+    for i in range(n):
+        ne[i], nb[i] = sh[n - 1 - i], st[n - 1 - i] * es
+    for i in range(n, 4):
+        nb[i] = nb[i - 1] * ne[i - 1]
+    return ne, nb
+
+
+def _dims_q(t, kind, what):
+    """The same for a uint8 tensor whose innermost dim holds the blocks of one row of a quantised type."""
+    block, size = BLOCK[kind]
+    ne, nb = _dims(t)
+    if t.element_size() != 1 or nb[0] != 1 or ne[0] % size:
+        raise B200Error(f"{what}: rows of {TYPE_NAMES.get(kind, kind)} are a uint8 tensor whose last dim holds whole blocks")
+    ne[0], nb[0] = ne[0] // size * block, size
+    return ne, nb
+
+
+def rope_multi(x, pos, dst, n_dims, mode, sections, freq_base=10000.0, freq_scale=1.0, attn_factor=1.0, stream=None):
+    """ROPE with several position axes (b200_rope_multi): x f32 / f16 [.., n_tokens, n_head, head_dim] with any
+    strides, pos int32 [4, n_tokens], dst contiguous of x's shape and type (x itself when contiguous)."""
+    _on(x, "rope_multi", pos, dst)
+    ne, nb = _dims(x)
+    if dst.dtype != x.dtype or dst.shape != x.shape or not dst.is_contiguous() or str(pos.dtype) != "torch.int32" or \
+            not pos.is_contiguous() or tuple(pos.shape) != (4, ne[2]):
+        raise B200Error("rope_multi: dst is contiguous and of x's shape and type, pos contiguous int32 [4, n_tokens]")
+    check(lib().b200_rope_multi(_type_of(x, "rope_multi"), x.data_ptr(), _I64x4(*ne), _SZx4(*nb), pos.data_ptr(), n_dims,
+                                mode, _I32x4(*sections), freq_base, freq_scale, attn_factor, dst.data_ptr(),
+                                _stream(stream)), "rope_multi")
+    return dst
+
+
+def set_rows(src, idx, dst, dst_type, dev_err, stream=None):
+    """dst[.., idx[i], :] = src[.., i, :] (b200_set_rows): src f32, idx int32 / int64 [.., n_rows], dst f32, f16 or,
+    for Q4_0 / Q8_0, a uint8 tensor whose last dim holds a row's blocks; quantised as they are written."""
+    _on(src, "set_rows", idx, dst, dev_err)
+    if str(src.dtype) != "torch.float32":
+        raise B200Error("set_rows: src is f32")
+    sne, snb = _dims(src)
+    ine, inb = _dims(idx)
+    if dst_type in (F32, F16):
+        if _type_of(dst, "set_rows") != dst_type:
+            raise B200Error("set_rows: dst is not of dst_type")
+        dne, dnb = _dims(dst)
+    else:
+        dne, dnb = _dims_q(dst, dst_type, "set_rows")
+    check(lib().b200_set_rows(src.data_ptr(), _I64x4(*sne), _SZx4(*snb), _type_of(idx, "set_rows"), idx.data_ptr(),
+                              _I64x4(*ine), _SZx4(*inb), dst_type, dst.data_ptr(), _I64x4(*dne), _SZx4(*dnb),
+                              dev_err.data_ptr(), _stream(stream)), "set_rows")
+    return dst
+
+
+def get_rows(src, src_type, idx, dst, dev_err, stream=None):
+    """dst[.., i, :] = src[.., idx[i], :] as f32 (b200_get_rows): src f32, f16 or, for Q4_0 / Q8_0, a uint8 tensor
+    whose last dim holds a row's blocks; idx int32; dst contiguous f32."""
+    _on(src, "get_rows", idx, dst, dev_err)
+    if src_type in (F32, F16):
+        if _type_of(src, "get_rows") != src_type:
+            raise B200Error("get_rows: src is not of src_type")
+        sne, snb = _dims(src)
+    else:
+        sne, snb = _dims_q(src, src_type, "get_rows")
+    ine, inb = _dims(idx)
+    if str(idx.dtype) != "torch.int32" or str(dst.dtype) != "torch.float32" or not dst.is_contiguous() or \
+            dst.numel() != sne[0] * idx.numel():
+        raise B200Error("get_rows: idx is int32, dst contiguous f32 with a row for every index")
+    check(lib().b200_get_rows(src_type, src.data_ptr(), _I64x4(*sne), _SZx4(*snb), idx.data_ptr(), _I64x4(*ine),
+                              _SZx4(*inb), dst.data_ptr(), dev_err.data_ptr(), _stream(stream)), "get_rows")
+    return dst
+
+
+def flash_attn_kvq_workspace_size(D, T, H, KV, HK, S=1):
+    return lib().b200_flash_attn_kvq_workspace_size(D, T, H, KV, HK, S)
+
+
+def flash_attn_kvq(kv_type, q, k, v, mask, dst, scale, workspace, dev_err, softcap=0.0, stream=None):
+    """Attention over a KV cache held in 4 bits (b200_flash_attn_kvq): q f32 / f16 [S, T, H, D], k and v uint8
+    [S, KV, HK, D / 32 * 18] (Q4_0 blocks), mask f16 [S or 1, T, KV] or None, dst contiguous f32 / f16 [S, T, H, D];
+    strides of q, k, v and mask are theirs."""
+    _on(q, "flash_attn_kvq", k, v, mask, dst, workspace, dev_err)
+    S, T, H, D = q.shape
+    es = q.element_size()
+    qs = q.stride()
+    kne, knb = _dims_q(k, kv_type, "flash_attn_kvq")
+    vne, vnb = _dims_q(v, kv_type, "flash_attn_kvq")
+    if dst.shape != q.shape or not dst.is_contiguous():
+        raise B200Error("flash_attn_kvq: dst is contiguous and of q's shape")
+    mnb = None
+    if mask is not None:
+        if str(mask.dtype) != "torch.float16" or mask.dim() != 3 or mask.shape[0] not in (1, S) or \
+                mask.shape[1] < T or mask.shape[2] < kne[2]:
+            raise B200Error("flash_attn_kvq: mask is f16 [S or 1, T, KV]")
+        ms = mask.stride()
+        mnb = _SZx4(2 * ms[2], 2 * ms[1], 0, 2 * ms[0] if mask.shape[0] == S else 0)
+    # a cache row holds the heads of a key side by side: ggml's view has the keys as dim 1, the heads as dim 2
+    check(lib().b200_flash_attn_kvq(
+        kv_type, _type_of(q, "flash_attn_kvq"), q.data_ptr(), _I64x4(D, T, H, S),
+        _SZx4(qs[3] * es, qs[1] * es, qs[2] * es, qs[0] * es), k.data_ptr(), _I64x4(kne[0], kne[2], kne[1], kne[3]),
+        _SZx4(knb[0], knb[2], knb[1], knb[3]), v.data_ptr(), _I64x4(vne[0], vne[2], vne[1], vne[3]),
+        _SZx4(vnb[0], vnb[2], vnb[1], vnb[3]), None if mask is None else mask.data_ptr(), mnb,
+        _type_of(dst, "flash_attn_kvq"), dst.data_ptr(), scale, softcap, workspace.data_ptr(),
+        workspace.numel() * workspace.element_size(), dev_err.data_ptr(), _stream(stream)), "flash_attn_kvq")
+    return dst
 
 
 def mul_mat_id_route_view(K, n_expert, n_used, n_tokens):

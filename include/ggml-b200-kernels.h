@@ -167,6 +167,27 @@ int    b200_flash_attn_ext(const float * q, int64_t q_nb1, int64_t q_nb2,
 int    b200_kv_to_f16(int type, const void * src, int64_t D, int64_t KV, int64_t HK, int64_t nb1, int64_t nb2,
                       void * dst, void * stream);
 
+/* FLASH_ATTN_EXT over a KV cache held in 4 bits, read as it is stored, for any number of tokens from
+ * one on and several streams (sequences with a cache view each, ggml's ne[3]). No counterpart in the
+ * reference (its handler takes F16 K / V only, ggml-rocket.cpp:7654-7700). ggml layouts, byte strides:
+ *   q    F32 (0) or F16 (1) [D, T, H, S]      k, v  Q4_0 (2) [D, KV, HK, S]: nb[0] 18, the others
+ *                                                   multiples of D / 16 bytes, as are the bases
+ *   mask F16 [KV, >= T, 1, S] (row t of stream s at mask + t * mnb[1] + s * mnb[3]; mnb[3] 0 shares one)
+ *        or NULL
+ *   dst  F32 (0) or F16 (1) [D, H, T, S] contiguous
+ *   dst[:, h, t, s] = sum_j softmax_j(S[j]) v[:, j, h / (H / HK), s],
+ *   S[j] = softcap * tanh(scale * q.k / softcap) (scale * q.k when softcap == 0) + mask[s][t][j]
+ * A key whose mask is -inf takes no part, whatever its bytes hold; a row with no other key is zeros. D in
+ * {64, 128}, H % HK == 0, KV <= 2^30. The workspace (256-byte aligned,
+ * b200_flash_attn_kvq_workspace_size bytes) holds the parts of rows whose keys several CTAs share; calls
+ * sharing one must not overlap on the GPU. No ALiBi, no sinks. */
+size_t b200_flash_attn_kvq_workspace_size(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S);
+int    b200_flash_attn_kvq(int kv_type, int q_type, const void * q, const int64_t qne[4], const size_t qnb[4],
+                           const void * k, const int64_t kne[4], const size_t knb[4], const void * v,
+                           const int64_t vne[4], const size_t vnb[4], const void * mask, const size_t mnb[4],
+                           int dst_type, void * dst, float scale, float softcap, void * workspace,
+                           size_t workspace_bytes, int * dev_err, void * stream);
+
 /* ---- decode-size MUL_MAT (M = 1..32) over Q4_K, Q6_K and Q8_0 weights ----------------------
  * The reference leaves decode (M below its ROCKET_MIN_M) on the CPU (ggml-rocket.cpp:7424-7496);
  * this is MUL_MAT for those M on the GPU: dst[m, n] = sum_k src1[m, k] * W[n, k] with W the
@@ -243,10 +264,36 @@ int b200_rope(const float * x, const int64_t ne[4], const size_t nb[4], const in
  * B200_E_UNSUPPORTED. */
 int b200_rope_f16(const float * x, const int64_t ne[4], const size_t nb[4], const int32_t * pos, int n_dims, int mode,
                   float freq_base, float freq_scale, float attn_factor, void * dst, const size_t dnb[4], void * stream);
-/* dst[:, i, j, k] = src[:, idx[i, j, k], j, k]; src f32 (0) or f16 (1), dst f32 [sne[0], ine[0],
- * ine[1], ine[2]]; an index outside src's rows records a device error and yields a zero row */
+/* ROPE with several position axes, ggml's modes MROPE (8), VISION (24) and IMROPE (40): x
+ * [head_dim, n_head, n_tokens, n_batch] F32 (0) or F16 (1), pos int32 [4][n_tokens] (time, height,
+ * width and one more axis of every token, shared by the batch), dst contiguous and of x's type (x
+ * itself when that is contiguous). Pair i of every head is turned by freq_scale * pos[axis(i)] *
+ * freq_base^(-2 step(i) / n_dims), cosine and sine times attn_factor, the angle formed in 64 bits:
+ *   MROPE, IMROPE  pairs (i, i + n_dims/2), i < n_dims/2, step(i) = i; values past n_dims are copied
+ *   VISION         pairs (i, i + n_dims), i < n_dims = head_dim/2, step(i) counted from the start of
+ *                  the section i lies in
+ * sections count pairs; sector(i) = i % their sum. MROPE, VISION: axis(i) is the section sector(i)
+ * lies in. IMROPE: axis(i) = sector % 3 while sector < 3 * sections[axis], else 3. Without YaRN
+ * extrapolation and frequency factors. Strides that are no multiple of the element, head_dim > 4096
+ * or more than 1024 pairs return B200_E_UNSUPPORTED. */
+int b200_rope_multi(int type, const void * x, const int64_t ne[4], const size_t nb[4], const int32_t * pos,
+                    int n_dims, int mode, const int32_t sections[4], float freq_base, float freq_scale,
+                    float attn_factor, void * dst, void * stream);
+/* dst[:, i, j, k] = src[:, idx[i, j, k], j, k]; src f32 (0), f16 (1), Q4_0 (2) or Q8_0 (8, ggml's
+ * dequantised values), dst f32 [sne[0], ine[0], ine[1], ine[2]]; an index outside src's rows records
+ * a device error and yields a zero row */
 int b200_get_rows(int src_type, const void * src, const int64_t sne[4], const size_t snb[4], const int32_t * idx,
                   const int64_t ine[4], const size_t inb[4], float * dst, int * dev_err, void * stream);
+/* SET_ROWS, a KV cache's write: dst[:, idx[i, j % ine[1], k % ine[2]], j, k] = src[:, i, j, k], src F32
+ * [n, n_rows, ..], idx I32 (26) or I64 (27) [n_rows, ..], dst a view of F32 (0), F16 (1), Q4_0 (2) or
+ * Q8_0 (8) rows with any strides (multiples of 2 bytes, 4 for F32), quantised as ggml's reference
+ * encoders do, bit for bit (n a multiple of 32 for those). Rows that no index names stay as they are; of
+ * several source rows for one destination row the last stays, as if written in order. An index outside
+ * dst's rows records a device error and its row is not written. A block that holds a NaN or an infinity
+ * is stored with a NaN scale (ggml leaves it undefined). */
+int b200_set_rows(const float * src, const int64_t sne[4], const size_t snb[4], int idx_type, const void * idx,
+                  const int64_t ine[4], const size_t inb[4], int dst_type, void * dst, const int64_t dne[4],
+                  const size_t dnb[4], int * dev_err, void * stream);
 /* element k of src (ne[0] fastest) to element k of dst, converting between f32 (0) and f16 (1)
  * (round to nearest even); dst has src's shape (any strides) or is contiguous */
 int b200_cpy(int src_type, const void * src, const int64_t sne[4], const size_t snb[4], int dst_type, void * dst,
