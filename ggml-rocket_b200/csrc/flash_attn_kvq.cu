@@ -6,10 +6,8 @@
 // with hk = h / (H / HK). A key whose mask is -inf is not read into the result, whatever its bytes
 // hold; a row whose keys are all masked is zero.
 //
-// The row kernel. A CTA takes 8 of the T * (H / HK) query rows that share a KV head, one stream and one
-// range of keys; its four warps take the range's 32-key tiles in turn, each with its own ring of
-// cp.async stages, running maximum, sum and output, so nothing but the end is shared between them.
-// Tiles whose keys are masked for all the rows are never fetched: the CTA reads its mask range first.
+// The row kernels. A warp holds 8 of the T * (H / HK) query rows that share a KV head and takes 32 keys at
+// a time, with its own running maximum, sum and output:
 //
 //   S = Q K^T     mma.sync m16n8k16, 8 keys a tile. Rows 0-7 of the A operand are the query rows'
 //                 fp16 high halves, rows 8-15 their low halves (q = hi + lo to 2^-22, scaled by a power
@@ -18,19 +16,29 @@
 //   O^T = V^T P^T the codes are the A operand (16 head dimensions x 16 keys), P times the value
 //                 scales the B operand, straight from the score fragments' layout.
 //
-// P * scale is brought into fp16's range by a power of two per tile (the tile's largest value scale)
-// and, for an f32 result, split into a high and a low half as well; for an fp16 result its rounding
-// (2^-12) stays below the result's own. Sums, maxima and outputs are fp32 throughout; a tile's output
-// sums are added to the running ones by an fp32 FMA.
+// P * scale is brought into fp16's range by a power of two per 32 keys (their largest value scale) and,
+// for an f32 result, split into a high and a low half as well; for an fp16 result its rounding (2^-12)
+// stays below the result's own. Sums, maxima and outputs are fp32 throughout; the output sums of 32
+// keys are added to the running ones by an fp32 FMA.
 //
 // Scores are in log2 units, taken relative to the largest mask value of the row in the CTA's range,
 // whose difference to a key's mask is exact in fp32 also when every mask value is fp16's lowest.
+//
+// A CTA takes one stream, one range of keys and 8 rows of each of the KV heads whose cache rows make 144
+// bytes (two heads of 128, four of 64): a producer warp brings tiles of 144 bytes x 32 or 64 keys by TMA
+// (a head's 72 or 36 bytes are no multiple of 16), four consumer warps take a head and 32 keys each. Rows
+// 144 bytes apart fall into different banks for every fragment load. Tiles whose keys are masked for all
+// the rows are never fetched: the CTA reads its mask range first. Caches TMA cannot address (heads not
+// side by side, bases or strides off 16 bytes, an odd number of heads) take the same arithmetic with
+// cp.async copies of 8 (4) bytes, of which an SM moves about one a cycle: 2.5 TB/s of cache against TMA's
+// full rate.
 //
 // With few rows the keys are split over CTAs and a second kernel joins the parts.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
 
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -43,23 +51,26 @@ namespace b200 {
 namespace {
 
 constexpr int KR_ROWS = 8;             // query rows per CTA
-constexpr int KR_WARPS = 4;
+constexpr int KR_WARPS = 4;            // that attend
 constexpr int KR_THREADS = 32 * KR_WARPS;
-constexpr int KR_TILE = 32;            // keys per tile
-constexpr int KR_STAGES = 3;
-constexpr int KR_MAX_TILES = 2048;     // tiles of a CTA's range (its list of live tiles)
+constexpr int KR_KEYS = 32;            // a warp takes at a time
+constexpr int KR_BOX = 144;            // bytes of a key's row in a TMA tile
+constexpr int KR_MAX_TILES = 1024;     // tiles of a CTA's range (its list of live tiles)
+constexpr int64_t KR_WAVES = 6;
+constexpr int64_t KR_MIN_SPLIT = 2048;   // keys of a part, where they are many
 constexpr float KR_LOG2E = 1.4426950408889634f;
 
 struct KvqArgs {
     const char* q;
     int64_t q_t, q_h, q_s;             // byte strides of q: token, head, stream
-    int q_f16;
+    int q_f16, q_vec;                  // q_vec: four values a load
     const char* k;
     int64_t k_r, k_h, k_s;             // byte strides of k: key, head, stream
     const char* v;
     int64_t v_r, v_h, v_s;
     const char* mask;                  // f16 or nullptr
     int64_t m_t, m_s;                  // byte strides: token, stream
+    int m_vec;                         // rows 16-byte aligned
     void* dst;                         // [S][T][H][D]
     int dst_f16;
     float* part;                       // [S][HK][rows][splits][D] outputs, then 3 floats a part
@@ -67,6 +78,7 @@ struct KvqArgs {
     int T, H, KV, HK, G, S;
     int splits, tiles_per_split;
     float scale, softcap;
+    int* err;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -86,9 +98,17 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same with no sum to add to.
+__device__ __forceinline__ void mma_16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // The eight 4-bit codes of a word as fp16 pairs of code - 8, exact: nibbles n0, n4 | n1, n5 | n2, n6 |
@@ -107,73 +127,189 @@ __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t (&o)[4]) {
     h = __hsub2(*reinterpret_cast<const __half2*>(&d), c72), o[3] = *reinterpret_cast<uint32_t*>(&h);
 }
 
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-    uint32_t v;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
-    return v;
+__device__ __forceinline__ uint32_t ld32(const uint8_t* p) { return *reinterpret_cast<const uint32_t*>(p); }
+__device__ __forceinline__ uint32_t ld16(const uint8_t* p) { return *reinterpret_cast<const uint16_t*>(p); }
+// two 2-byte words as the halves of one
+__device__ __forceinline__ uint32_t ld16x2(const uint8_t* lo, const uint8_t* hi) {
+    return __byte_perm(ld16(lo), ld16(hi), 0x5410);
 }
-__device__ __forceinline__ uint32_t lds16(uint32_t a) {
-    uint16_t v;
-    asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(a));
-    return v;
+__device__ __forceinline__ float2 h2f(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+    if constexpr (N == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x, w[1] = v.y;
+    }
 }
 
-template <int D>
+
+// HPB: KV heads a CTA takes; 1 with cp.async copies, 256 / D with TMA.
+template <int D, int MT, int HPB>
 struct KrCfg {
-    static constexpr int NB = D / 32;              // blocks of a head's row
-    static constexpr int CH = D / 16;              // bytes of a cp.async: nine of them make a head's row
-    static constexpr int PITCH = D == 128 ? 80 : 40;   // of a row in shared memory: the eight rows a fragment
-                                                       // load touches fall into different banks
-    static constexpr int HALF = KR_TILE * PITCH;
-    static constexpr int STAGE = 2 * HALF;         // K rows, then V rows
-    static constexpr int SCL = KR_TILE * NB * 2;   // a tile's scales (fp16), K then V
-    static constexpr int OFF_SCL = KR_STAGES * STAGE;
-    static constexpr int OFF_MSK = OFF_SCL + 2 * SCL;
-    static constexpr int WARP(int mt) { return OFF_MSK + mt * KR_TILE * 4; }
-    static constexpr int OUT = KR_ROWS * D * 4 + 2 * KR_ROWS * 4;
-    static constexpr int OFF_LIST(int mt) { return KR_WARPS * (WARP(mt) > OUT ? WARP(mt) : OUT); }
-    static constexpr int OFF_REF(int mt) { return OFF_LIST(mt) + KR_MAX_TILES * 2; }
-    static constexpr int SMEM(int mt) { return OFF_REF(mt) + KR_WARPS * KR_ROWS * 4 + 16; }
+    static constexpr bool TMA = HPB > 1;
+    static constexpr int NB = D / 32;                      // blocks of a head's row
+    static constexpr int CH = D / 16;                      // bytes of a cp.async: nine make a head's row
+    static constexpr int PARTS = KR_WARPS / HPB;           // warps that share a head
+    static constexpr int TK = KR_KEYS * PARTS;             // keys of a CTA's tile
+    static constexpr int THREADS = KR_THREADS + (TMA ? 32 : 0);
+    static constexpr int WARPS = THREADS / 32;
+    static constexpr int PITCH = TMA ? KR_BOX : D == 128 ? 80 : 40;   // of a row in shared memory: the eight
+                                                           // rows a fragment load touches fall into different banks
+    static constexpr int HALF = (TMA ? TK : KR_KEYS) * PITCH;
+    static constexpr int STAGE = 2 * HALF;                 // K rows, then V rows; of the CTA, or of a warp
+    static constexpr int STAGES = TMA ? 3 * 18432 / STAGE : 3;
+    static constexpr int RING = STAGES * STAGE * (TMA ? 1 : KR_WARPS);
+    static constexpr int SCL = KR_KEYS * NB * 2;           // the scales of 32 keys (fp16), K then V
+    static constexpr int OFF_SCL = RING;
+    static constexpr int OFF_MSK = OFF_SCL + KR_WARPS * 2 * SCL;
+    static constexpr int OFF_Q = OFF_MSK + KR_WARPS * MT * KR_KEYS * 4;
+    static constexpr int OFF_BACK = OFF_Q + HPB * 2 * NB * 512;
+    static constexpr int OFF_REF = OFF_BACK + HPB * KR_ROWS * 4;
+    static constexpr int OFF_BAR = OFF_REF + (WARPS + 1) * KR_ROWS * 4;
+    static constexpr int OFF_LIST = OFF_BAR + 16 * STAGES + 16;
+    static constexpr int SMEM = OFF_LIST + KR_MAX_TILES * 2;
+    static constexpr int OUT = (KR_ROWS * D + 2 * KR_ROWS) * 4;   // a warp's result, in the ring's place
+    static_assert(KR_WARPS * OUT <= RING && OFF_BAR % 8 == 0 && OFF_Q % 16 == 0 && HALF % 128 == 0);
 };
 
 // MT: the most tokens a CTA's rows come from (1 or 8). EXACT: f32 results (P split in two halves).
-template <int D, int MT, bool EXACT>
-__global__ void __launch_bounds__(KR_THREADS) kvq_rows_kernel(const KvqArgs a) {
-    using C = KrCfg<D>;
-    extern __shared__ __align__(16) uint8_t sm[];
-    grid_dep_wait();
-    grid_dep_launch();
+template <int D, int MT, bool EXACT, int HPB>
+__global__ void __launch_bounds__(KrCfg<D, MT, HPB>::THREADS, 3)
+kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const KvqArgs a) {
+    using C = KrCfg<D, MT, HPB>;
+    extern __shared__ __align__(128) uint8_t sm[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-    const int split = blockIdx.x, hk = blockIdx.y % a.HK, rt = blockIdx.y / a.HK, str = blockIdx.z;
+    const int packs = a.HK / HPB;
+    const int split = blockIdx.x, pack = blockIdx.y % packs, rt = blockIdx.y / packs, str = blockIdx.z;
     const int rows_all = a.T * a.G, row0 = rt * KR_ROWS;
     const int rows = min(KR_ROWS, rows_all - row0);
     const int t_first = row0 / a.G, n_tok = MT == 1 ? 1 : (row0 + rows - 1) / a.G - t_first + 1;
-    const int n_tiles = (a.KV + KR_TILE - 1) / KR_TILE;
+    const int n_tiles = (a.KV + C::TK - 1) / C::TK;
     const int tile0 = split * a.tiles_per_split, tile1 = min(n_tiles, tile0 + a.tiles_per_split);
-    uint16_t* list = reinterpret_cast<uint16_t*>(sm + C::OFF_LIST(MT));
-    float* refs = reinterpret_cast<float*>(sm + C::OFF_REF(MT));           // [warp][8]
-    int* n_live = reinterpret_cast<int*>(sm + C::OFF_REF(MT) + KR_WARPS * KR_ROWS * 4);
+    const int range = max(0, tile1 - tile0);
+    uint16_t* list = reinterpret_cast<uint16_t*>(sm + C::OFF_LIST);
+    float* refs = reinterpret_cast<float*>(sm + C::OFF_REF);               // [warp][8], then per row
+    float* backs = reinterpret_cast<float*>(sm + C::OFF_BACK);             // [head][row]
+    uint4* q_frag = reinterpret_cast<uint4*>(sm + C::OFF_Q);               // [head][k-step][lane]
+    const uint32_t bar = smem_u32(sm) + C::OFF_BAR;
+    auto full = [&](int st) { return bar + 16u * st; };
+    auto empty = [&](int st) { return bar + 16u * st + 8u; };
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + C::OFF_BAR + 16 * C::STAGES);
+    int* n_live = reinterpret_cast<int*>(sm + C::OFF_BAR + 16 * C::STAGES + 4);
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        if constexpr (C::TMA) {
+            for (int st = 0; st < C::STAGES; st++) {
+                mbar_init(full(st), 1);
+                mbar_init(empty(st), KR_WARPS);
+            }
+            fence_barrier_init();
+            tma_prefetch_desc(&tm_k);
+            tma_prefetch_desc(&tm_v);
+        }
+    }
+    grid_dep_wait();
+    grid_dep_launch();
 
-    // ---- the range's mask: live tiles and each token's largest mask value ----
+    // ---- q (warp i: head i of the CTA): high and low halves of the row, times a power of two that brings
+    // its maximum to 2^10, in shared memory for every warp of the head, a k-step at a time ----
+    if (warp < HPB) {
+        const int r = row0 + g;
+        const bool in = g < rows;
+        const int t = in ? r / a.G : 0, h = (pack * HPB + warp) * a.G + (in ? r - t * a.G : 0);
+        const char* qp = a.q + (int64_t)str * a.q_s + (int64_t)t * a.q_t + (int64_t)h * a.q_h;
+        float x[C::NB][8];
+        float amax = 0.0f;
+#pragma unroll
+        for (int b = 0; b < C::NB; b++)
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const int d = 32 * b + 4 * e + 4 * t4;   // values 32 b + {0, 16} + 4 t4 ..
+#pragma unroll
+                for (int n = 0; n < 4; n++) x[b][e + n] = 0.0f;
+                if (!in) continue;
+                if (a.q_vec) {
+                    if (a.q_f16) {
+                        const uint2 v = *reinterpret_cast<const uint2*>(qp + 2 * d);
+                        const float2 lo = h2f(v.x), hi = h2f(v.y);
+                        x[b][e] = lo.x, x[b][e + 1] = lo.y, x[b][e + 2] = hi.x, x[b][e + 3] = hi.y;
+                    } else {
+                        const float4 v = *reinterpret_cast<const float4*>(qp + 4 * d);
+                        x[b][e] = v.x, x[b][e + 1] = v.y, x[b][e + 2] = v.z, x[b][e + 3] = v.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < 4; n++)
+                        x[b][e + n] = a.q_f16 ? __half2float(reinterpret_cast<const __half*>(qp)[d + n])
+                                              : reinterpret_cast<const float*>(qp)[d + n];
+                }
+            }
+#pragma unroll
+        for (int b = 0; b < C::NB; b++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[b][e]));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        int ex = 0;
+        if (amax > 0.0f && amax <= 3.402823466e38f) frexpf(amax, &ex);
+        ex = max(-100, ex - 10);
+        const float mul = ldexpf(1.0f, -ex);
+        if (t4 == 0) backs[warp * KR_ROWS + g] = ldexpf(a.scale, ex);   // what undoes it, with the scale
+#pragma unroll
+        for (int b = 0; b < C::NB; b++)
+#pragma unroll
+            for (int st = 0; st < 2; st++) {             // k-step 2b + st: values 16 st + {0, 2}, then {1, 3}
+                float hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float v = x[b][4 * st + e] * mul;
+                    hi[e] = __half2float(__float2half_rn(v));
+                    lo[e] = v - hi[e];
+                }
+                q_frag[(warp * 2 * C::NB + 2 * b + st) * 32 + lane] =
+                    make_uint4(pack_half2(hi[0], hi[2]), pack_half2(lo[0], lo[2]), pack_half2(hi[1], hi[3]),
+                               pack_half2(lo[1], lo[3]));
+            }
+    }
+
+    // ---- the range's mask: live tiles and each token's largest mask value; eight keys a lane where the
+    // mask's rows are 16-byte aligned ----
     const char* mbase = a.mask ? a.mask + (int64_t)str * a.m_s + (int64_t)t_first * a.m_t : nullptr;
-    float ref = 0.0f;                                    // of this lane's row (g)
-    const int my_tok = MT == 1 ? 0 : min(row0 + g, rows_all - 1) / a.G - t_first;
     if (mbase) {
         float top[MT];
 #pragma unroll
         for (int k = 0; k < MT; k++) top[k] = -INFINITY;
-        for (int i = tile0 + warp; i < tile1; i += KR_WARPS) {
-            const int key = i * KR_TILE + lane;
+        constexpr int LT = C::TK / 8, PER = 32 / LT;     // lanes of a tile, tiles of a load
+        for (int i = PER * warp; i < range; i += PER * C::WARPS) {
+            const int key = (tile0 + i) * C::TK + 8 * lane;
             bool any = false;
 #pragma unroll
             for (int k = 0; k < MT; k++) {
-                if (k >= n_tok || key >= a.KV) continue;
-                const float m = __half2float(*reinterpret_cast<const __half*>(mbase + k * a.m_t + 2 * (int64_t)key));
-                any |= !(m == -INFINITY);
-                top[k] = fmaxf(top[k], m);
+                if (k >= n_tok || i + lane / LT >= range) continue;
+                const uint16_t* mp = reinterpret_cast<const uint16_t*>(mbase + k * a.m_t) + key;
+                uint32_t w[4] = {0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u};
+                if (a.m_vec && key + 8 <= a.KV) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(mp);
+                    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+                } else {
+#pragma unroll
+                    for (int n = 0; n < 8; n++)
+                        if (key + n < a.KV)
+                            w[n >> 1] = (w[n >> 1] & (n & 1 ? 0x0000ffffu : 0xffff0000u)) | ((uint32_t)mp[n] << (16 * (n & 1)));
+                }
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    any |= w[n] != 0xfc00fc00u;
+                    const float2 f = h2f(w[n]);
+                    top[k] = fmaxf(top[k], fmaxf(f.x, f.y));
+                }
             }
-            const bool on = __any_sync(0xffffffffu, any);
-            if (lane == 0) list[i - tile0] = on ? 1 : 0;
+            const uint32_t votes = __ballot_sync(0xffffffffu, any);
+            if (lane < PER && i + lane < range) list[i + lane] = (votes >> (LT * lane)) & ((1u << LT) - 1u) ? 1 : 0;
         }
 #pragma unroll
         for (int k = 0; k < MT; k++) {
@@ -181,16 +317,25 @@ __global__ void __launch_bounds__(KR_THREADS) kvq_rows_kernel(const KvqArgs a) {
             for (int o = 16; o > 0; o >>= 1) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
             if (lane == 0) refs[warp * KR_ROWS + k] = top[k];
         }
-        __syncthreads();
-        ref = -INFINITY;
+    }
+    __syncthreads();
+    float ref_of[MT];                                    // the largest mask value, per token
 #pragma unroll
-        for (int w = 0; w < KR_WARPS; w++) ref = fmaxf(ref, refs[w * KR_ROWS + my_tok]);
-        if (!(fabsf(ref) <= 65504.0f)) ref = 0.0f;       // all masked (or an infinite mask): nothing to gain
-        if (warp == 0) {                                 // the live tiles in order, in place
+    for (int k = 0; k < MT; k++) {
+        float r = -INFINITY;
+        if (mbase && k < n_tok)
+#pragma unroll
+            for (int w = 0; w < C::WARPS; w++) r = fmaxf(r, refs[w * KR_ROWS + k]);
+        ref_of[k] = fabsf(r) <= 65504.0f ? r : 0.0f;     // all masked (or an infinite mask): nothing to gain
+    }
+    const int my_tok = MT == 1 ? 0 : min(row0 + g, rows_all - 1) / a.G - t_first;   // of this lane's row (g)
+    float* row_ref = refs + C::WARPS * KR_ROWS;
+    if (mbase) {
+        if (warp == C::WARPS - 1) {                      // the live tiles in order, in place
             int n = 0;
-            for (int i0 = 0; i0 < tile1 - tile0; i0 += 32) {
+            for (int i0 = 0; i0 < range; i0 += 32) {
                 const int i = i0 + lane;
-                const bool on = i < tile1 - tile0 && list[i] != 0;
+                const bool on = i < range && list[i] != 0;
                 const uint32_t votes = __ballot_sync(0xffffffffu, on);
                 if (on) list[n + __popc(votes & ((1u << lane) - 1u))] = (uint16_t)i;
                 n += __popc(votes);
@@ -199,81 +344,89 @@ __global__ void __launch_bounds__(KR_THREADS) kvq_rows_kernel(const KvqArgs a) {
             if (lane == 0) *n_live = n;
         }
     } else {
-        for (int i = threadIdx.x; i < tile1 - tile0; i += KR_THREADS) list[i] = (uint16_t)i;
-        if (threadIdx.x == 0) *n_live = max(0, tile1 - tile0);
+        for (int i = threadIdx.x; i < range; i += C::THREADS) list[i] = (uint16_t)i;
+        if (threadIdx.x == 0) *n_live = range;
+    }
+    if (warp == 0 && t4 == 0) {
+        float r = ref_of[0];
+#pragma unroll
+        for (int k = 1; k < MT; k++) r = my_tok == k ? ref_of[k] : r;
+        row_ref[g] = r;
     }
     __syncthreads();
     const int live = *n_live;
 
-    // ---- q: high and low halves of the row, times a power of two that brings its maximum to 2^10 ----
-    uint32_t qa[2 * C::NB][4];
-    float back = 1.0f;                                   // what undoes it, with the scale
-    {
-        const int r = row0 + g;
-        const bool in = g < rows;
-        const int t = in ? r / a.G : 0, h = hk * a.G + (in ? r - t * a.G : 0);
-        const char* qp = a.q + (int64_t)str * a.q_s + (int64_t)t * a.q_t + (int64_t)h * a.q_h;
-        float x[C::NB][8];
-        float amax = 0.0f;
+    if (C::TMA && warp == KR_WARPS) {
+        // ---- the producer: live tiles into the CTA's stages ----
+        if (lane == 0) {
+            bool ok = true;
+            int issued[C::STAGES];
 #pragma unroll
-        for (int b = 0; b < C::NB; b++)
+            for (int st = 0; st < C::STAGES; st++) issued[st] = -1;
+            for (int e0 = 0, ph = 0; e0 < live && ok; e0 += C::STAGES, ph ^= 1) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int d = 32 * b + 16 * (e >> 2) + 4 * t4 + (e & 3);
-                float v = 0.0f;
-                if (in) v = a.q_f16 ? __half2float(reinterpret_cast<const __half*>(qp)[d]) : reinterpret_cast<const float*>(qp)[d];
-                x[b][e] = v;
-                amax = fmaxf(amax, fabsf(v));
-            }
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        int ex = 0;
-        if (amax > 0.0f && amax <= 3.402823466e38f) frexpf(amax, &ex);
-        ex = max(-100, ex - 10);
-        const float mul = ldexpf(1.0f, -ex);
-        back = ldexpf(a.scale, ex);
-#pragma unroll
-        for (int b = 0; b < C::NB; b++)
-#pragma unroll
-            for (int s = 0; s < 2; s++) {                // k-step 2b + s: values 16 s + {0, 2}, then {1, 3}
-                float hi[4], lo[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float v = x[b][4 * s + e] * mul;
-                    hi[e] = __half2float(__float2half_rn(v));
-                    lo[e] = v - hi[e];
+                for (int st = 0; st < C::STAGES; st++) {
+                    const int e = e0 + st;
+                    if (e >= live || !ok) break;
+                    if (!mbar_wait(empty(st), (uint32_t)ph ^ 1u, a.err, ERR_WAIT_PRODUCER, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    issued[st] = ph;
+                    const int key0 = (tile0 + list[e]) * C::TK;
+                    const uint32_t d = smem_u32(sm) + st * C::STAGE;
+                    mbar_arrive_expect_tx(full(st), C::STAGE);
+                    tma_load_3d(d, &tm_k, full(st), pack * KR_BOX, key0, str);
+                    tma_load_3d(d + C::HALF, &tm_v, full(st), pack * KR_BOX, key0, str);
                 }
-                qa[2 * b + s][0] = pack_half2(hi[0], hi[2]);
-                qa[2 * b + s][1] = pack_half2(lo[0], lo[2]);
-                qa[2 * b + s][2] = pack_half2(hi[1], hi[3]);
-                qa[2 * b + s][3] = pack_half2(lo[1], lo[3]);
             }
+            // let every copy land before the CTA reuses or leaves its memory
+            bool drained = true;
+#pragma unroll
+            for (int st = 0; st < C::STAGES; st++)
+                if (issued[st] >= 0) drained &= mbar_drain(full(st), (uint32_t)issued[st]);
+            if (!drained) atomicCAS(a.err, 0, ERR_WAIT_DRAIN);
+        }
+        cta_sync();
+        cta_sync();
+        return;
     }
 
-    // ---- the warp's own stages ----
-    const uint32_t wsm = smem_u32(sm) + warp * (C::WARP(MT) > C::OUT ? C::WARP(MT) : C::OUT);
-    const int c_row = lane / 9, c_chunk = lane - 9 * c_row;   // lanes 0-26: three rows of nine pieces
-    const char* kp = a.k + (int64_t)str * a.k_s + (int64_t)hk * a.k_h + c_chunk * C::CH;
-    const char* vp = a.v + (int64_t)str * a.v_s + (int64_t)hk * a.v_h + c_chunk * C::CH;
-    auto fetch = [&](int i) {                                 // the i-th live tile of this warp
-        const int e = warp + i * KR_WARPS;
+    // ---- a warp's 32 keys of every live tile ----
+    const int hs = warp % HPB, part = warp / HPB;        // its head of the CTA's, its keys of the tile's
+    const float back = backs[hs * KR_ROWS + g], back2 = back * KR_LOG2E;
+    const uint4* qs = q_frag + hs * 2 * C::NB * 32;
+    uint8_t* ring = sm + (C::TMA ? 0 : warp * C::STAGES * C::STAGE);
+    uint8_t* scl = sm + C::OFF_SCL + warp * 2 * C::SCL;
+    float* msk = reinterpret_cast<float*>(sm + C::OFF_MSK) + warp * MT * KR_KEYS;
+
+    const int c_row = lane / 9, c_chunk = lane - 9 * c_row;   // cp.async: lanes 0-26, three rows of nine pieces
+    const char* kp = a.k + (int64_t)str * a.k_s + (int64_t)pack * a.k_h + c_row * a.k_r + c_chunk * C::CH;
+    const char* vp = a.v + (int64_t)str * a.v_s + (int64_t)pack * a.v_h + c_row * a.v_r + c_chunk * C::CH;
+    const uint32_t c_dst = smem_u32(ring) + c_row * C::PITCH + c_chunk * C::CH;
+    auto fetch = [&](int e, int st) {                         // the warp's keys of live tile e into a stage
         if (e < live && lane < 27) {
-            const int key0 = (tile0 + list[e]) * KR_TILE;
-            const uint32_t d = wsm + (i % KR_STAGES) * C::STAGE + c_row * C::PITCH + c_chunk * C::CH;
+            const int key0 = (tile0 + list[e]) * C::TK + part * KR_KEYS;
+            const uint32_t d = c_dst + st * C::STAGE;
+            const char* ks = kp + key0 * a.k_r;
+            const char* vs = vp + key0 * a.v_r;
 #pragma unroll
             for (int n = 0; n < 11; n++) {
                 const int row = 3 * n + c_row;
-                if (n == 10 && row >= KR_TILE) break;
-                const bool in = key0 + row < a.KV;
-                const int64_t key = in ? key0 + row : a.KV - 1;
-                cp_async<C::CH>(d + 3 * n * C::PITCH, kp + key * a.k_r, in);
-                cp_async<C::CH>(d + 3 * n * C::PITCH + C::HALF, vp + key * a.v_r, in);
+                if (row >= KR_KEYS) break;
+                const bool in = key0 + row < a.KV;       // rows behind the last key as zeros
+                cp_async<C::CH>(d + 3 * n * C::PITCH, in ? ks : a.k, in);
+                cp_async<C::CH>(d + 3 * n * C::PITCH + C::HALF, in ? vs : a.v, in);
+                ks += 3 * a.k_r;
+                vs += 3 * a.v_r;
             }
         }
         cp_async_commit();
     };
+    if constexpr (!C::TMA) {
 #pragma unroll
-    for (int i = 0; i < KR_STAGES - 1; i++) fetch(i);
+        for (int i = 0; i < C::STAGES - 1; i++) fetch(i, i);
+    }
 
     float o[2 * C::NB][4];
 #pragma unroll
@@ -282,99 +435,108 @@ __global__ void __launch_bounds__(KR_THREADS) kvq_rows_kernel(const KvqArgs a) {
         for (int e = 0; e < 4; e++) o[m][e] = 0.0f;
     float run_max = -INFINITY, run_sum = 0.0f;           // of row g (the sum: this lane's keys)
     int unit = 0;                                        // o is in units of 2^unit
-    const uint32_t scl = wsm + C::OFF_SCL, msk = wsm + C::OFF_MSK;
 
-    for (int i = 0; warp + i * KR_WARPS < live; i++) {
-        const int key0 = (tile0 + list[warp + i * KR_WARPS]) * KR_TILE;
-        float mv[MT];                                    // key key0 + lane's mask, per token
-        bool seen = key0 + lane < a.KV;
-        if (mbase) {
-            bool any = false;
+    // the lane's key's mask bits in live tile e, per token; 0xfc00 (-inf) where there is no such key
+    auto load_mask = [&](int e, uint16_t (&m)[MT]) {
+        const int key = e < live ? (tile0 + list[e]) * C::TK + part * KR_KEYS + lane : a.KV;
 #pragma unroll
-            for (int k = 0; k < MT; k++) {
-                mv[k] = -INFINITY;
-                if (k < n_tok && seen)
-                    mv[k] = __half2float(*reinterpret_cast<const __half*>(mbase + k * a.m_t + 2 * (int64_t)(key0 + lane)));
-                any |= !(mv[k] == -INFINITY);
-            }
-            seen = any;
-        } else {
-#pragma unroll
-            for (int k = 0; k < MT; k++) mv[k] = seen ? 0.0f : -INFINITY;
+        for (int k = 0; k < MT; k++) {
+            m[k] = key < a.KV ? 0 : 0xfc00;
+            if (mbase && key < a.KV && k < n_tok) m[k] = *reinterpret_cast<const uint16_t*>(mbase + k * a.m_t + 2 * (int64_t)key);
         }
-        cp_async_wait<KR_STAGES - 2>();
+    };
+    uint16_t mnext[MT];
+    load_mask(0, mnext);
+
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int e = 0; e < live; e++) {
+        bool seen = false;
+#pragma unroll
+        for (int k = 0; k < MT; k++) {
+            if (k >= n_tok) continue;
+            seen |= mnext[k] != 0xfc00;
+            const float m = __half2float(__ushort_as_half(mnext[k]));
+            msk[k * KR_KEYS + lane] = m == -INFINITY ? m : (m - ref_of[k]) * KR_LOG2E;
+        }
+        load_mask(e + 1, mnext);
+        const uint8_t *ks, *vs;
+        if constexpr (C::TMA) {
+            if (!mbar_wait(full(stage), phase, a.err, ERR_WAIT_STREAM, abort_flag)) break;
+            ks = ring + stage * C::STAGE + part * KR_KEYS * C::PITCH + hs * (18 * C::NB);
+        } else {
+            cp_async_wait<C::STAGES - 2>();
+            ks = ring + stage * C::STAGE;
+        }
+        vs = ks + C::HALF;
         __syncwarp();
-        const uint32_t ks = wsm + (i % KR_STAGES) * C::STAGE, vs = ks + C::HALF;
         // the scales of key `lane`, apart from the codes; a key no row sees gets zeros
         uint32_t dk[C::NB / 2], dv[C::NB / 2];
         float vmax = 0.0f;
 #pragma unroll
         for (int p = 0; p < C::NB / 2; p++) {
-            const uint32_t rk = ks + lane * C::PITCH + 36 * p, rv = vs + lane * C::PITCH + 36 * p;
-            dk[p] = lds16(rk) | (lds16(rk + 18) << 16);
-            dv[p] = lds16(rv) | (lds16(rv + 18) << 16);
-            if (!seen) dk[p] = dv[p] = 0;
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&dv[p]));
-            vmax = fmaxf(vmax, fmaxf(fabsf(f.x), fabsf(f.y)));
+            const uint8_t* rk = ks + lane * C::PITCH + 36 * p;
+            const uint8_t* rv = vs + lane * C::PITCH + 36 * p;
+            dk[p] = seen ? ld16x2(rk, rk + 18) : 0u;
+            dv[p] = seen ? ld16x2(rv, rv + 18) : 0u;
+            const float2 f = h2f(dv[p] & 0x7fff7fffu);
+            vmax = fmaxf(vmax, fmaxf(f.x, f.y));
         }
         if constexpr (C::NB == 4) {
-            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(scl + lane * 8), "r"(dk[0]), "r"(dk[1]) : "memory");
-            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(scl + C::SCL + lane * 8), "r"(dv[0]), "r"(dv[1]) : "memory");
+            *reinterpret_cast<uint2*>(scl + lane * 8) = make_uint2(dk[0], dk[1]);
+            *reinterpret_cast<uint2*>(scl + C::SCL + lane * 8) = make_uint2(dv[0], dv[1]);
         } else {
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(scl + lane * 4), "r"(dk[0]) : "memory");
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(scl + C::SCL + lane * 4), "r"(dv[0]) : "memory");
+            *reinterpret_cast<uint32_t*>(scl + lane * 4) = dk[0];
+            *reinterpret_cast<uint32_t*>(scl + C::SCL + lane * 4) = dv[0];
         }
-#pragma unroll
-        for (int k = 0; k < MT; k++)
-            if (k < n_tok)
-                asm volatile("st.shared.b32 [%0], %1;" ::"r"(msk + (k * KR_TILE + lane) * 4), "f"(mv[k]) : "memory");
-        // the power of two that brings the tile's largest value scale to at most 2^11
+        // the power of two that brings the tile's largest value scale to [2^10, 2^11)
         const uint32_t vbits = __reduce_max_sync(0xffffffffu, __float_as_uint(vmax));
         int vexp = (int)(vbits >> 23) - 127 - 10;
-        if (vbits == 0 || vbits >= 0x7f800000u) vexp = 0;
+        if (vbits == 0 || vbits >= 0x7f800000u) vexp = unit;
         const float vmul = __uint_as_float((uint32_t)(127 - vexp) << 23);
         __syncwarp();
 
-        // ---- S = Q K^T ----
+        // ---- S = Q K^T: a block of 32 values at a time, four 8-key columns side by side ----
         float s[4][2];
+        uint32_t dd[4][C::NB];                           // scales of keys 8j + 2 t4 and + 1
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            float s0 = 0.0f, s1 = 0.0f;
-            uint32_t dd[C::NB];                          // scales of keys 8j + 2 t4 and + 1
-            const uint32_t da = scl + (8 * j + 2 * t4) * (C::NB * 2);
-            if constexpr (C::NB == 4)
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(dd[0]), "=r"(dd[1]), "=r"(dd[2]), "=r"(dd[3]) : "r"(da));
-            else
-                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(dd[0]), "=r"(dd[1]) : "r"(da));
-            const uint32_t kr = ks + (8 * j + g) * C::PITCH + 4 * t4;
+            s[j][0] = s[j][1] = 0.0f;
+            load_words(scl + (8 * j + 2 * t4) * (C::NB * 2), dd[j]);
+        }
 #pragma unroll
-            for (int p = 0; p < C::NB / 2; p++) {
-                const float2 e0 = __half22float2(*reinterpret_cast<const __half2*>(&dd[p]));
-                const float2 e1 = __half22float2(*reinterpret_cast<const __half2*>(&dd[C::NB / 2 + p]));
-                const uint32_t w0 = lds32(kr + 36 * p), w1 = lds32(kr + 36 * p + 4), w2 = lds32(kr + 36 * p + 20);
+        for (int b = 0; b < C::NB; b++) {
+            const uint4 qa = qs[(2 * b) * 32 + lane], qb = qs[(2 * b + 1) * 32 + lane];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint8_t* kr = ks + (8 * j + g) * C::PITCH + 4 * t4 + 36 * (b >> 1);
+                // a block of even number starts two bytes into a word
+                const uint32_t w = (b & 1) ? ld32(kr + 20) : __byte_perm(ld32(kr), ld32(kr + 4), 0x5432);
                 uint32_t f[4];
-                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                codes_f16(__byte_perm(w0, w1, 0x5432), f);
-                mma_16816(c, qa[4 * p][0], qa[4 * p][1], qa[4 * p][2], qa[4 * p][3], f[0], f[2]);
-                mma_16816(c, qa[4 * p + 1][0], qa[4 * p + 1][1], qa[4 * p + 1][2], qa[4 * p + 1][3], f[1], f[3]);
-                s0 = fmaf(e0.x, c[0] + c[2], s0);
-                s1 = fmaf(e1.x, c[1] + c[3], s1);
-                float c2[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                codes_f16(w2, f);
-                mma_16816(c2, qa[4 * p + 2][0], qa[4 * p + 2][1], qa[4 * p + 2][2], qa[4 * p + 2][3], f[0], f[2]);
-                mma_16816(c2, qa[4 * p + 3][0], qa[4 * p + 3][1], qa[4 * p + 3][2], qa[4 * p + 3][3], f[1], f[3]);
-                s0 = fmaf(e0.y, c2[0] + c2[2], s0);
-                s1 = fmaf(e1.y, c2[1] + c2[3], s1);
+                float c[4];
+                codes_f16(w, f);
+                mma_16816_first(c, qa.x, qa.y, qa.z, qa.w, f[0], f[2]);
+                mma_16816(c, qb.x, qb.y, qb.z, qb.w, f[1], f[3]);
+                const float2 e0 = h2f(dd[j][b >> 1]), e1 = h2f(dd[j][C::NB / 2 + (b >> 1)]);
+                s[j][0] = fmaf((b & 1) ? e0.y : e0.x, c[0] + c[2], s[j][0]);
+                s[j][1] = fmaf((b & 1) ? e1.y : e1.x, c[1] + c[3], s[j][1]);
             }
-            s0 *= back, s1 *= back;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 m = *reinterpret_cast<const float2*>(msk + my_tok * KR_KEYS + 8 * j + 2 * t4);
             if (a.softcap != 0.0f) {
-                s0 = a.softcap * tanhf(s0 / a.softcap);
-                s1 = a.softcap * tanhf(s1 / a.softcap);
+                s[j][0] = a.softcap * KR_LOG2E * tanhf(s[j][0] * back / a.softcap) + m.x;
+                s[j][1] = a.softcap * KR_LOG2E * tanhf(s[j][1] * back / a.softcap) + m.y;
+            } else {
+                s[j][0] = fmaf(s[j][0], back2, m.x);
+                s[j][1] = fmaf(s[j][1], back2, m.y);
             }
-            float m0, m1;
-            asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(m0), "=f"(m1) : "r"(msk + (my_tok * KR_TILE + 8 * j + 2 * t4) * 4));
-            s[j][0] = m0 == -INFINITY ? -INFINITY : (s0 + (m0 - ref)) * KR_LOG2E;
-            s[j][1] = m1 == -INFINITY ? -INFINITY : (s1 + (m1 - ref)) * KR_LOG2E;
+            // K's scales were zeroed where no row sees the key; one that other rows see may still give no number
+            if constexpr (MT > 1) {
+                s[j][0] = m.x == -INFINITY ? -INFINITY : s[j][0];
+                s[j][1] = m.y == -INFINITY ? -INFINITY : s[j][1];
+            }
         }
 
         // ---- running maximum and sum ----
@@ -396,79 +558,80 @@ __global__ void __launch_bounds__(KR_THREADS) kvq_rows_kernel(const KvqArgs a) {
         }
         run_sum = fmaf(run_sum, alpha, sum);
 
-        // ---- O^T = V^T P^T over the tile ----
-        float ot[2 * C::NB][4];
-#pragma unroll
-        for (int m = 0; m < 2 * C::NB; m++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) ot[m][e] = 0.0f;
-#pragma unroll
-        for (int jj = 0; jj < 2; jj++) {
-            uint32_t da[C::NB], db[C::NB];               // value scales of keys 16 jj + 2 t4, + 1 and those 8 on
-            const uint32_t dp = scl + C::SCL + (16 * jj + 2 * t4) * (C::NB * 2);
-            if constexpr (C::NB == 4) {
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(da[0]), "=r"(da[1]), "=r"(da[2]), "=r"(da[3]) : "r"(dp));
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(db[0]), "=r"(db[1]), "=r"(db[2]), "=r"(db[3]) : "r"(dp + 8 * C::NB * 2));
-            } else {
-                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(da[0]), "=r"(da[1]) : "r"(dp));
-                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(db[0]), "=r"(db[1]) : "r"(dp + 8 * C::NB * 2));
-            }
-            float pv[4] = {s[2 * jj][0] * vmul, s[2 * jj][1] * vmul, s[2 * jj + 1][0] * vmul, s[2 * jj + 1][1] * vmul};
-            const uint32_t vr = vs + (16 * jj + 2 * t4) * C::PITCH + 2 + 2 * g;
-#pragma unroll
-            for (int b = 0; b < C::NB; b++) {
-                const int p = b >> 1;
-                const float2 x0 = __half22float2(*reinterpret_cast<const __half2*>(&da[p]));
-                const float2 x1 = __half22float2(*reinterpret_cast<const __half2*>(&da[C::NB / 2 + p]));
-                const float2 x2 = __half22float2(*reinterpret_cast<const __half2*>(&db[p]));
-                const float2 x3 = __half22float2(*reinterpret_cast<const __half2*>(&db[C::NB / 2 + p]));
-                float w[4] = {pv[0] * ((b & 1) ? x0.y : x0.x), pv[1] * ((b & 1) ? x1.y : x1.x),
-                              pv[2] * ((b & 1) ? x2.y : x2.x), pv[3] * ((b & 1) ? x3.y : x3.x)};
-                if constexpr (MT > 1) {                  // a key other rows see: its scale may be no number
-#pragma unroll
-                    for (int e = 0; e < 4; e++) w[e] = pv[e] == 0.0f ? 0.0f : w[e];
-                }
-                const uint32_t b0 = pack_half2(w[0], w[1]), b1 = pack_half2(w[2], w[3]);
-                const uint32_t va = vr + 18 * b;
-                const uint32_t y0 = lds16(va) | (lds16(va + C::PITCH) << 16);
-                const uint32_t y1 = lds16(va + 8 * C::PITCH) | (lds16(va + 9 * C::PITCH) << 16);
-                uint32_t f0[4], f1[4];                   // {2g, 16 + 2g, 2g + 1, 17 + 2g} of the block, key pairs
-                codes_f16(y0, f0);
-                codes_f16(y1, f1);
-                mma_16816(ot[2 * b], f0[0], f0[1], f1[0], f1[1], b0, b1);
-                mma_16816(ot[2 * b + 1], f0[2], f0[3], f1[2], f1[3], b0, b1);
-                if constexpr (EXACT) {
-                    const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&b0));
-                    const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&b1));
-                    const uint32_t l0 = pack_half2(w[0] - h0.x, w[1] - h0.y), l1 = pack_half2(w[2] - h1.x, w[3] - h1.y);
-                    mma_16816(ot[2 * b], f0[0], f0[1], f1[0], f1[1], l0, l1);
-                    mma_16816(ot[2 * b + 1], f0[2], f0[3], f1[2], f1[3], l0, l1);
-                }
-            }
-        }
-        // columns 2 t4 and 2 t4 + 1 of o are those query rows: their alpha, and the change of unit
-        const float f = ldexpf(1.0f, max(-126, min(126, unit - vexp)));
+        // ---- O^T = V^T P^T over the tile, a block of 32 values at a time ----
+        // columns 2 t4 and 2 t4 + 1 of o are those query rows: their alpha, and the change of unit (scales
+        // are fp16 numbers, so units lie in [-34, 5])
+        const float f = __uint_as_float((uint32_t)(127 + unit - vexp) << 23);
         unit = vexp;
         const float al0 = __shfl_sync(0xffffffffu, alpha, 8 * t4) * f;
         const float al1 = __shfl_sync(0xffffffffu, alpha, 8 * t4 + 4) * f;
+        uint32_t dw[4][C::NB];                           // value scales of keys 8j + 2 t4 and + 1
 #pragma unroll
-        for (int m = 0; m < 2 * C::NB; m++) {
-            o[m][0] = fmaf(o[m][0], al0, ot[m][0]);
-            o[m][1] = fmaf(o[m][1], al1, ot[m][1]);
-            o[m][2] = fmaf(o[m][2], al0, ot[m][2]);
-            o[m][3] = fmaf(o[m][3], al1, ot[m][3]);
+        for (int j = 0; j < 4; j++) {
+            load_words(scl + C::SCL + (8 * j + 2 * t4) * (C::NB * 2), dw[j]);
+            s[j][0] *= vmul, s[j][1] *= vmul;
         }
-        __syncwarp();                                    // the stage and the scales are free again
-        fetch(i + KR_STAGES - 1);
+#pragma unroll
+        for (int b = 0; b < C::NB; b++) {
+            float ot[2][4];
+#pragma unroll
+            for (int jj = 0; jj < 2; jj++) {
+                uint32_t ph[2], pl[2];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const int j = 2 * jj + k;
+                    const float2 x0 = h2f(dw[j][b >> 1]), x1 = h2f(dw[j][C::NB / 2 + (b >> 1)]);
+                    float w0 = s[j][0] * ((b & 1) ? x0.y : x0.x), w1 = s[j][1] * ((b & 1) ? x1.y : x1.x);
+                    if constexpr (MT > 1) {              // a key other rows see: its scale may be no number
+                        w0 = s[j][0] == 0.0f ? 0.0f : w0;
+                        w1 = s[j][1] == 0.0f ? 0.0f : w1;
+                    }
+                    ph[k] = pack_half2(w0, w1);
+                    if constexpr (EXACT) {
+                        const float2 h = h2f(ph[k]);
+                        pl[k] = pack_half2(w0 - h.x, w1 - h.y);
+                    }
+                }
+                const uint8_t* va = vs + (16 * jj + 2 * t4) * C::PITCH + 2 + 2 * g + 18 * b;
+                uint32_t f0[4], f1[4];                   // {2g, 16 + 2g, 2g + 1, 17 + 2g} of the block, key pairs
+                codes_f16(ld16x2(va, va + C::PITCH), f0);
+                codes_f16(ld16x2(va + 8 * C::PITCH, va + 9 * C::PITCH), f1);
+                if (jj == 0) {
+                    mma_16816_first(ot[0], f0[0], f0[1], f1[0], f1[1], ph[0], ph[1]);
+                    mma_16816_first(ot[1], f0[2], f0[3], f1[2], f1[3], ph[0], ph[1]);
+                } else {
+                    mma_16816(ot[0], f0[0], f0[1], f1[0], f1[1], ph[0], ph[1]);
+                    mma_16816(ot[1], f0[2], f0[3], f1[2], f1[3], ph[0], ph[1]);
+                }
+                if constexpr (EXACT) {
+                    mma_16816(ot[0], f0[0], f0[1], f1[0], f1[1], pl[0], pl[1]);
+                    mma_16816(ot[1], f0[2], f0[3], f1[2], f1[3], pl[0], pl[1]);
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                o[2 * b + m][0] = fmaf(o[2 * b + m][0], al0, ot[m][0]);
+                o[2 * b + m][1] = fmaf(o[2 * b + m][1], al1, ot[m][1]);
+                o[2 * b + m][2] = fmaf(o[2 * b + m][2], al0, ot[m][2]);
+                o[2 * b + m][3] = fmaf(o[2 * b + m][3], al1, ot[m][3]);
+            }
+        }
+        __syncwarp();                                    // the stage, the scales and the mask are free again
+        if constexpr (C::TMA) {
+            if (lane == 0) mbar_arrive(empty(stage));
+        } else {
+            fetch(e + C::STAGES - 1, stage == 0 ? C::STAGES - 1 : stage - 1);
+        }
+        if (++stage == C::STAGES) stage = 0, phase ^= 1u;
     }
-    cp_async_wait<0>();
-    __syncthreads();
+    if constexpr (!C::TMA) cp_async_wait<0>();
+    cta_sync();
 
-    // ---- join the warps ----
-    float* wout = reinterpret_cast<float*>(sm + warp * (C::WARP(MT) > C::OUT ? C::WARP(MT) : C::OUT));
+    // ---- join the warps of a head ----
+    float* wout = reinterpret_cast<float*>(sm + warp * C::OUT);
     run_sum += __shfl_xor_sync(0xffffffffu, run_sum, 1);
     run_sum += __shfl_xor_sync(0xffffffffu, run_sum, 2);
-    const float lift = ldexpf(1.0f, unit);
+    const float lift = __uint_as_float((uint32_t)(127 + unit) << 23);
 #pragma unroll
     for (int b = 0; b < C::NB; b++)
 #pragma unroll
@@ -480,96 +643,122 @@ __global__ void __launch_bounds__(KR_THREADS) kvq_rows_kernel(const KvqArgs a) {
             c[16] = o[2 * b + m][2] * lift;
             c[D + 16] = o[2 * b + m][3] * lift;
         }
-    float* wstat = wout + KR_ROWS * D;
     if (t4 == 0) {
-        wstat[g] = run_max;
-        wstat[KR_ROWS + g] = run_sum;
-        if (warp == 0) refs[g] = ref;                    // per row from here on
+        wout[KR_ROWS * D + g] = run_max;
+        wout[KR_ROWS * D + KR_ROWS + g] = run_sum;
     }
-    __syncthreads();
-    constexpr int WSTRIDE = (C::WARP(MT) > C::OUT ? C::WARP(MT) : C::OUT) / 4;
-    const float* all = reinterpret_cast<const float*>(sm);
-    for (int r = threadIdx.x / D; r < rows; r += KR_THREADS / D) {
-        const int d = threadIdx.x % D;
+    cta_sync();
+    for (int i = threadIdx.x; i < HPB * rows * D; i += KR_THREADS) {
+        const int d = i % D, r = (i / D) % rows, head = i / (D * rows);
+        const float* first = reinterpret_cast<const float*>(sm + head * C::OUT);
+        constexpr int STEP = HPB * C::OUT / 4;           // to the head's next warp
         float m = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < KR_WARPS; w++) m = fmaxf(m, all[w * WSTRIDE + KR_ROWS * D + r]);
+        for (int w = 0; w < C::PARTS; w++) m = fmaxf(m, first[w * STEP + KR_ROWS * D + r]);
         const float base = m == -INFINITY ? 0.0f : m;
         float l = 0.0f, acc = 0.0f;
 #pragma unroll
-        for (int w = 0; w < KR_WARPS; w++) {
-            const float* p = all + w * WSTRIDE;
-            const float e = ex2(p[KR_ROWS * D + r] - base);
-            l = fmaf(p[KR_ROWS * D + KR_ROWS + r], e, l);
-            acc = fmaf(p[r * D + d], e, acc);
+        for (int w = 0; w < C::PARTS; w++) {
+            const float* p = first + w * STEP;
+            const float f = ex2(p[KR_ROWS * D + r] - base);
+            l = fmaf(p[KR_ROWS * D + KR_ROWS + r], f, l);
+            acc = fmaf(p[r * D + d], f, acc);
         }
-        const int row = row0 + r, t = row / a.G, h = hk * a.G + row - t * a.G;
+        const int row = row0 + r, t = row / a.G, h = (pack * HPB + head) * a.G + row - t * a.G;
+        const int64_t at = ((int64_t)str * a.T + t) * a.H + h;
         if (a.splits == 1) {
             const float y = l == 0.0f ? 0.0f : acc / l;
-            const int64_t at = (((int64_t)str * a.T + t) * a.H + h) * D + d;
-            if (a.dst_f16) static_cast<__half*>(a.dst)[at] = __float2half_rn(y);
-            else static_cast<float*>(a.dst)[at] = y;
+            if (a.dst_f16) static_cast<__half*>(a.dst)[at * D + d] = __float2half_rn(y);
+            else static_cast<float*>(a.dst)[at * D + d] = y;
         } else {
-            const int64_t p = (((int64_t)str * a.T + t) * a.H + h) * a.splits + split;
+            const int64_t p = at * a.splits + split;
             a.part[p * D + d] = acc;
             if (d == 0) {
                 a.stat[3 * p] = m;
                 a.stat[3 * p + 1] = l;
-                a.stat[3 * p + 2] = refs[r];
+                a.stat[3 * p + 2] = row_ref[r];
             }
         }
     }
 }
 
-// Joins the parts of a row: one warp per (stream, token, head). Maxima are compared as maximum plus
-// mask reference; their differences are formed apart, where they are exact.
+// Joins the parts of a row: one CTA per (stream, token, head), its four warps taking the parts in turn.
+// Maxima are compared as maximum plus mask reference; their differences are formed apart, where they are
+// exact.
 template <int D>
 __global__ void __launch_bounds__(128) kvq_join_kernel(const float* __restrict__ part, const float* __restrict__ stat,
-                                                       int splits, int64_t n_rows, int dst_f16, void* __restrict__ dst) {
+                                                       int splits, int dst_f16, void* __restrict__ dst) {
     grid_dep_wait();
     grid_dep_launch();
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= n_rows) return;
-    const int lane = threadIdx.x & 31;
+    __shared__ float sums[4][D + 1];
+    const int64_t row = blockIdx.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float* st = stat + 3 * row * splits;
     float top = -INFINITY, m_best = 0.0f, r_best = 0.0f;
-    for (int i = 0; i < splits; i++) {
-        const float l = st[3 * i + 1], m = st[3 * i], r = st[3 * i + 2];
+    for (int i = lane; i < splits; i += 32) {
+        const float m = st[3 * i], l = st[3 * i + 1], r = st[3 * i + 2];
         const float v = m + r * KR_LOG2E;
         if (l != 0.0f && v > top) top = v, m_best = m, r_best = r;
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float v = __shfl_xor_sync(0xffffffffu, top, o), m = __shfl_xor_sync(0xffffffffu, m_best, o);
+        const float r = __shfl_xor_sync(0xffffffffu, r_best, o);
+        // equal sums of different terms: the same pair on every lane
+        if (v > top || (v == top && m > m_best)) top = v, m_best = m, r_best = r;
+    }
     constexpr int PER = D / 32;
     float acc[PER] = {}, l_all = 0.0f;
-    for (int i = 0; i < splits; i++) {
+#pragma unroll 4
+    for (int i = warp; i < splits; i += 4) {
         const float l = st[3 * i + 1];
-        if (l == 0.0f) continue;                         // no key of this part is seen
-        const float e = ex2((st[3 * i] - m_best) + (st[3 * i + 2] - r_best) * KR_LOG2E);
-        l_all = fmaf(l, e, l_all);
+        // a part with no visible key may hold anything but counts for nothing
+        const float f = l == 0.0f ? 0.0f : ex2((st[3 * i] - m_best) + (st[3 * i + 2] - r_best) * KR_LOG2E);
+        l_all = fmaf(l, f, l_all);
         const float* p = part + (row * splits + i) * D + lane * PER;
+        float x[PER];
+        if constexpr (PER == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p);
+            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+        } else {
+            const float2 v = *reinterpret_cast<const float2*>(p);
+            x[0] = v.x, x[1] = v.y;
+        }
 #pragma unroll
-        for (int k = 0; k < PER; k++) acc[k] = fmaf(p[k], e, acc[k]);
+        for (int k = 0; k < PER; k++) acc[k] = fmaf(x[k], f, acc[k]);
     }
 #pragma unroll
-    for (int k = 0; k < PER; k++) {
-        const float y = l_all == 0.0f ? 0.0f : acc[k] / l_all;
-        const int64_t at = row * D + lane * PER + k;
-        if (dst_f16) static_cast<__half*>(dst)[at] = __float2half_rn(y);
-        else static_cast<float*>(dst)[at] = y;
+    for (int k = 0; k < PER; k++) sums[warp][lane * PER + k] = acc[k];
+    if (lane == 0) sums[warp][D] = l_all;
+    __syncthreads();
+    for (int d = threadIdx.x; d < D; d += 128) {
+        const float l = (sums[0][D] + sums[1][D]) + (sums[2][D] + sums[3][D]);
+        const float x = (sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d]);
+        const float y = l == 0.0f ? 0.0f : x / l;
+        if (dst_f16) static_cast<__half*>(dst)[row * D + d] = __float2half_rn(y);
+        else static_cast<float*>(dst)[row * D + d] = y;
     }
 }
 
 struct KvqPlan {
+    int heads;                                   // KV heads a CTA takes (1: the cp.async kernel)
     int splits, tiles_per_split;
     size_t part_off, stat_off, total;
 };
 
-KvqPlan kvq_plan(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S) {
+// tma: the cache's layout lets TMA address it. The workspace covers either kernel.
+KvqPlan kvq_plan(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S, bool tma) {
     KvqPlan p{};
-    const int64_t rows = T * (H / HK), tiles = (KV + KR_TILE - 1) / KR_TILE;
-    const int64_t ctas = S * HK * ((rows + KR_ROWS - 1) / KR_ROWS);
-    const int64_t target = (int64_t)device_sm_count() * 3;   // three CTAs an SM
-    int64_t splits = std::max<int64_t>(1, target / ctas);
-    splits = std::min(splits, (tiles + KR_WARPS - 1) / KR_WARPS);
+    p.heads = tma && HK % (256 / D) == 0 ? (int)(256 / D) : 1;
+    const int64_t tk = KR_KEYS * KR_WARPS / p.heads;
+    const int64_t rows = T * (H / HK), tiles = (KV + tk - 1) / tk;
+    const int64_t ctas = S * (HK / p.heads) * ((rows + KR_ROWS - 1) / KR_ROWS);
+    // Three CTAs fit an SM. One wave of them when the keys are few; several where they are many, with at
+    // least KR_MIN_SPLIT keys each, so that streams of unequal length even out.
+    const int64_t slots = (int64_t)device_sm_count() * 3;
+    int64_t splits = std::max<int64_t>(1, slots / ctas);
+    splits = std::max(splits, std::min(KR_WAVES * slots / ctas, tiles * tk / KR_MIN_SPLIT));
+    splits = std::min(splits, tiles);
     splits = std::max(splits, (tiles + KR_MAX_TILES - 1) / KR_MAX_TILES);
     const int64_t per = (tiles + splits - 1) / splits;
     splits = (tiles + per - 1) / per;
@@ -582,32 +771,57 @@ KvqPlan kvq_plan(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_
     return p;
 }
 
-template <int D, int MT, bool EXACT>
-cudaError_t launch_rows(const KvqArgs& a, dim3 grid, cudaStream_t st) {
-    constexpr int smem = KrCfg<D>::SMEM(MT);
+// The cache as [streams][keys][bytes of a key's heads], tiles of 144 bytes x `keys`; rows behind the last
+// key read as zeros.
+bool make_cache_map(CUtensorMap* map, const void* base, int64_t row_bytes, int64_t KV, int64_t S, int64_t nb_key,
+                    int64_t nb_stream, int keys) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult qr;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) != cudaSuccess ||
+            qr != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<Encode>(p);
+    }();
+    if (!encode) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)row_bytes, (cuuint64_t)KV, (cuuint64_t)S};
+    const cuuint64_t strides[2] = {(cuuint64_t)nb_key, (cuuint64_t)nb_stream};
+    const cuuint32_t box[3] = {(cuuint32_t)KR_BOX, (cuuint32_t)keys, 1}, step[3] = {1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, int MT, bool EXACT, int HPB>
+cudaError_t launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const KvqArgs& a, dim3 grid, cudaStream_t st) {
+    using C = KrCfg<D, MT, HPB>;
     static bool set[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
-    if (dev >= 0 && dev < 64 && !set[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(kvq_rows_kernel<D, MT, EXACT>,
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (dev < 0 || dev >= 64 || !set[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kvq_rows_kernel<D, MT, EXACT, HPB>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) return e;
-        set[dev] = true;
+        if (dev >= 0 && dev < 64) set[dev] = true;
     }
-    return launch_pdl(kvq_rows_kernel<D, MT, EXACT>, grid, dim3(KR_THREADS), smem, st, a);
+    return launch_pdl(kvq_rows_kernel<D, MT, EXACT, HPB>, grid, dim3(C::THREADS), C::SMEM, st, tk, tv, a);
 }
 
-template <int D>
-cudaError_t launch_kvq(const KvqArgs& a, const KvqPlan& p, cudaStream_t st) {
+template <int D, int HPB>
+cudaError_t launch_kvq(const CUtensorMap& tk, const CUtensorMap& tv, const KvqArgs& a, cudaStream_t st) {
     const int64_t rows = (int64_t)a.T * a.G;
-    const dim3 grid((unsigned)p.splits, (unsigned)(a.HK * ((rows + KR_ROWS - 1) / KR_ROWS)), (unsigned)a.S);
+    const dim3 grid((unsigned)a.splits, (unsigned)(a.HK / HPB * ((rows + KR_ROWS - 1) / KR_ROWS)), (unsigned)a.S);
+    // one token a CTA: its mask is one row, and keys it hides are hidden from all the CTA's rows
+    const bool one = a.T == 1 || a.G % KR_ROWS == 0;
     cudaError_t e;
-    if (a.T == 1) e = a.dst_f16 ? launch_rows<D, 1, false>(a, grid, st) : launch_rows<D, 1, true>(a, grid, st);
-    else e = a.dst_f16 ? launch_rows<D, 8, false>(a, grid, st) : launch_rows<D, 8, true>(a, grid, st);
-    if (e != cudaSuccess || p.splits == 1) return e;
-    const int64_t n = (int64_t)a.S * a.T * a.H;
-    return launch_pdl(kvq_join_kernel<D>, dim3((unsigned)((n + 3) / 4)), dim3(128), 0, st, (const float*)a.part,
-                      (const float*)a.stat, p.splits, n, a.dst_f16, a.dst);
+    if (one) e = a.dst_f16 ? launch_rows<D, 1, false, HPB>(tk, tv, a, grid, st) : launch_rows<D, 1, true, HPB>(tk, tv, a, grid, st);
+    else e = a.dst_f16 ? launch_rows<D, 8, false, HPB>(tk, tv, a, grid, st) : launch_rows<D, 8, true, HPB>(tk, tv, a, grid, st);
+    if (e != cudaSuccess || a.splits == 1) return e;
+    return launch_pdl(kvq_join_kernel<D>, dim3((unsigned)((int64_t)a.S * a.T * a.H)), dim3(128), 0, st,
+                      (const float*)a.part, (const float*)a.stat, a.splits, a.dst_f16, a.dst);
 }
 
 bool kvq_dims_ok(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S) {
@@ -623,7 +837,7 @@ extern "C" {
 size_t b200_flash_attn_kvq_workspace_size(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S) {
     using namespace b200;
     if (!kvq_dims_ok(D, T, H, KV, HK, S)) return 0;
-    return kvq_plan(D, T, H, KV, HK, S).total;
+    return std::max(kvq_plan(D, T, H, KV, HK, S, true).total, kvq_plan(D, T, H, KV, HK, S, false).total);
 }
 
 int b200_flash_attn_kvq(int kv_type, int q_type, const void* q, const int64_t qne[4], const size_t qnb[4],
@@ -650,18 +864,27 @@ int b200_flash_attn_kvq(int kv_type, int q_type, const void* q, const int64_t qn
         off(dst, dst_type == 1 ? 2 : 4))
         return B200_E_UNSUPPORTED;
     if (mask && (mnb[0] != 2 || ((mnb[1] | mnb[3]) & 1) || off(mask, 2))) return B200_E_UNSUPPORTED;
-    const KvqPlan p = kvq_plan(D, T, H, KV, HK, S);
-    if (!workspace || workspace_bytes < p.total || off(workspace, 256)) return B200_E_WORKSPACE;
+    const int64_t row = D / 32 * 18;
+    // what a tensor map of the cache needs: heads side by side, 16-byte bases and strides, strides below 2^40
+    auto tma_ok = [&](const void* p, const size_t* s) {
+        return (int64_t)s[2] == row && ((s[1] | s[3]) & 15) == 0 && !off(p, 16) && (int64_t)s[1] >= HK * row &&
+               s[1] < (1ull << 40) && s[3] < (1ull << 40) && (S == 1 || s[3] > 0);
+    };
+    const KvqPlan p = kvq_plan(D, T, H, KV, HK, S, tma_ok(k, knb) && tma_ok(v, vnb));
+    if (!workspace || workspace_bytes < b200_flash_attn_kvq_workspace_size(D, T, H, KV, HK, S) || off(workspace, 256))
+        return B200_E_WORKSPACE;
     KvqArgs a{};
     a.q = static_cast<const char*>(q);
     a.q_t = (int64_t)qnb[1], a.q_h = (int64_t)qnb[2], a.q_s = (int64_t)qnb[3];
     a.q_f16 = q_type == 1;
+    a.q_vec = (qnb[1] | qnb[2] | qnb[3]) % (4 * qe) == 0 && !off(q, 4 * qe);
     a.k = static_cast<const char*>(k);
     a.k_r = (int64_t)knb[1], a.k_h = (int64_t)knb[2], a.k_s = (int64_t)knb[3];
     a.v = static_cast<const char*>(v);
     a.v_r = (int64_t)vnb[1], a.v_h = (int64_t)vnb[2], a.v_s = (int64_t)vnb[3];
     a.mask = static_cast<const char*>(mask);
     a.m_t = mask ? (int64_t)mnb[1] : 0, a.m_s = mask ? (int64_t)mnb[3] : 0;
+    a.m_vec = mask && ((mnb[1] | mnb[3]) & 15) == 0 && !off(mask, 16);
     a.dst = dst;
     a.dst_f16 = dst_type == 1;
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.part_off);
@@ -670,7 +893,19 @@ int b200_flash_attn_kvq(int kv_type, int q_type, const void* q, const int64_t qn
     a.splits = p.splits, a.tiles_per_split = p.tiles_per_split;
     a.scale = scale, a.softcap = softcap;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = D == 64 ? launch_kvq<64>(a, p, st) : launch_kvq<128>(a, p, st);
+    a.err = dev_err;
+    CUtensorMap tk{}, tv{};
+    if (p.heads > 1) {
+        const int keys = KR_KEYS * KR_WARPS / p.heads;
+        // a single stream's stride is never used but has to be one a map accepts
+        const int64_t ks = S > 1 ? (int64_t)knb[3] : 16, vs = S > 1 ? (int64_t)vnb[3] : 16;
+        if (!make_cache_map(&tk, k, HK * row, KV, S, (int64_t)knb[1], ks, keys) ||
+            !make_cache_map(&tv, v, HK * row, KV, S, (int64_t)vnb[1], vs, keys))
+            return B200_E_CUDA;
+    }
+    cudaError_t e;
+    if (D == 64) e = p.heads > 1 ? launch_kvq<64, 4>(tk, tv, a, st) : launch_kvq<64, 1>(tk, tv, a, st);
+    else e = p.heads > 1 ? launch_kvq<128, 2>(tk, tv, a, st) : launch_kvq<128, 1>(tk, tv, a, st);
     return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? B200_OK : B200_E_CUDA;
 }
 
