@@ -25,8 +25,8 @@
 // whose difference to a key's mask is exact in fp32 also when every mask value is fp16's lowest.
 //
 // A CTA takes one stream, one range of keys and 8 rows of each of the KV heads whose cache rows make 144
-// bytes (two heads of 128, four of 64): a producer warp brings tiles of 144 bytes x 32 or 64 keys by TMA
-// (a head's 72 or 36 bytes are no multiple of 16), four consumer warps take a head and 32 keys each. Rows
+// bytes (two heads of 128, four of 64): one thread brings tiles of 144 bytes x 32 or 64 keys by TMA (a
+// head's 72 or 36 bytes are no multiple of 16), four warps take a head and 32 keys each. Rows
 // 144 bytes apart fall into different banks for every fragment load. Tiles whose keys are masked for all
 // the rows are never fetched: the CTA reads its mask range first. Caches TMA cannot address (heads not
 // side by side, bases or strides off 16 bytes, an odd number of heads) take the same arithmetic with
@@ -51,7 +51,7 @@ namespace b200 {
 namespace {
 
 constexpr int KR_ROWS = 8;             // query rows per CTA
-constexpr int KR_WARPS = 4;            // that attend
+constexpr int KR_WARPS = 4;
 constexpr int KR_THREADS = 32 * KR_WARPS;
 constexpr int KR_KEYS = 32;            // a warp takes at a time
 constexpr int KR_BOX = 144;            // bytes of a key's row in a TMA tile
@@ -155,8 +155,7 @@ struct KrCfg {
     static constexpr int CH = D / 16;                      // bytes of a cp.async: nine make a head's row
     static constexpr int PARTS = KR_WARPS / HPB;           // warps that share a head
     static constexpr int TK = KR_KEYS * PARTS;             // keys of a CTA's tile
-    static constexpr int THREADS = KR_THREADS + (TMA ? 32 : 0);
-    static constexpr int WARPS = THREADS / 32;
+    static constexpr int THREADS = KR_THREADS, WARPS = KR_WARPS;
     static constexpr int PITCH = TMA ? KR_BOX : D == 128 ? 80 : 40;   // of a row in shared memory: the eight
                                                            // rows a fragment load touches fall into different banks
     static constexpr int HALF = (TMA ? TK : KR_KEYS) * PITCH;
@@ -176,11 +175,15 @@ struct KrCfg {
     static_assert(KR_WARPS * OUT <= RING && OFF_BAR % 8 == 0 && OFF_Q % 16 == 0 && HALF % 128 == 0);
 };
 
-// MT: the most tokens a CTA's rows come from (1 or 8). EXACT: f32 results (P split in two halves).
-template <int D, int MT, bool EXACT, int HPB>
+// MT: the most tokens a CTA's rows come from (1 or 8). MODE: 0 f16 q and result (q has no low half), 1 f16
+// result, 2 f32 result (P split in two halves). Leaving the codes' offsets in the MMA and starting its sums
+// from minus the offset times sum(q), sum(P) saves 24 of about 30 fp16 subtractions per key but measured
+// 2 % slower (562 against 554 us over 64 streams x 32000 keys): the subtractions use a pipe that is idle.
+template <int D, int MT, int MODE, int HPB>
 __global__ void __launch_bounds__(KrCfg<D, MT, HPB>::THREADS, 3)
 kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const KvqArgs a) {
     using C = KrCfg<D, MT, HPB>;
+    constexpr bool EXACT = MODE == 2, QLO = MODE > 0;
     extern __shared__ __align__(128) uint8_t sm[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const int packs = a.HK / HPB;
@@ -356,42 +359,6 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     __syncthreads();
     const int live = *n_live;
 
-    if (C::TMA && warp == KR_WARPS) {
-        // ---- the producer: live tiles into the CTA's stages ----
-        if (lane == 0) {
-            bool ok = true;
-            int issued[C::STAGES];
-#pragma unroll
-            for (int st = 0; st < C::STAGES; st++) issued[st] = -1;
-            for (int e0 = 0, ph = 0; e0 < live && ok; e0 += C::STAGES, ph ^= 1) {
-#pragma unroll
-                for (int st = 0; st < C::STAGES; st++) {
-                    const int e = e0 + st;
-                    if (e >= live || !ok) break;
-                    if (!mbar_wait(empty(st), (uint32_t)ph ^ 1u, a.err, ERR_WAIT_PRODUCER, abort_flag)) {
-                        ok = false;
-                        break;
-                    }
-                    issued[st] = ph;
-                    const int key0 = (tile0 + list[e]) * C::TK;
-                    const uint32_t d = smem_u32(sm) + st * C::STAGE;
-                    mbar_arrive_expect_tx(full(st), C::STAGE);
-                    tma_load_3d(d, &tm_k, full(st), pack * KR_BOX, key0, str);
-                    tma_load_3d(d + C::HALF, &tm_v, full(st), pack * KR_BOX, key0, str);
-                }
-            }
-            // let every copy land before the CTA reuses or leaves its memory
-            bool drained = true;
-#pragma unroll
-            for (int st = 0; st < C::STAGES; st++)
-                if (issued[st] >= 0) drained &= mbar_drain(full(st), (uint32_t)issued[st]);
-            if (!drained) atomicCAS(a.err, 0, ERR_WAIT_DRAIN);
-        }
-        cta_sync();
-        cta_sync();
-        return;
-    }
-
     // ---- a warp's 32 keys of every live tile ----
     const int hs = warp % HPB, part = warp / HPB;        // its head of the CTA's, its keys of the tile's
     const float back = backs[hs * KR_ROWS + g], back2 = back * KR_LOG2E;
@@ -423,7 +390,20 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         }
         cp_async_commit();
     };
-    if constexpr (!C::TMA) {
+    // TMA: one thread brings live tile e into a stage of the CTA's
+    int sent = 0;
+    auto send = [&](int st) {
+        if (sent >= live) return;
+        const int key0 = (tile0 + list[sent++]) * C::TK;
+        const uint32_t d = smem_u32(sm) + st * C::STAGE;
+        mbar_arrive_expect_tx(full(st), C::STAGE);
+        tma_load_3d(d, &tm_k, full(st), pack * KR_BOX, key0, str);
+        tma_load_3d(d + C::HALF, &tm_v, full(st), pack * KR_BOX, key0, str);
+    };
+    if constexpr (C::TMA) {
+        if (threadIdx.x == 0)
+            for (int i = 0; i < C::STAGES - 1; i++) send(i);
+    } else {
 #pragma unroll
         for (int i = 0; i < C::STAGES - 1; i++) fetch(i, i);
     }
@@ -462,6 +442,15 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         load_mask(e + 1, mnext);
         const uint8_t *ks, *vs;
         if constexpr (C::TMA) {
+            // the tile STAGES - 1 on, into the stage every warp has left behind
+            if (threadIdx.x == 0) {
+                const int prev = stage == 0 ? C::STAGES - 1 : stage - 1;
+                if (e > 0 && sent < live &&
+                    !mbar_wait(empty(prev), stage == 0 ? phase ^ 1u : phase, a.err, ERR_WAIT_PRODUCER, abort_flag))
+                    sent = live;                         // an abort: the other waits end on its flag
+                send(prev);
+            }
+            __syncwarp();
             if (!mbar_wait(full(stage), phase, a.err, ERR_WAIT_STREAM, abort_flag)) break;
             ks = ring + stage * C::STAGE + part * KR_KEYS * C::PITCH + hs * (18 * C::NB);
         } else {
@@ -518,8 +507,8 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                 mma_16816_first(c, qa.x, qa.y, qa.z, qa.w, f[0], f[2]);
                 mma_16816(c, qb.x, qb.y, qb.z, qb.w, f[1], f[3]);
                 const float2 e0 = h2f(dd[j][b >> 1]), e1 = h2f(dd[j][C::NB / 2 + (b >> 1)]);
-                s[j][0] = fmaf((b & 1) ? e0.y : e0.x, c[0] + c[2], s[j][0]);
-                s[j][1] = fmaf((b & 1) ? e1.y : e1.x, c[1] + c[3], s[j][1]);
+                s[j][0] = fmaf((b & 1) ? e0.y : e0.x, QLO ? c[0] + c[2] : c[0], s[j][0]);
+                s[j][1] = fmaf((b & 1) ? e1.y : e1.x, QLO ? c[1] + c[3] : c[1], s[j][1]);
             }
         }
 #pragma unroll
@@ -573,39 +562,35 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         }
 #pragma unroll
         for (int b = 0; b < C::NB; b++) {
+            uint32_t ph[4], pl[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float2 x0 = h2f(dw[j][b >> 1]), x1 = h2f(dw[j][C::NB / 2 + (b >> 1)]);
+                float w0 = s[j][0] * ((b & 1) ? x0.y : x0.x), w1 = s[j][1] * ((b & 1) ? x1.y : x1.x);
+                if constexpr (MT > 1) {                  // a key other rows see: its scale may be no number
+                    w0 = s[j][0] == 0.0f ? 0.0f : w0;
+                    w1 = s[j][1] == 0.0f ? 0.0f : w1;
+                }
+                ph[j] = pack_half2(w0, w1);
+                if constexpr (EXACT) {
+                    const float2 h = h2f(ph[j]);
+                    pl[j] = pack_half2(w0 - h.x, w1 - h.y);
+                }
+            }
             float ot[2][4];
 #pragma unroll
             for (int jj = 0; jj < 2; jj++) {
-                uint32_t ph[2], pl[2];
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const int j = 2 * jj + k;
-                    const float2 x0 = h2f(dw[j][b >> 1]), x1 = h2f(dw[j][C::NB / 2 + (b >> 1)]);
-                    float w0 = s[j][0] * ((b & 1) ? x0.y : x0.x), w1 = s[j][1] * ((b & 1) ? x1.y : x1.x);
-                    if constexpr (MT > 1) {              // a key other rows see: its scale may be no number
-                        w0 = s[j][0] == 0.0f ? 0.0f : w0;
-                        w1 = s[j][1] == 0.0f ? 0.0f : w1;
-                    }
-                    ph[k] = pack_half2(w0, w1);
-                    if constexpr (EXACT) {
-                        const float2 h = h2f(ph[k]);
-                        pl[k] = pack_half2(w0 - h.x, w1 - h.y);
-                    }
-                }
                 const uint8_t* va = vs + (16 * jj + 2 * t4) * C::PITCH + 2 + 2 * g + 18 * b;
+                const uint32_t y0 = ld16x2(va, va + C::PITCH), y1 = ld16x2(va + 8 * C::PITCH, va + 9 * C::PITCH);
                 uint32_t f0[4], f1[4];                   // {2g, 16 + 2g, 2g + 1, 17 + 2g} of the block, key pairs
-                codes_f16(ld16x2(va, va + C::PITCH), f0);
-                codes_f16(ld16x2(va + 8 * C::PITCH, va + 9 * C::PITCH), f1);
-                if (jj == 0) {
-                    mma_16816_first(ot[0], f0[0], f0[1], f1[0], f1[1], ph[0], ph[1]);
-                    mma_16816_first(ot[1], f0[2], f0[3], f1[2], f1[3], ph[0], ph[1]);
-                } else {
-                    mma_16816(ot[0], f0[0], f0[1], f1[0], f1[1], ph[0], ph[1]);
-                    mma_16816(ot[1], f0[2], f0[3], f1[2], f1[3], ph[0], ph[1]);
-                }
-                if constexpr (EXACT) {
-                    mma_16816(ot[0], f0[0], f0[1], f1[0], f1[1], pl[0], pl[1]);
-                    mma_16816(ot[1], f0[2], f0[3], f1[2], f1[3], pl[0], pl[1]);
+                codes_f16(y0, f0);
+                codes_f16(y1, f1);
+#pragma unroll
+                for (int m = 0; m < 2; m++) {
+                    if (jj > 0) mma_16816(ot[m], f0[2 * m], f0[2 * m + 1], f1[2 * m], f1[2 * m + 1], ph[2 * jj], ph[2 * jj + 1]);
+                    else mma_16816_first(ot[m], f0[2 * m], f0[2 * m + 1], f1[2 * m], f1[2 * m + 1], ph[0], ph[1]);
+                    if constexpr (EXACT)
+                        mma_16816(ot[m], f0[2 * m], f0[2 * m + 1], f1[2 * m], f1[2 * m + 1], pl[2 * jj], pl[2 * jj + 1]);
                 }
             }
 #pragma unroll
@@ -624,7 +609,17 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         }
         if (++stage == C::STAGES) stage = 0, phase ^= 1u;
     }
-    if constexpr (!C::TMA) cp_async_wait<0>();
+    if constexpr (C::TMA) {
+        // after an abort, let every copy land before the CTA reuses or leaves its memory
+        if (threadIdx.x == 0 && *abort_flag) {
+            bool drained = true;
+            for (int i = max(0, sent - C::STAGES); i < sent; i++)
+                drained &= mbar_drain(full(i % C::STAGES), (uint32_t)(i / C::STAGES) & 1u);
+            if (!drained) atomicCAS(a.err, 0, ERR_WAIT_DRAIN);
+        }
+    } else {
+        cp_async_wait<0>();
+    }
     cta_sync();
 
     // ---- join the warps of a head ----
@@ -795,19 +790,19 @@ bool make_cache_map(CUtensorMap* map, const void* base, int64_t row_bytes, int64
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, int MT, bool EXACT, int HPB>
+template <int D, int MT, int MODE, int HPB>
 cudaError_t launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const KvqArgs& a, dim3 grid, cudaStream_t st) {
     using C = KrCfg<D, MT, HPB>;
     static bool set[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !set[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(kvq_rows_kernel<D, MT, EXACT, HPB>,
+        const cudaError_t e = cudaFuncSetAttribute(kvq_rows_kernel<D, MT, MODE, HPB>,
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) set[dev] = true;
     }
-    return launch_pdl(kvq_rows_kernel<D, MT, EXACT, HPB>, grid, dim3(C::THREADS), C::SMEM, st, tk, tv, a);
+    return launch_pdl(kvq_rows_kernel<D, MT, MODE, HPB>, grid, dim3(C::THREADS), C::SMEM, st, tk, tv, a);
 }
 
 template <int D, int HPB>
@@ -816,9 +811,14 @@ cudaError_t launch_kvq(const CUtensorMap& tk, const CUtensorMap& tv, const KvqAr
     const dim3 grid((unsigned)a.splits, (unsigned)(a.HK / HPB * ((rows + KR_ROWS - 1) / KR_ROWS)), (unsigned)a.S);
     // one token a CTA: its mask is one row, and keys it hides are hidden from all the CTA's rows
     const bool one = a.T == 1 || a.G % KR_ROWS == 0;
+    const int mode = a.dst_f16 ? (a.q_f16 ? 0 : 1) : 2;
     cudaError_t e;
-    if (one) e = a.dst_f16 ? launch_rows<D, 1, false, HPB>(tk, tv, a, grid, st) : launch_rows<D, 1, true, HPB>(tk, tv, a, grid, st);
-    else e = a.dst_f16 ? launch_rows<D, 8, false, HPB>(tk, tv, a, grid, st) : launch_rows<D, 8, true, HPB>(tk, tv, a, grid, st);
+    if (one)
+        e = mode == 0 ? launch_rows<D, 1, 0, HPB>(tk, tv, a, grid, st)
+          : mode == 1 ? launch_rows<D, 1, 1, HPB>(tk, tv, a, grid, st) : launch_rows<D, 1, 2, HPB>(tk, tv, a, grid, st);
+    else
+        e = mode == 0 ? launch_rows<D, 8, 0, HPB>(tk, tv, a, grid, st)
+          : mode == 1 ? launch_rows<D, 8, 1, HPB>(tk, tv, a, grid, st) : launch_rows<D, 8, 2, HPB>(tk, tv, a, grid, st);
     if (e != cudaSuccess || a.splits == 1) return e;
     return launch_pdl(kvq_join_kernel<D>, dim3((unsigned)((int64_t)a.S * a.T * a.H)), dim3(128), 0, st,
                       (const float*)a.part, (const float*)a.stat, a.splits, a.dst_f16, a.dst);
