@@ -47,6 +47,13 @@ struct FaArgs {
     int T, H, KV, HK, GP, TQ, n_hg, n_tb, n_kvb;
     float softcap;
     int* err;
+    // the extended form only (several streams, parts of the keys, f16 results; q16 not scaled)
+    int64_t m_stream;          // mask stride of a stream, elements
+    float scale;
+    int splits, kvb_per_split;
+    int dst_f16;
+    float* part;               // [S][T][H][splits][DV] outputs not divided by their sums (splits > 1)
+    float* stat;               // {max in log2 units, sum, 0} of every part
 };
 
 __device__ __forceinline__ float ex2_approx(float x) {
@@ -229,7 +236,9 @@ struct FaCfg {
     static constexpr uint32_t IDESC_O = idesc_f16_f32_bmn(FA_ROWS, DV);
 };
 
-template <int D, int DV>
+// EXT: streams in blockIdx.y (heads of q16 and of K / V numbered stream by stream), a part of the keys in
+// blockIdx.z, scores scaled after the product, a key whose mask is -inf left out whatever its score.
+template <int D, int DV, bool EXT>
 __global__ void __launch_bounds__(FA_THREADS, 1)
 fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
           const __grid_constant__ CUtensorMap tmV, const FaArgs args) {
@@ -260,7 +269,10 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
     const int hg = (int)(blockIdx.x % args.n_hg);
     const int G = args.H / args.HK;
     const int hk = (hg * args.GP) / G;
-    const uint8_t* flags = args.flags + (int64_t)tb * args.n_kvb;
+    const int str = EXT ? (int)blockIdx.y : 0;
+    const uint8_t* flags = args.flags + ((int64_t)str * args.n_tb + tb) * args.n_kvb;
+    const int j_first = EXT ? (int)blockIdx.z * args.kvb_per_split : 0;
+    const int j_end = EXT ? min(args.n_kvb, j_first + args.kvb_per_split) : args.n_kvb;
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
@@ -306,11 +318,12 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
         if (lane == 0) {
             mbar_arrive_expect_tx(q_full, C::Q_BYTES);
             for (int c = 0; c < D / 64; c++)
-                tma_load_3d(sb + C::OFF_Q + c * (FA_ROWS * 128), &tmQ, q_full, c * 64, tb * args.TQ, hg * args.GP);
+                tma_load_3d(sb + C::OFF_Q + c * (FA_ROWS * 128), &tmQ, q_full, c * 64, tb * args.TQ,
+                            str * args.H + hg * args.GP);
             int i = 0;
             bool ok = true;
             int k_issued[2] = {-1, -1}, v_issued[2] = {-1, -1};
-            for (int j = 0; j < args.n_kvb && ok; j++) {
+            for (int j = j_first; j < j_end && ok; j++) {
                 if (flags[j] == MF_MASKED) continue;
                 const int s = i & 1;
                 const uint32_t ph = (uint32_t)(i >> 1) & 1u;
@@ -318,12 +331,12 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
                 k_issued[s] = (int)ph;
                 mbar_arrive_expect_tx(k_full(s), C::K_BYTES);
                 for (int c = 0; c < D / 64; c++)
-                    tma_load_3d(sb + C::OFF_K + s * C::K_BYTES + c * (FA_KB * 128), &tmK, k_full(s), c * 64, j * FA_KB, hk);
+                    tma_load_3d(sb + C::OFF_K + s * C::K_BYTES + c * (FA_KB * 128), &tmK, k_full(s), c * 64, j * FA_KB, str * args.HK + hk);
                 if (!mbar_wait(v_empty(s), ph ^ 1u, args.err, ERR_WAIT_PRODUCER, abort_flag)) { ok = false; break; }
                 v_issued[s] = (int)ph;
                 mbar_arrive_expect_tx(v_full(s), C::V_BYTES);
                 for (int c = 0; c < DV / 64; c++)
-                    tma_load_3d(sb + C::OFF_V + s * C::V_BYTES + c * (FA_KB * 128), &tmV, v_full(s), c * 64, j * FA_KB, hk);
+                    tma_load_3d(sb + C::OFF_V + s * C::V_BYTES + c * (FA_KB * 128), &tmV, v_full(s), c * 64, j * FA_KB, str * args.HK + hk);
                 i++;
             }
             if (!ok) {   // let every copy already issued land before the CTA exits
@@ -357,7 +370,7 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
                 mma_commit(v_empty(s));
                 return true;
             };
-            for (int j = 0; j < args.n_kvb && ok; j++) {
+            for (int j = j_first; j < j_end && ok; j++) {
                 if (flags[j] == MF_MASKED) continue;
                 const int i = n_active;
                 const int s = i & 1;
@@ -397,8 +410,10 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
         const int h = hg * args.GP + g;
         const int t = tb * args.TQ + tq;
         const bool row_valid = t < args.T;
-        const float qs = row_valid ? __ldg(args.qscale + (int64_t)h * args.T + t) : 1.0f;
-        const uint16_t* mrow = (args.mask && row_valid) ? args.mask + (int64_t)t * args.m_stride : nullptr;
+        const float qs = (row_valid ? __ldg(args.qscale + ((int64_t)str * args.H + h) * args.T + t) : 1.0f) *
+                         (EXT ? args.scale : 1.0f);
+        const uint16_t* mrow = (args.mask && row_valid) ? args.mask + (EXT ? str * args.m_stream : 0) + (int64_t)t * args.m_stride
+                                                        : nullptr;
         const float LOG2E = 1.4426950408889634f;
         const float c2 = qs * LOG2E;                     // raw score -> log2 units
         const float softcap = args.softcap;
@@ -445,7 +460,7 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
         float l = 0.0f;                                  // this thread's partial row sum
         int i = 0;
         bool ok = true;
-        for (int j = 0; j < args.n_kvb && ok; j++) {
+        for (int j = j_first; j < j_end && ok; j++) {
             const uint8_t fl = flags[j];
             if (fl == MF_MASKED) continue;
             const bool use_mask = (fl == MF_MIXED) && (mrow != nullptr);
@@ -487,6 +502,7 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
                             const uint32_t mw = (&mv[e >> 3].x)[(e & 7) >> 1];
                             const uint16_t mb = (uint16_t)((e & 1) ? (mw >> 16) : (mw & 0xFFFFu));
                             sv = fmaf(__half2float(__ushort_as_half(mb)), LOG2E, sv);
+                            if (EXT && mb == 0xFC00u) sv = -INFINITY;
                         }
                         if (k0 + c0 + e >= args.KV) sv = -INFINITY;
                         x[c0 + e] = sv;
@@ -566,7 +582,41 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
         float l_tot = 0.0f;
 #pragma unroll
         for (int k = 0; k < FA_SPLIT; k++) l_tot += sums[k];
-        if (ok && have_o) {
+        if constexpr (EXT) {
+            if (ok) {                                    // tcgen05.ld is a whole warp's: rows past T load too
+                const int64_t row = ((int64_t)str * args.T + t) * args.H + h;
+                const bool whole = args.splits == 1;
+                const int64_t at = whole ? row : row * args.splits + blockIdx.z;
+                const float inv = whole ? 1.0f / l_tot : 1.0f;
+                if (!whole && pt == 0 && row_valid) {
+                    args.stat[3 * at] = m;
+                    args.stat[3 * at + 1] = l_tot;
+                    args.stat[3 * at + 2] = 0.0f;
+                }
+#pragma unroll
+                for (int c0 = 0; c0 < OPT; c0 += 16) {
+                    uint32_t ov[16];
+                    if (have_o) {
+                        tmem_ld16(o_tmem + (uint32_t)c0, ov);
+                        tmem_ld_wait();
+                    }
+                    float y[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) y[e] = have_o && l_tot != 0.0f ? __uint_as_float(ov[e]) * inv : 0.0f;
+                    if (!row_valid) {
+                    } else if (whole && args.dst_f16) {
+                        uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<__half*>(args.dst) + at * DV + pt * OPT + c0);
+                        out[0] = make_uint4(pack_half2(y[0], y[1]), pack_half2(y[2], y[3]), pack_half2(y[4], y[5]), pack_half2(y[6], y[7]));
+                        out[1] = make_uint4(pack_half2(y[8], y[9]), pack_half2(y[10], y[11]), pack_half2(y[12], y[13]), pack_half2(y[14], y[15]));
+                    } else {
+                        float* out = (whole ? args.dst : args.part) + at * DV + pt * OPT + c0;
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4)
+                            *reinterpret_cast<float4*>(out + e) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+                    }
+                }
+            }
+        } else if (ok && have_o) {
             const float inv = l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
             float* out = args.dst + ((int64_t)t * args.H + h) * DV + pt * OPT;
 #pragma unroll
@@ -627,19 +677,19 @@ static FaLayout fa_layout(int D, int T, int H, int KV, int HK) {
     return L;
 }
 
-template <int D, int DV>
+template <int D, int DV, bool EXT = false>
 static cudaError_t launch_fa(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const FaArgs& a,
-                             int grid, cudaStream_t st) {
+                             dim3 grid, cudaStream_t st) {
     using C = FaCfg<D, DV>;
     static bool set[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 0 && dev < 64 && !set[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(fa_kernel<D, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        cudaError_t e = cudaFuncSetAttribute(fa_kernel<D, DV, EXT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) return e;
         set[dev] = true;
     }
-    return launch_pdl(fa_kernel<D, DV>, dim3((unsigned)grid), dim3(FA_THREADS), C::SMEM, st, tq, tk, tv, a);
+    return launch_pdl(fa_kernel<D, DV, EXT>, grid, dim3(FA_THREADS), C::SMEM, st, tq, tk, tv, a);
 }
 
 int flash_attn_impl(const float* q, int64_t q_nb1, int64_t q_nb2, const void* k, int64_t k_nb1, int64_t k_nb2,
@@ -696,13 +746,214 @@ int flash_attn_impl(const float* q, int64_t q_nb1, int64_t q_nb2, const void* k,
     a.n_kvb = L.n_kvb;
     a.softcap = softcap;
     a.err = dev_err;
-    const int grid = L.n_hg * L.n_tb;
+    const dim3 grid((unsigned)(L.n_hg * L.n_tb));
     cudaError_t e;
     if (D == 128 && DV == 128) e = launch_fa<128, 128>(tq, tk, tv, a, grid, st);
     else if (D == 64 && DV == 64) e = launch_fa<64, 64>(tq, tk, tv, a, grid, st);
     else if (D == 128 && DV == 64) e = launch_fa<128, 64>(tq, tk, tv, a, grid, st);
     else e = launch_fa<64, 128>(tq, tk, tv, a, grid, st);
     return e == cudaSuccess ? B200_OK : B200_E_CUDA;
+}
+
+// ---- the kernels over several streams, from a Q4_0 cache brought to fp16 tiles (b200_flash_attn_kvq) ----
+
+// Set-up pass of one launch: CTAs [0, q_ctas) bring q to fp16 (one warp a row, a power-of-two divisor for
+// rows beyond fp16's range; not scaled, so that f16 values stay exact), the next m_ctas classify the mask,
+// the rest bring the cache to fp16: four lanes a block of 32 values, each eight of them.
+struct FaQuantPrep {
+    const char* q;
+    int64_t q_t, q_h, q_s;
+    int q_f16;
+    __half* q16;
+    float* qscale;
+    const uint16_t* mask;
+    int64_t m_stride, m_stream;
+    int mask_vec;
+    uint8_t* flags;
+    const uint8_t* k;
+    int64_t k_r, k_h, k_s;
+    const uint8_t* v;
+    int64_t v_r, v_h, v_s;
+    __half* k16;
+    __half* v16;
+    int T, H, KV, HK, S, TQ, n_kvb, n_tb, q_ctas, m_ctas, m_grid;
+};
+
+// The eight values of bytes b of a Q4_0 block as fp16, each code * d rounded once: low nibbles, high nibbles.
+__device__ __forceinline__ void q4_0_values(uint32_t b, uint32_t d2, uint2* lo, uint2* hi) {
+    const __half2 c1032 = __half2half2(__ushort_as_half(0x6408)), c72 = __half2half2(__ushort_as_half(0x5480));
+    const __half2 d = *reinterpret_cast<const __half2*>(&d2);
+    const uint32_t u = b >> 8;
+    const uint32_t w[4] = {(b & 0x000f000fu) | 0x64006400u, (u & 0x000f000fu) | 0x64006400u,
+                           (b & 0x00f000f0u) | 0x54005400u, (u & 0x00f000f0u) | 0x54005400u};
+    uint32_t x[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const __half2 h = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&w[i]), i < 2 ? c1032 : c72), d);
+        x[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    *lo = make_uint2(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[0], x[1], 0x7632));
+    *hi = make_uint2(__byte_perm(x[2], x[3], 0x5410), __byte_perm(x[2], x[3], 0x7632));
+}
+
+template <int D>
+__global__ void __launch_bounds__(256) fa_quant_prep_kernel(const FaQuantPrep a) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const int lane = threadIdx.x & 31;
+    if ((int)blockIdx.x < a.q_ctas) {
+        const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);   // (stream, head, token)
+        if (row >= (int64_t)a.S * a.H * a.T) return;
+        const int t = (int)(row % a.T), h = (int)(row / a.T % a.H), s = (int)(row / a.T / a.H);
+        const char* src = a.q + s * a.q_s + h * a.q_h + t * a.q_t;
+        constexpr int PER = D / 32;
+        float x[PER], amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            x[i] = a.q_f16 ? __half2float(reinterpret_cast<const __half*>(src)[lane * PER + i])
+                           : reinterpret_cast<const float*>(src)[lane * PER + i];
+            amax = fmaxf(amax, fabsf(x[i]));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        // f32 rows are brought near 1 as well, so that small ones keep fp16's full precision
+        int e = 0;
+        if (!a.q_f16 && amax > 0.0f && amax <= 3.402823466e38f) frexpf(amax, &e);
+        e = max(-100, e);
+#pragma unroll
+        for (int i = 0; i < PER; i += 2)
+            *reinterpret_cast<uint32_t*>(a.q16 + row * D + lane * PER + i) = pack_half2(ldexpf(x[i], -e), ldexpf(x[i + 1], -e));
+        if (lane == 0) a.qscale[row] = ldexpf(1.0f, e);
+        return;
+    }
+    const int mi = (int)blockIdx.x - a.q_ctas;
+    if (mi < a.m_grid) {
+        if (!a.mask) {
+            for (int i = threadIdx.x; i < a.S * a.n_tb * a.n_kvb; i += blockDim.x) a.flags[i] = MF_ZERO;
+            return;
+        }
+        for (int i = mi; i < a.m_ctas; i += a.m_grid) {
+            const int j = i % a.n_kvb, tb = i / a.n_kvb % a.n_tb, s = i / a.n_kvb / a.n_tb;
+            fa_mask_block(a.mask + s * a.m_stream, a.m_stride, a.mask_vec != 0, a.T, a.KV, a.TQ, tb, j, a.n_kvb,
+                          a.flags + (int64_t)s * a.n_tb * a.n_kvb);
+        }
+        return;
+    }
+    // A key whose value scales are no finite numbers gets zeros for them and NaN keys: rows that see it
+    // become NaN through their scores, rows that do not stay clear of it (0 * NaN is NaN).
+    constexpr int NB = D / 32, LANES = 4 * NB;           // lanes of a key's row
+    const int64_t rows = (int64_t)a.S * a.HK * a.KV;
+    const int64_t first = ((int64_t)(mi - a.m_grid) * 256 + threadIdx.x) / LANES;
+    const int64_t step = (int64_t)(gridDim.x - a.q_ctas - a.m_grid) * 256 / LANES;
+    const int c = (int)(threadIdx.x % LANES), b = c >> 2, p = c & 3;
+    for (int64_t r0 = first - (threadIdx.x & 31) / LANES; r0 < rows; r0 += step) {   // warp-uniform bound
+        const int64_t r = r0 + (threadIdx.x & 31) / LANES;
+        const bool in = r < rows;
+        const int64_t key = in ? r % a.KV : 0, sh = in ? r / a.KV : 0;
+        const int64_t hk = sh % a.HK, s = sh / a.HK;
+        const uint16_t* kb = reinterpret_cast<const uint16_t*>(a.k + s * a.k_s + hk * a.k_h + key * a.k_r + 18 * b);
+        const uint16_t* vb = reinterpret_cast<const uint16_t*>(a.v + s * a.v_s + hk * a.v_h + key * a.v_r + 18 * b);
+        uint32_t dk = __ldg(kb), dv = __ldg(vb);
+        const uint32_t kw = __ldg(kb + 1 + 2 * p) | ((uint32_t)__ldg(kb + 2 + 2 * p) << 16);
+        const uint32_t vw = __ldg(vb + 1 + 2 * p) | ((uint32_t)__ldg(vb + 2 + 2 * p) << 16);
+        // codes of -8 may still take a large scale past fp16's range: such values count as no numbers too
+        const float worst = fabsf(__half2float(__ushort_as_half((unsigned short)dv))) * 8.0f;
+        const uint32_t votes = __ballot_sync(0xffffffffu, !(worst <= 65504.0f));
+        if ((votes >> ((threadIdx.x & 31) / LANES * LANES)) & (LANES == 32 ? 0xffffffffu : (1u << LANES) - 1u))
+            dk = 0x7e00u, dv = 0u;
+        if (!in) continue;
+        uint2 lo, hi;
+        q4_0_values(kw, dk | (dk << 16), &lo, &hi);
+        __half* ko = a.k16 + r * D + 32 * b + 4 * p;
+        *reinterpret_cast<uint2*>(ko) = lo;
+        *reinterpret_cast<uint2*>(ko + 16) = hi;
+        q4_0_values(vw, dv | (dv << 16), &lo, &hi);
+        __half* vo = a.v16 + r * D + 32 * b + 4 * p;
+        *reinterpret_cast<uint2*>(vo) = lo;
+        *reinterpret_cast<uint2*>(vo + 16) = hi;
+    }
+}
+
+struct FaQuantLayout {
+    FaLayout L;
+    int splits, kvb_per_split;
+    size_t q16_off, qs_off, flags_off, k_off, v_off, part_off, stat_off, total;
+};
+
+static FaQuantLayout fa_quant_layout(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S) {
+    FaQuantLayout Q{};
+    Q.L = fa_layout((int)D, (int)T, (int)H, (int)KV, (int)HK);
+    // few query tiles: the keys split until the SMs are filled twice, at least four blocks a part
+    const int64_t tiles = S * Q.L.n_hg * Q.L.n_tb;
+    int64_t splits = std::max<int64_t>(1, 2 * device_sm_count() / tiles);
+    splits = std::min<int64_t>(splits, std::max<int64_t>(1, Q.L.n_kvb / 4));
+    Q.kvb_per_split = (int)((Q.L.n_kvb + splits - 1) / splits);
+    Q.splits = (Q.L.n_kvb + Q.kvb_per_split - 1) / Q.kvb_per_split;
+    auto al = [](size_t x) { return (x + 255) & ~(size_t)255; };
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t o = at; at += al(n); return o; };
+    Q.q16_off = take((size_t)(S * H * T * D) * 2);
+    Q.qs_off = take((size_t)(S * H * T) * 4);
+    Q.flags_off = take((size_t)S * Q.L.n_tb * Q.L.n_kvb);
+    Q.k_off = take((size_t)(S * HK * KV * D) * 2);
+    Q.v_off = take((size_t)(S * HK * KV * D) * 2);
+    Q.part_off = take(Q.splits > 1 ? (size_t)(S * T * H * Q.splits * D) * 4 : 0);
+    Q.stat_off = take(Q.splits > 1 ? (size_t)(S * T * H * Q.splits) * 12 : 0);
+    Q.total = at;
+    return Q;
+}
+
+size_t fa_quant_workspace(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S) {
+    return fa_quant_layout(D, T, H, KV, HK, S).total;
+}
+
+cudaError_t fa_quant_run(const FaQuantArgs& q, char* ws, int* splits, float** part, float** stat, cudaStream_t st) {
+    const FaQuantLayout Q = fa_quant_layout(q.D, q.T, q.H, q.KV, q.HK, q.S);
+    const FaLayout& L = Q.L;
+    FaQuantPrep p{};
+    p.q = q.q, p.q_t = q.q_t, p.q_h = q.q_h, p.q_s = q.q_s, p.q_f16 = q.q_f16;
+    p.q16 = reinterpret_cast<__half*>(ws + Q.q16_off);
+    p.qscale = reinterpret_cast<float*>(ws + Q.qs_off);
+    p.mask = reinterpret_cast<const uint16_t*>(q.mask);
+    p.m_stride = q.m_t / 2, p.m_stream = q.m_s / 2, p.mask_vec = q.m_vec;
+    p.flags = reinterpret_cast<uint8_t*>(ws + Q.flags_off);
+    p.k = reinterpret_cast<const uint8_t*>(q.k), p.k_r = q.k_r, p.k_h = q.k_h, p.k_s = q.k_s;
+    p.v = reinterpret_cast<const uint8_t*>(q.v), p.v_r = q.v_r, p.v_h = q.v_h, p.v_s = q.v_s;
+    p.k16 = reinterpret_cast<__half*>(ws + Q.k_off);
+    p.v16 = reinterpret_cast<__half*>(ws + Q.v_off);
+    p.T = q.T, p.H = q.H, p.KV = q.KV, p.HK = q.HK, p.S = q.S;
+    p.TQ = L.TQ, p.n_kvb = L.n_kvb, p.n_tb = L.n_tb;
+    const int sms = device_sm_count();
+    p.q_ctas = (int)(((int64_t)q.S * q.H * q.T + 7) / 8);
+    p.m_ctas = q.mask ? q.S * L.n_tb * L.n_kvb : 1;
+    p.m_grid = std::min(p.m_ctas, sms * 16);
+    const int64_t lanes = (int64_t)q.S * q.HK * q.KV * (q.D / 8);
+    const int c_grid = (int)std::max<int64_t>(1, std::min<int64_t>((lanes + 255) / 256, (int64_t)sms * 16));
+    const dim3 grid((unsigned)(p.q_ctas + p.m_grid + c_grid)), block(256);
+    cudaError_t e = q.D == 64 ? launch_pdl(fa_quant_prep_kernel<64>, grid, block, 0, st, p)
+                              : launch_pdl(fa_quant_prep_kernel<128>, grid, block, 0, st, p);
+    if (e != cudaSuccess) return e;
+    const uint64_t D = (uint64_t)q.D, row = D * 2;
+    CUtensorMap tq, tk, tv;
+    if (!make_tmap_3d_f16(&tq, p.q16, D, q.T, (uint64_t)q.S * q.H, row, (uint64_t)q.T * row, 64, L.TQ, L.GP) ||
+        !make_tmap_3d_f16(&tk, p.k16, D, q.KV, (uint64_t)q.S * q.HK, row, (uint64_t)q.KV * row, 64, FA_KB, 1) ||
+        !make_tmap_3d_f16(&tv, p.v16, D, q.KV, (uint64_t)q.S * q.HK, row, (uint64_t)q.KV * row, 64, FA_KB, 1))
+        return cudaErrorInvalidValue;
+    FaArgs a{};
+    a.qscale = p.qscale;
+    a.mask = p.mask;
+    a.m_stride = p.m_stride, a.m_stream = p.m_stream, a.mask_vec = q.m_vec != 0;
+    a.flags = p.flags;
+    a.dst = static_cast<float*>(q.dst);
+    a.T = q.T, a.H = q.H, a.KV = q.KV, a.HK = q.HK, a.GP = L.GP, a.TQ = L.TQ, a.n_hg = L.n_hg, a.n_tb = L.n_tb, a.n_kvb = L.n_kvb;
+    a.softcap = q.softcap, a.scale = q.scale, a.dst_f16 = q.dst_f16;
+    a.splits = Q.splits, a.kvb_per_split = Q.kvb_per_split;
+    a.part = reinterpret_cast<float*>(ws + Q.part_off);
+    a.stat = reinterpret_cast<float*>(ws + Q.stat_off);
+    a.err = q.err;
+    *splits = Q.splits, *part = a.part, *stat = a.stat;
+    const dim3 fgrid((unsigned)(L.n_hg * L.n_tb), (unsigned)q.S, (unsigned)Q.splits);
+    return q.D == 64 ? launch_fa<64, 64, true>(tq, tk, tv, a, fgrid, st) : launch_fa<128, 128, true>(tq, tk, tv, a, fgrid, st);
 }
 
 }  // namespace b200

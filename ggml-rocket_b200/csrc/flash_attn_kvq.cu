@@ -58,6 +58,9 @@ constexpr int KR_BOX = 144;            // bytes of a key's row in a TMA tile
 constexpr int KR_MAX_TILES = 1024;     // tiles of a CTA's range (its list of live tiles)
 constexpr int64_t KR_WAVES = 6;
 constexpr int64_t KR_MIN_SPLIT = 2048;   // keys of a part, where they are many
+// More query rows a KV head than this go to the tcgen05 kernel over fp16 tiles of the cache: the row kernel
+// reads the cache again for every 8 rows, the tiles cost two passes over it whatever the rows.
+constexpr int64_t KR_MAX_ROWS = 32;
 constexpr float KR_LOG2E = 1.4426950408889634f;
 
 struct KvqArgs {
@@ -837,6 +840,7 @@ extern "C" {
 size_t b200_flash_attn_kvq_workspace_size(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S) {
     using namespace b200;
     if (!kvq_dims_ok(D, T, H, KV, HK, S)) return 0;
+    if (T * (H / HK) > KR_MAX_ROWS) return fa_quant_workspace(D, T, H, KV, HK, S);
     return std::max(kvq_plan(D, T, H, KV, HK, S, true).total, kvq_plan(D, T, H, KV, HK, S, false).total);
 }
 
@@ -855,15 +859,40 @@ int b200_flash_attn_kvq(int kv_type, int q_type, const void* q, const int64_t qn
         return B200_E_INVALID;
     if (kv_type != 2 || (q_type != 0 && q_type != 1) || (dst_type != 0 && dst_type != 1)) return B200_E_UNSUPPORTED;
     const size_t qe = q_type == 1 ? 2 : 4, unit = (size_t)D / 16;
-    if (!kvq_dims_ok(D, T, H, KV, HK, S) || T > 65536 || S > 65535 || KV > (1ll << 30) || T * (H / HK) > (1 << 20) ||
+    if (!kvq_dims_ok(D, T, H, KV, HK, S) || T > 65536 || S > 65535 || KV > (1ll << 30) || T * (H / HK) > (1 << 20) || S * T * H > INT32_MAX / 4 ||
         HK * ((T * (H / HK) + KR_ROWS - 1) / KR_ROWS) > 65535)
         return B200_E_UNSUPPORTED;
     auto off = [](const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; };
     if (qnb[0] != qe || (qnb[1] | qnb[2] | qnb[3]) % qe != 0 || off(q, qe) || knb[0] != 18 || vnb[0] != 18 ||
         (knb[1] | knb[2] | knb[3] | vnb[1] | vnb[2] | vnb[3]) % unit != 0 || off(k, unit) || off(v, unit) ||
-        off(dst, dst_type == 1 ? 2 : 4))
+        off(dst, 16))
         return B200_E_UNSUPPORTED;
     if (mask && (mnb[0] != 2 || ((mnb[1] | mnb[3]) & 1) || off(mask, 2))) return B200_E_UNSUPPORTED;
+    const size_t need = b200_flash_attn_kvq_workspace_size(D, T, H, KV, HK, S);
+    if (!workspace || workspace_bytes < need || off(workspace, 256)) return B200_E_WORKSPACE;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (T * (H / HK) > KR_MAX_ROWS) {
+        FaQuantArgs f{};
+        f.q = static_cast<const char*>(q);
+        f.q_t = (int64_t)qnb[1], f.q_h = (int64_t)qnb[2], f.q_s = (int64_t)qnb[3], f.q_f16 = q_type == 1;
+        f.k = static_cast<const char*>(k), f.k_r = (int64_t)knb[1], f.k_h = (int64_t)knb[2], f.k_s = (int64_t)knb[3];
+        f.v = static_cast<const char*>(v), f.v_r = (int64_t)vnb[1], f.v_h = (int64_t)vnb[2], f.v_s = (int64_t)vnb[3];
+        f.mask = static_cast<const char*>(mask);
+        f.m_t = mask ? (int64_t)mnb[1] : 0, f.m_s = mask ? (int64_t)mnb[3] : 0;
+        f.m_vec = mask && ((mnb[1] | mnb[3]) & 15) == 0 && !off(mask, 16);
+        f.dst = dst, f.dst_f16 = dst_type == 1;
+        f.D = (int)D, f.T = (int)T, f.H = (int)H, f.KV = (int)KV, f.HK = (int)HK, f.S = (int)S;
+        f.scale = scale, f.softcap = softcap, f.err = dev_err;
+        int splits = 1;
+        float *part = nullptr, *stat = nullptr;
+        cudaError_t e = fa_quant_run(f, static_cast<char*>(workspace), &splits, &part, &stat, st);
+        if (e == cudaSuccess && splits > 1) {
+            const dim3 rows((unsigned)(S * T * H)), block(128);
+            e = D == 64 ? launch_pdl(kvq_join_kernel<64>, rows, block, 0, st, (const float*)part, (const float*)stat, splits, f.dst_f16, dst)
+                        : launch_pdl(kvq_join_kernel<128>, rows, block, 0, st, (const float*)part, (const float*)stat, splits, f.dst_f16, dst);
+        }
+        return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? B200_OK : B200_E_CUDA;
+    }
     const int64_t row = D / 32 * 18;
     // what a tensor map of the cache needs: heads side by side, 16-byte bases and strides, strides below 2^40
     auto tma_ok = [&](const void* p, const size_t* s) {
@@ -871,8 +900,6 @@ int b200_flash_attn_kvq(int kv_type, int q_type, const void* q, const int64_t qn
                s[1] < (1ull << 40) && s[3] < (1ull << 40) && (S == 1 || s[3] > 0);
     };
     const KvqPlan p = kvq_plan(D, T, H, KV, HK, S, tma_ok(k, knb) && tma_ok(v, vnb));
-    if (!workspace || workspace_bytes < b200_flash_attn_kvq_workspace_size(D, T, H, KV, HK, S) || off(workspace, 256))
-        return B200_E_WORKSPACE;
     KvqArgs a{};
     a.q = static_cast<const char*>(q);
     a.q_t = (int64_t)qnb[1], a.q_h = (int64_t)qnb[2], a.q_s = (int64_t)qnb[3];
@@ -892,7 +919,6 @@ int b200_flash_attn_kvq(int kv_type, int q_type, const void* q, const int64_t qn
     a.T = (int)T, a.H = (int)H, a.KV = (int)KV, a.HK = (int)HK, a.G = (int)(H / HK), a.S = (int)S;
     a.splits = p.splits, a.tiles_per_split = p.tiles_per_split;
     a.scale = scale, a.softcap = softcap;
-    const cudaStream_t st = static_cast<cudaStream_t>(stream);
     a.err = dev_err;
     CUtensorMap tk{}, tv{};
     if (p.heads > 1) {

@@ -6,7 +6,11 @@ of A, the tensor core truncating) and forms the exponent with |s| log2(e) rounde
 2^-22: a weight is within e = A 2^-18 + 2^-20 of its value, relative. Outputs are ratios of sums of such
 weights, each added in fp32 over at most a few hundred steps (2^-15 at the worst, far less in truth):
 |dO| <= (2 e + 2^-15) V. An f16 result adds the rounding of P (2^-11 of each weight) and of itself
-(2^-11): |dO| <= (2 e + 2^-15 + 2^-11) V + 2^-11 |O| + 2^-25."""
+(2^-11): |dO| <= (2 e + 2^-15 + 2^-11) V + 2^-11 |O| + 2^-25.
+
+More than 32 query rows a KV head take the tcgen05 kernel over fp16 tiles: q, the decoded keys, the
+decoded values and P each round to fp16 (2^-11 of a value), and a score plus its mask M to fp32 (2^-24 of
+1.45 M in log2 units, 2^-24 M of the weight; 2^-23 allowed), so e = 2 * 2^-11 A + A 2^-18 + 2^-23 M + 2^-20, and |dO| <= (2 e + 2^-15 + 2 * 2^-11) V for the rest, the maximum taken over V."""
 import math
 
 import numpy as np
@@ -99,8 +103,12 @@ def run(q, k, v, mask, scale, f16=False, softcap=0.0, stream=None, ws=None):
 def check(out, q, k, v, mask, scale, softcap=0.0):
     import torch
     want, A, vmax = reference(q, k, v, mask, scale, softcap)
-    e = A * 2.0 ** -18 + 2.0 ** -20
-    tol = (2 * e + 2.0 ** -15) * vmax
+    prompt = q.shape[1] * (q.shape[2] // k.shape[2]) > 32
+    e = A * (2.0 ** -18 + (2 * 2.0 ** -11 if prompt else 0)) + 2.0 ** -20
+    if prompt and mask is not None:      # score + mask rounded to fp32
+        fin = mask[torch.isfinite(mask)]
+        e = e + (float(fin.abs().max()) * 2.0 ** -23 if fin.numel() else 0.0)
+    tol = (2 * e + 2.0 ** -15 + (2 * 2.0 ** -11 if prompt else 0)) * vmax
     if out.dtype == torch.float16:
         tol = tol + 2.0 ** -11 * vmax + 2.0 ** -11 * want.abs() + 2.0 ** -25
     assert torch.equal(torch.isnan(out), torch.isnan(want))
@@ -155,8 +163,34 @@ def test_rows_against_definition(cuda, S, T, H, HK, D, KV, f16):
     check(run(q, k, v, None, scale, f16), q, k, v, None, scale)
 
 
+PROMPTS = [
+    # S, T, H, HK, D, KV
+    (1, 33, 1, 1, 64, 33),
+    (1, 40, 4, 1, 128, 129),
+    (1, 200, 32, 8, 128, 1000),
+    (2, 130, 14, 2, 64, 700),        # seven heads a group: one query head a tile
+    (3, 17, 8, 2, 128, 2000),        # parts of the keys over several CTAs
+    (1, 512, 8, 2, 128, 4096),
+    (1, 9, 32, 4, 64, 20000),
+]
+
+
 @pytest.mark.parametrize("f16", [False, True])
-@pytest.mark.parametrize("T", [1, 6])
+@pytest.mark.parametrize("S,T,H,HK,D,KV", PROMPTS)
+def test_prompts_against_definition(cuda, S, T, H, HK, D, KV, f16):
+    q, k, v = inputs(S, T, H, HK, D, KV, q_f16=f16)
+    scale = 1 / math.sqrt(D)
+    m = causal(S, T, KV, [KV - (KV - T) * s // (S + 1) for s in range(S)])
+    out = run(q, k, v, m, scale, f16)
+    check(out, q, k, v, m, scale)
+    want = reference(q, k, v, m, scale)[0]
+    assert float((out.double() - want).norm() / want.norm()) < 2e-3     # random roundings: far below the bound
+    check(run(q, k, v, None, scale, f16), q, k, v, None, scale)
+    check(run(q, k, v, None, scale, f16, softcap=5.0), q, k, v, None, scale, softcap=5.0)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("T", [1, 6, 50])
 def test_masks(cuda, T, f16):
     """Rows that see nothing, one key, only keys of fp16's lowest value, that value beside visible keys,
     finite biases, a gap of more than a tile, and a mask row wider and off alignment."""
