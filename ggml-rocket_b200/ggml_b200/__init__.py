@@ -6,6 +6,7 @@ fails loudly when the library has not been built: there is no Python or CPU fall
 """
 import ctypes
 import os
+import struct as _struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
@@ -603,35 +604,54 @@ def mul_mat_id_ffn(wtype_gate_up, gate, up, wtype_down, down, H, F, n_expert, x,
 
 
 ROPE_MROPE, ROPE_VISION, ROPE_IMROPE = 8, 24, 40
-_I64x4, _SZx4, _I32x4 = ctypes.c_int64 * 4, ctypes.c_size_t * 4, ctypes.c_int32 * 4
-_ROW_TYPES = {"torch.float32": F32, "torch.float16": F16, "torch.int32": I32, "torch.int64": I64}
+
+# What the wrappers below need of torch, looked up once: they run once an op of a decoded token, where the
+# kernel takes a few microseconds. ne / nb go to C as packed bytes (a ctypes array takes seven times as long).
+_torch_types = None
+_raw_stream = _device = None
+_ne4 = _struct.Struct("4q").pack
+_sec4 = _struct.Struct("4i").pack
+
+
+def _types():
+    global _torch_types, _raw_stream, _device
+    if _torch_types is None:
+        import torch
+        _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+        torch.cuda.init()
+        _torch_types = {torch.float32: F32, torch.float16: F16, torch.int32: I32, torch.int64: I64}
+    return _torch_types
+
+
+def _on(what, *tensors):
+    """The current device, which every tensor of a call has to be on (kernels launch there)."""
+    _torch_types or _types()
+    dev = _device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise B200Error(f"{what}: a tensor is on {t.device}, the current device is cuda:{dev}")
+    return dev
 
 
 def _type_of(t, what):
-    ty = _ROW_TYPES.get(str(t.dtype))
+    ty = _torch_types.get(t.dtype)
     if ty is None:
         raise B200Error(f"{what}: dtype {t.dtype} is not supported")
     return ty
 
 
-def _on(t, what, *others):
-    """The current device must hold every tensor of a call (kernels launch on the current device)."""
-    import torch
-    dev = torch.cuda.current_device()
-    for x in (t,) + others:
-        if x is not None and (not x.is_cuda or x.device.index != dev):
-            raise B200Error(f"{what}: a tensor is on {x.device}, the current device is cuda:{dev}")
+def _stream_of(stream, dev):
+    return _raw_stream(dev) if stream is None else stream.cuda_stream
 
 
 def _dims(t):
     """ggml's ne / nb (bytes) of a torch tensor of 1 to 4 dims, outermost first."""
-    sh, st, es = t.shape, t.stride(), t.element_size()
-    n = len(sh)
-    ne, nb = [1, 1, 1, 1], [es, es, es, es]
-    for i in range(n):
-        ne[i], nb[i] = sh[n - 1 - i], st[n - 1 - i] * es
-    for i in range(n, 4):
-        nb[i] = nb[i - 1] * ne[i - 1]
+    es = t.element_size()
+    ne = list(t.shape)[::-1]
+    nb = [x * es for x in t.stride()][::-1]
+    while len(ne) < 4:
+        nb.append(nb[-1] * ne[-1] if nb else es)
+        ne.append(1)
     return ne, nb
 
 
@@ -648,22 +668,24 @@ def _dims_q(t, kind, what):
 def rope_multi(x, pos, dst, n_dims, mode, sections, freq_base=10000.0, freq_scale=1.0, attn_factor=1.0, stream=None):
     """ROPE with several position axes (b200_rope_multi): x f32 / f16 [.., n_tokens, n_head, head_dim] with any
     strides, pos int32 [4, n_tokens], dst contiguous of x's shape and type (x itself when contiguous)."""
-    _on(x, "rope_multi", pos, dst)
+    dev = _on("rope_multi", x, pos, dst)
+    ty = _type_of(x, "rope_multi")
     ne, nb = _dims(x)
-    if dst.dtype != x.dtype or dst.shape != x.shape or not dst.is_contiguous() or str(pos.dtype) != "torch.int32" or \
-            not pos.is_contiguous() or tuple(pos.shape) != (4, ne[2]):
+    if dst.dtype != x.dtype or dst.shape != x.shape or not dst.is_contiguous() or _type_of(pos, "rope_multi") != I32 or \
+            not pos.is_contiguous() or pos.shape != (4, ne[2]):
         raise B200Error("rope_multi: dst is contiguous and of x's shape and type, pos contiguous int32 [4, n_tokens]")
-    check(lib().b200_rope_multi(_type_of(x, "rope_multi"), x.data_ptr(), _I64x4(*ne), _SZx4(*nb), pos.data_ptr(), n_dims,
-                                mode, _I32x4(*sections), freq_base, freq_scale, attn_factor, dst.data_ptr(),
-                                _stream(stream)), "rope_multi")
+    rc = lib().b200_rope_multi(ty, x.data_ptr(), _ne4(*ne), _ne4(*nb), pos.data_ptr(), n_dims, mode, _sec4(*sections),
+                               freq_base, freq_scale, attn_factor, dst.data_ptr(), _stream_of(stream, dev))
+    if rc:
+        check(rc, "rope_multi")
     return dst
 
 
 def set_rows(src, idx, dst, dst_type, dev_err, stream=None):
     """dst[.., idx[i], :] = src[.., i, :] (b200_set_rows): src f32, idx int32 / int64 [.., n_rows], dst f32, f16 or,
     for Q4_0 / Q8_0, a uint8 tensor whose last dim holds a row's blocks; quantised as they are written."""
-    _on(src, "set_rows", idx, dst, dev_err)
-    if str(src.dtype) != "torch.float32":
+    dev = _on("set_rows", src, idx, dst, dev_err)
+    if _type_of(src, "set_rows") != F32:
         raise B200Error("set_rows: src is f32")
     sne, snb = _dims(src)
     ine, inb = _dims(idx)
@@ -673,16 +695,18 @@ def set_rows(src, idx, dst, dst_type, dev_err, stream=None):
         dne, dnb = _dims(dst)
     else:
         dne, dnb = _dims_q(dst, dst_type, "set_rows")
-    check(lib().b200_set_rows(src.data_ptr(), _I64x4(*sne), _SZx4(*snb), _type_of(idx, "set_rows"), idx.data_ptr(),
-                              _I64x4(*ine), _SZx4(*inb), dst_type, dst.data_ptr(), _I64x4(*dne), _SZx4(*dnb),
-                              dev_err.data_ptr(), _stream(stream)), "set_rows")
+    rc = lib().b200_set_rows(src.data_ptr(), _ne4(*sne), _ne4(*snb), _type_of(idx, "set_rows"), idx.data_ptr(), _ne4(*ine),
+                             _ne4(*inb), dst_type, dst.data_ptr(), _ne4(*dne), _ne4(*dnb), dev_err.data_ptr(),
+                             _stream_of(stream, dev))
+    if rc:
+        check(rc, "set_rows")
     return dst
 
 
 def get_rows(src, src_type, idx, dst, dev_err, stream=None):
     """dst[.., i, :] = src[.., idx[i], :] as f32 (b200_get_rows): src f32, f16 or, for Q4_0 / Q8_0, a uint8 tensor
     whose last dim holds a row's blocks; idx int32; dst contiguous f32."""
-    _on(src, "get_rows", idx, dst, dev_err)
+    dev = _on("get_rows", src, idx, dst, dev_err)
     if src_type in (F32, F16):
         if _type_of(src, "get_rows") != src_type:
             raise B200Error("get_rows: src is not of src_type")
@@ -690,11 +714,13 @@ def get_rows(src, src_type, idx, dst, dev_err, stream=None):
     else:
         sne, snb = _dims_q(src, src_type, "get_rows")
     ine, inb = _dims(idx)
-    if str(idx.dtype) != "torch.int32" or str(dst.dtype) != "torch.float32" or not dst.is_contiguous() or \
+    if _type_of(idx, "get_rows") != I32 or _type_of(dst, "get_rows") != F32 or not dst.is_contiguous() or \
             dst.numel() != sne[0] * idx.numel():
         raise B200Error("get_rows: idx is int32, dst contiguous f32 with a row for every index")
-    check(lib().b200_get_rows(src_type, src.data_ptr(), _I64x4(*sne), _SZx4(*snb), idx.data_ptr(), _I64x4(*ine),
-                              _SZx4(*inb), dst.data_ptr(), dev_err.data_ptr(), _stream(stream)), "get_rows")
+    rc = lib().b200_get_rows(src_type, src.data_ptr(), _ne4(*sne), _ne4(*snb), idx.data_ptr(), _ne4(*ine), _ne4(*inb),
+                             dst.data_ptr(), dev_err.data_ptr(), _stream_of(stream, dev))
+    if rc:
+        check(rc, "get_rows")
     return dst
 
 
@@ -706,29 +732,29 @@ def flash_attn_kvq(kv_type, q, k, v, mask, dst, scale, workspace, dev_err, softc
     """Attention over a KV cache held in 4 bits (b200_flash_attn_kvq): q f32 / f16 [S, T, H, D], k and v uint8
     [S, KV, HK, D / 32 * 18] (Q4_0 blocks), mask f16 [S or 1, T, KV] or None, dst contiguous f32 / f16 [S, T, H, D];
     strides of q, k, v and mask are theirs."""
-    _on(q, "flash_attn_kvq", k, v, mask, dst, workspace, dev_err)
+    dev = _on("flash_attn_kvq", q, k, v, mask, dst, workspace, dev_err)
     S, T, H, D = q.shape
     es = q.element_size()
-    qs = q.stride()
-    kne, knb = _dims_q(k, kv_type, "flash_attn_kvq")
-    vne, vnb = _dims_q(v, kv_type, "flash_attn_kvq")
+    qs, qt, qh, qd = q.stride()
+    # a cache row holds the heads of a key side by side: ggml's view has the keys as dim 1, the heads as dim 2
+    (kn, khk, kkv, kst), (k0, kh, kr, ks) = _dims_q(k, kv_type, "flash_attn_kvq")
+    (vn, vhk, vkv, vst), (v0, vh, vr, vs) = _dims_q(v, kv_type, "flash_attn_kvq")
     if dst.shape != q.shape or not dst.is_contiguous():
         raise B200Error("flash_attn_kvq: dst is contiguous and of q's shape")
-    mnb = None
+    mp = mnb = None
     if mask is not None:
-        if str(mask.dtype) != "torch.float16" or mask.dim() != 3 or mask.shape[0] not in (1, S) or \
-                mask.shape[1] < T or mask.shape[2] < kne[2]:
+        if _type_of(mask, "flash_attn_kvq") != F16 or mask.dim() != 3 or mask.shape[0] not in (1, S) or \
+                mask.shape[1] < T or mask.shape[2] < kkv:
             raise B200Error("flash_attn_kvq: mask is f16 [S or 1, T, KV]")
-        ms = mask.stride()
-        mnb = _SZx4(2 * ms[2], 2 * ms[1], 0, 2 * ms[0] if mask.shape[0] == S else 0)
-    # a cache row holds the heads of a key side by side: ggml's view has the keys as dim 1, the heads as dim 2
-    check(lib().b200_flash_attn_kvq(
-        kv_type, _type_of(q, "flash_attn_kvq"), q.data_ptr(), _I64x4(D, T, H, S),
-        _SZx4(qs[3] * es, qs[1] * es, qs[2] * es, qs[0] * es), k.data_ptr(), _I64x4(kne[0], kne[2], kne[1], kne[3]),
-        _SZx4(knb[0], knb[2], knb[1], knb[3]), v.data_ptr(), _I64x4(vne[0], vne[2], vne[1], vne[3]),
-        _SZx4(vnb[0], vnb[2], vnb[1], vnb[3]), None if mask is None else mask.data_ptr(), mnb,
-        _type_of(dst, "flash_attn_kvq"), dst.data_ptr(), scale, softcap, workspace.data_ptr(),
-        workspace.numel() * workspace.element_size(), dev_err.data_ptr(), _stream(stream)), "flash_attn_kvq")
+        ms, mt, mk = mask.stride()
+        mp, mnb = mask.data_ptr(), _ne4(2 * mk, 2 * mt, 0, 2 * ms if mask.shape[0] == S else 0)
+    rc = lib().b200_flash_attn_kvq(
+        kv_type, _type_of(q, "flash_attn_kvq"), q.data_ptr(), _ne4(D, T, H, S), _ne4(qd * es, qt * es, qh * es, qs * es),
+        k.data_ptr(), _ne4(kn, kkv, khk, kst), _ne4(k0, kr, kh, ks), v.data_ptr(), _ne4(vn, vkv, vhk, vst),
+        _ne4(v0, vr, vh, vs), mp, mnb, _type_of(dst, "flash_attn_kvq"), dst.data_ptr(), scale, softcap,
+        workspace.data_ptr(), workspace.numel() * workspace.element_size(), dev_err.data_ptr(), _stream_of(stream, dev))
+    if rc:
+        check(rc, "flash_attn_kvq")
     return dst
 
 
