@@ -49,6 +49,7 @@ bool dims_ok(const int64_t ne[4], const size_t nb[4]) {
 constexpr int KV_THREADS = 256;
 constexpr int KV_WARPS = KV_THREADS / 32;
 constexpr int KV_MAX_UNITS = 8;                        // 128-value chunks per warp
+constexpr int KV_AHEAD = 4;                            // of them with their loads under way
 constexpr int KV_MAX_ROWS = KV_WARPS * KV_MAX_UNITS;   // rows a CTA can touch
 
 __device__ __forceinline__ int64_t load_index(const char* p, int is64) {
@@ -137,60 +138,90 @@ __global__ void __launch_bounds__(KV_THREADS) set_rows_kernel(const char* __rest
     grid_dep_launch();
     __shared__ int64_t row_at[KV_MAX_ROWS + 1];
     __shared__ int live[KV_MAX_ROWS + 1];
-    const int64_t n_rows = ss.ne[1], n_units = n_rows * cpr;
-    const int64_t u0 = (int64_t)blockIdx.x * KV_WARPS * upw;
-    const int64_t u1 = min(n_units, u0 + (int64_t)KV_WARPS * upw);
-    const int64_t r0 = u0 / cpr;
-    const int rows = (int)((u1 - 1) / cpr - r0) + 1;
-    for (int64_t slice = blockIdx.y; slice < ss.ne[2] * ss.ne[3]; slice += gridDim.y) {
-        const int64_t i2 = slice % ss.ne[2], i3 = slice / ss.ne[2];
-        const char* ip = idx + (i2 % si.ne[1]) * si.nb[1] + (i3 % si.ne[2]) * si.nb[2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n_rows = (int)ss.ne[1], n_units = n_rows * cpr;          // below 2^31
+    const int u0 = blockIdx.x * KV_WARPS * upw;
+    const int u1 = min(n_units, u0 + KV_WARPS * upw);
+    const int r0 = u0 / cpr;
+    const int rows = (u1 - 1) / cpr - r0 + 1;
+    const int n2 = (int)ss.ne[2], slices = n2 * (int)ss.ne[3];
+    for (int slice = blockIdx.y; slice < slices; slice += gridDim.y) {
+        const int i2 = slices == 1 ? 0 : slice % n2, i3 = slices == 1 ? 0 : slice / n2;
+        const char* ip = idx;
+        if (slices > 1) ip += (i2 % (int)si.ne[1]) * si.nb[1] + (i3 % (int)si.ne[2]) * si.nb[2];
+        const char* sp = src + i2 * ss.nb[2] + i3 * ss.nb[3];
+        char* dp = dst + i2 * sd.nb[2] + i3 * sd.nb[3];
+        // the warp's 128 values of its units k .. k + KV_AHEAD - 1, all under way together
+        auto load = [&](int k, float (&x)[KV_AHEAD][4]) {
+#pragma unroll
+            for (int n = 0; n < KV_AHEAD; n++) {
+                const int u = u0 + (k + n) * KV_WARPS + warp;
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[n][e] = 0.0f;
+                if (k + n >= upw || u >= u1) continue;
+                const int r = u / cpr;
+                const int64_t e0 = 128ll * (u - r * cpr) + 4 * lane;
+                const float* p = reinterpret_cast<const float*>(sp + r * ss.nb[1]) + e0;
+                if constexpr (VEC) {
+                    if (e0 < ss.ne[0]) {
+                        const float4 v = __ldg(reinterpret_cast<const float4*>(p));
+                        x[n][0] = v.x, x[n][1] = v.y, x[n][2] = v.z, x[n][3] = v.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (e0 + e < ss.ne[0]) x[n][e] = __ldg(p + e);
+                }
+            }
+        };
+        float x[KV_AHEAD][4];
+        load(0, x);                      // under way while the indices are read
         for (int r = threadIdx.x; r < rows; r += KV_THREADS) {
-            const int64_t at = load_index(ip + (r0 + r) * si.nb[0], idx64);
+            const int64_t at = load_index(ip + (int64_t)(r0 + r) * si.nb[0], idx64);
             const bool in = at >= 0 && at < sd.ne[1];
             if (!in) atomicCAS(err, 0, ERR_BAD_INDEX);
             row_at[r] = at;
             live[r] = in ? 1 : 0;
         }
         __syncthreads();
-        for (int64_t j = r0 + 1 + threadIdx.x; j < n_rows; j += KV_THREADS) {
-            const int64_t at = load_index(ip + j * si.nb[0], idx64);
-            const int before = (int)min((int64_t)rows, j - r0);
-            for (int r = 0; r < before; r++)
-                if (row_at[r] == at) live[r] = 0;
+        constexpr int SCAN = 4;          // indices a thread has in flight
+        for (int64_t j0 = r0 + 1 + threadIdx.x; j0 < n_rows; j0 += KV_THREADS * SCAN) {
+            int64_t at[SCAN];
+#pragma unroll
+            for (int n = 0; n < SCAN; n++) {
+                const int64_t j = j0 + n * KV_THREADS;
+                at[n] = j < n_rows ? load_index(ip + j * si.nb[0], idx64) : -1;
+            }
+#pragma unroll
+            for (int n = 0; n < SCAN; n++) {
+                const int before = at[n] < 0 ? 0 : (int)min((int64_t)rows, j0 + n * KV_THREADS - r0);
+                for (int r = 0; r < before; r++)
+                    if (row_at[r] == at[n]) live[r] = 0;
+            }
         }
         __syncthreads();
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        for (int k = 0; k < upw; k++) {
-            const int64_t u = u0 + (int64_t)k * KV_WARPS + warp;
-            if (u >= u1) break;
-            const int64_t r = u / cpr;
-            if (!live[r - r0]) continue;
-            const int64_t e0 = 128 * (u - r * cpr) + 4 * lane;
-            const bool in = e0 < ss.ne[0];   // rows of quantised types are whole blocks of 8 lanes
-            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            const char* sp = src + r * ss.nb[1] + i2 * ss.nb[2] + i3 * ss.nb[3] + e0 * 4;
-            if (in) {
-                if constexpr (VEC) {
-                    const float4 v = __ldg(reinterpret_cast<const float4*>(sp));
-                    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+        for (int k = 0; k < upw; k += KV_AHEAD) {
+            if (k > 0) load(k, x);
+#pragma unroll
+            for (int n = 0; n < KV_AHEAD; n++) {
+                const int u = u0 + (k + n) * KV_WARPS + warp;
+                if (k + n >= upw || u >= u1) break;
+                const int r = u / cpr;
+                const int64_t e0 = 128ll * (u - r * cpr) + 4 * lane;
+                const bool in = e0 < ss.ne[0];   // rows of quantised types are whole blocks of 8 lanes
+                if (!live[r - r0]) continue;
+                char* out = dp + row_at[r - r0] * sd.nb[1];
+                if constexpr (TYPE == KT_Q4_0) {
+                    put_q4_0(x[n], in ? reinterpret_cast<uint8_t*>(out) + (e0 / 32) * 18 : nullptr);
+                } else if constexpr (TYPE == KT_Q8_0) {
+                    put_q8_0(x[n], in ? reinterpret_cast<uint8_t*>(out) + (e0 / 32) * 34 : nullptr);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (e0 + e < ss.ne[0]) x[e] = __ldg(reinterpret_cast<const float*>(sp) + e);
-                }
-            }
-            char* dp = dst + row_at[r - r0] * sd.nb[1] + i2 * sd.nb[2] + i3 * sd.nb[3];
-            if constexpr (TYPE == KT_Q4_0) {
-                put_q4_0(x, in ? reinterpret_cast<uint8_t*>(dp) + (e0 / 32) * 18 : nullptr);
-            } else if constexpr (TYPE == KT_Q8_0) {
-                put_q8_0(x, in ? reinterpret_cast<uint8_t*>(dp) + (e0 / 32) * 34 : nullptr);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if (e0 + e >= ss.ne[0]) continue;
-                    if constexpr (TYPE == KT_F16) reinterpret_cast<__half*>(dp)[e0 + e] = __float2half_rn(x[e]);
-                    else reinterpret_cast<float*>(dp)[e0 + e] = x[e];
+                    for (int e = 0; e < 4; e++) {
+                        if (e0 + e >= ss.ne[0]) continue;
+                        if constexpr (TYPE == KT_F16) reinterpret_cast<__half*>(out)[e0 + e] = __float2half_rn(x[n][e]);
+                        else reinterpret_cast<float*>(out)[e0 + e] = x[n][e];
+                    }
                 }
             }
         }
@@ -198,8 +229,11 @@ __global__ void __launch_bounds__(KV_THREADS) set_rows_kernel(const char* __rest
     }
 }
 
-// GET_ROWS of a quantised table: unit u is 128 values of output row u / cpr. An index outside the
-// table records ERR_BAD_INDEX and yields a zero row, as get_rows_kernel does for f32 / f16.
+// GET_ROWS of a quantised table: unit u is 128 values of output row u / cpr; a warp takes GET_UNITS
+// consecutive ones, all their loads under way before the first is used (the index, then the block, are two
+// memory latencies in a row). An index outside the table records ERR_BAD_INDEX and yields a zero row, as
+// get_rows_kernel does for f32 / f16.
+constexpr int GET_UNITS = 4;
 template <int TYPE>
 __global__ void __launch_bounds__(KV_THREADS) get_rows_q_kernel(const char* __restrict__ src, Dims4 ss,
                                                                const char* __restrict__ idx, Dims4 si,
@@ -207,39 +241,125 @@ __global__ void __launch_bounds__(KV_THREADS) get_rows_q_kernel(const char* __re
                                                                int64_t n_units, int* err) {
     grid_dep_wait();
     grid_dep_launch();
+    constexpr int BYTES = TYPE == KT_Q8_0 ? 34 : 18;
     const int lane = threadIdx.x & 31, q = lane & 7;
-    const int64_t stride = (int64_t)gridDim.x * KV_WARPS;
-    for (int64_t u = (int64_t)blockIdx.x * KV_WARPS + (threadIdx.x >> 5); u < n_units; u += stride) {
-        const int64_t orow = u / cpr;
-        const int64_t e0 = 128 * (u - orow * cpr) + 4 * lane;
-        if (e0 >= ss.ne[0]) continue;
-        const int64_t i10 = orow % si.ne[0], i11 = (orow / si.ne[0]) % si.ne[1], i12 = orow / (si.ne[0] * si.ne[1]);
-        const int64_t r = *reinterpret_cast<const int32_t*>(idx + i10 * si.nb[0] + i11 * si.nb[1] + i12 * si.nb[2]);
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (r < 0 || r >= ss.ne[1]) {
-            if (lane == 0) atomicCAS(err, 0, ERR_BAD_INDEX);
-        } else {
-            constexpr int BYTES = TYPE == KT_Q8_0 ? 34 : 18;
-            const uint16_t* b = reinterpret_cast<const uint16_t*>(src + r * ss.nb[1] + i11 * ss.nb[2] + i12 * ss.nb[3] +
-                                                                  (e0 / 32) * BYTES);
-            const float d = __half2float(__ushort_as_half(__ldg(b)));
-            const int w = TYPE == KT_Q8_0 ? 2 * q : 2 * (q & 3);
-            uint32_t c = (uint32_t)__ldg(b + 1 + w) | ((uint32_t)__ldg(b + 2 + w) << 16);
-            if constexpr (TYPE == KT_Q8_0) {
+    const bool flat = si.ne[1] == 1 && si.ne[2] == 1;      // one index row: no division by its shape
+    const int64_t stride = (int64_t)gridDim.x * KV_WARPS * GET_UNITS;
+    for (int64_t u0 = ((int64_t)blockIdx.x * KV_WARPS + (threadIdx.x >> 5)) * GET_UNITS; u0 < n_units; u0 += stride) {
+        int64_t orow = n_units < (1ll << 31) ? (int64_t)((uint32_t)u0 / (uint32_t)cpr) : u0 / cpr;
+        int c = (int)(u0 - orow * cpr);
+        int64_t r[GET_UNITS], out[GET_UNITS];
+        const uint16_t* b[GET_UNITS];
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = __fmul_rn((float)(int8_t)(c >> (8 * e)), d);
+        for (int n = 0; n < GET_UNITS; n++) {
+            const int64_t e0 = 128ll * c + 4 * lane;
+            out[n] = u0 + n < n_units && e0 < ss.ne[0] ? orow * ss.ne[0] + e0 : -1;
+            r[n] = -1;
+            b[n] = nullptr;
+            if (out[n] >= 0) {
+                int64_t i10 = orow, i11 = 0, i12 = 0;
+                if (!flat) {
+                    i10 = orow % si.ne[0];
+                    i11 = orow / si.ne[0] % si.ne[1];
+                    i12 = orow / (si.ne[0] * si.ne[1]);
+                }
+                r[n] = __ldg(reinterpret_cast<const int32_t*>(idx + i10 * si.nb[0] + i11 * si.nb[1] + i12 * si.nb[2]));
+                b[n] = reinterpret_cast<const uint16_t*>(src + i11 * ss.nb[2] + i12 * ss.nb[3] + (e0 / 32) * BYTES);
+            }
+            if (++c == cpr) c = 0, orow++;
+        }
+        uint32_t d[GET_UNITS], w[GET_UNITS];
+#pragma unroll
+        for (int n = 0; n < GET_UNITS; n++) {
+            d[n] = w[n] = 0;
+            if (out[n] < 0) continue;
+            if (r[n] < 0 || r[n] >= ss.ne[1]) {
+                atomicCAS(err, 0, ERR_BAD_INDEX);
+                out[n] = -2 - out[n];                      // zeros, past the loads
+                continue;
+            }
+            const uint16_t* p = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(b[n]) + r[n] * ss.nb[1]);
+            const int at = TYPE == KT_Q8_0 ? 2 * q : 2 * (q & 3);
+            d[n] = __ldg(p);
+            w[n] = (uint32_t)__ldg(p + 1 + at) | ((uint32_t)__ldg(p + 2 + at) << 16);
+        }
+#pragma unroll
+        for (int n = 0; n < GET_UNITS; n++) {
+            if (out[n] == -1) continue;
+            const bool bad = out[n] < -1;
+            const float f = __half2float(__ushort_as_half((unsigned short)d[n]));
+            const uint32_t x = TYPE == KT_Q8_0 || q < 4 ? w[n] : w[n] >> 4;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int code = TYPE == KT_Q8_0 ? (int)(int8_t)(x >> (8 * e)) : (int)((x >> (8 * e)) & 15u) - 8;
+                v[e] = bad ? 0.0f : __fmul_rn((float)code, f);
+            }
+            float* o = dst + (bad ? -2 - out[n] : out[n]);
+            if (vec_out) {
+                *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
             } else {
-                if (q >= 4) c >>= 4;
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = __fmul_rn((float)((int)((c >> (8 * e)) & 15u) - 8), d);
+                for (int e = 0; e < 4; e++) o[e] = v[e];
             }
         }
-        float* out = dst + orow * ss.ne[0] + e0;
+    }
+}
+
+// The same for rows of at least GET_UNITS units: a warp takes WIDE_UNITS consecutive units of one row, so
+// that the index and the row's address are worked out once and a unit costs three loads and one store.
+constexpr int WIDE_UNITS = 8;
+template <int TYPE>
+__global__ void __launch_bounds__(KV_THREADS) get_rows_q_wide_kernel(const char* __restrict__ src, Dims4 ss,
+                                                                    const char* __restrict__ idx, Dims4 si,
+                                                                    float* __restrict__ dst, int vec_out, int cpr,
+                                                                    int64_t n_rows, int* err) {
+    grid_dep_wait();
+    grid_dep_launch();
+    constexpr int BYTES = TYPE == KT_Q8_0 ? 34 : 18;
+    const int lane = threadIdx.x & 31, q = lane & 7;
+    const int64_t orow = (int64_t)blockIdx.x * KV_WARPS + (threadIdx.x >> 5);
+    if (orow >= n_rows) return;
+    const int c0 = blockIdx.y * WIDE_UNITS;
+    int64_t i10 = orow, i11 = 0, i12 = 0;
+    if (si.ne[1] != 1 || si.ne[2] != 1) {
+        i10 = orow % si.ne[0];
+        i11 = orow / si.ne[0] % si.ne[1];
+        i12 = orow / (si.ne[0] * si.ne[1]);
+    }
+    const int64_t r = __ldg(reinterpret_cast<const int32_t*>(idx + i10 * si.nb[0] + i11 * si.nb[1] + i12 * si.nb[2]));
+    const bool bad = r < 0 || r >= ss.ne[1];
+    if (bad && lane == 0) atomicCAS(err, 0, ERR_BAD_INDEX);
+    const uint16_t* row = reinterpret_cast<const uint16_t*>(src + (bad ? 0 : r) * ss.nb[1] + i11 * ss.nb[2] + i12 * ss.nb[3]);
+    const uint16_t* p = row + ((int64_t)c0 * 4 + (lane >> 3)) * (BYTES / 2);
+    const int at = TYPE == KT_Q8_0 ? 1 + 2 * q : 1 + 2 * (q & 3);
+    const int left = (int)min((int64_t)(WIDE_UNITS * 128), ss.ne[0] - (int64_t)c0 * 128) - 4 * lane;   // values from this lane's first
+    uint32_t d[WIDE_UNITS], w[WIDE_UNITS];
+#pragma unroll
+    for (int n = 0; n < WIDE_UNITS; n++) {
+        d[n] = w[n] = 0;
+        if (128 * n < left && !bad) {
+            d[n] = __ldg(p + 2 * n * BYTES);
+            w[n] = (uint32_t)__ldg(p + 2 * n * BYTES + at) | ((uint32_t)__ldg(p + 2 * n * BYTES + at + 1) << 16);
+        }
+    }
+    float* out = dst + orow * ss.ne[0] + 128ll * c0 + 4 * lane;
+#pragma unroll
+    for (int n = 0; n < WIDE_UNITS; n++) {
+        if (128 * n >= left) break;
+        const float f = __half2float(__ushort_as_half((unsigned short)d[n]));
+        const uint32_t x = TYPE == KT_Q8_0 || q < 4 ? w[n] : w[n] >> 4;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int code = TYPE == KT_Q8_0 ? (int)(int8_t)(x >> (8 * e)) : (int)((x >> (8 * e)) & 15u) - 8;
+            v[e] = bad ? 0.0f : __fmul_rn((float)code, f);
+        }
         if (vec_out) {
-            *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(out + 128 * n) = make_float4(v[0], v[1], v[2], v[3]);
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) out[e] = v[e];
+            for (int e = 0; e < 4; e++) out[128 * n + e] = v[e];
         }
     }
 }
@@ -258,7 +378,19 @@ int get_rows_quant_impl(int src_type, const void* src, const int64_t sne[4], con
         return B200_E_UNSUPPORTED;
     const int cpr = (int)((sne[0] + 127) / 128);
     const int64_t n_units = ine[0] * ine[1] * ine[2] * cpr;
-    const int64_t want = (n_units + KV_WARPS - 1) / KV_WARPS;
+    const int64_t n_rows = ine[0] * ine[1] * ine[2], gx = (n_rows + KV_WARPS - 1) / KV_WARPS;
+    const int gy = (cpr + WIDE_UNITS - 1) / WIDE_UNITS;
+    if (cpr >= GET_UNITS && gx <= INT32_MAX && gy <= 65535) {
+        const int vo = (reinterpret_cast<uintptr_t>(dst) & 15u) == 0 ? 1 : 0;
+        const dim3 wide((unsigned)gx, (unsigned)gy), block(KV_THREADS);
+        const char* ix = reinterpret_cast<const char*>(idx);
+        return launched(src_type == KT_Q8_0
+                            ? launch_pdl(get_rows_q_wide_kernel<KT_Q8_0>, wide, block, 0, st, static_cast<const char*>(src),
+                                         dims_of(sne, snb), ix, dims_of(ine, inb), dst, vo, cpr, n_rows, dev_err)
+                            : launch_pdl(get_rows_q_wide_kernel<KT_Q4_0>, wide, block, 0, st, static_cast<const char*>(src),
+                                         dims_of(sne, snb), ix, dims_of(ine, inb), dst, vo, cpr, n_rows, dev_err));
+    }
+    const int64_t want = (n_units + KV_WARPS * GET_UNITS - 1) / (KV_WARPS * GET_UNITS);
     const unsigned grid = (unsigned)std::min<int64_t>(want, (int64_t)device_sm_count() * 32);
     const int vec = (reinterpret_cast<uintptr_t>(dst) & 15u) == 0 ? 1 : 0;
     const char* s = static_cast<const char*>(src);
@@ -298,11 +430,11 @@ int b200_set_rows(const float* src, const int64_t sne[4], const size_t snb[4], i
     const bool vec = sne[0] % 4 == 0 && ((snb[1] | snb[2] | snb[3]) & 15) == 0 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0;
     const int cpr = (int)((sne[0] + 127) / 128);
     const int64_t n_units = sne[1] * cpr;
-    // more units a warp once every SM has its CTAs, so that long calls scan their indices less often
+    // more units a warp once every SM has its four CTAs: fewer scans of the indices, more loads in flight
     int upw = 1;
-    while (upw < KV_MAX_UNITS && n_units / (KV_WARPS * upw) > (int64_t)device_sm_count() * 16) upw *= 2;
+    while (upw < KV_MAX_UNITS && n_units / (KV_WARPS * upw) > (int64_t)device_sm_count() * 4) upw *= 2;
     const int64_t gx = (n_units + (int64_t)KV_WARPS * upw - 1) / ((int64_t)KV_WARPS * upw);
-    if (gx > INT32_MAX) return B200_E_UNSUPPORTED;
+    if (n_units > INT32_MAX - 1024 || sne[2] * sne[3] > INT32_MAX) return B200_E_UNSUPPORTED;
     const dim3 grid((unsigned)gx, (unsigned)std::min<int64_t>(sne[2] * sne[3], 65535)), block(KV_THREADS);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     auto go = [&](auto kernel) {

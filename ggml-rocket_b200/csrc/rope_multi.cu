@@ -32,7 +32,7 @@ namespace {
 constexpr int RM_THREADS = 256;
 constexpr int RM_TABLE = 1024;      // (token, pair) entries of a CTA's cosine / sine table
 constexpr int RM_MAX_TOKENS = 16;   // tokens a CTA takes at most
-constexpr int RM_U = 2;             // items a thread holds in registers at a time
+constexpr int RM_U = 4;             // items (16 bytes of either half) a thread has in flight
 
 struct RopeMulti {
     const char* x;
@@ -43,11 +43,13 @@ struct RopeMulti {
     int heads, dim, pairs, gap, tpc;   // tpc: tokens a CTA
     int s[4];
     int mode;
-    double freq_scale, log2_base_step;   // log2(base) * -2 / n_dims
+    double first;                   // half turns a position of pair step 0: freq_scale / pi
+    double power[10];               // base^(-2 2^k / n_dims): a step's frequency is the product over its bits
     float attn_factor;
 };
 
-__device__ __forceinline__ float2 angle_cos_sin(const RopeMulti& a, int i, int64_t tok) {
+// Pair i's axis and its angle a token position, in half turns.
+__device__ __forceinline__ double half_turns_per_position(const RopeMulti& a, int i, int* axis_out) {
     const int total = a.s[0] + a.s[1] + a.s[2] + a.s[3];
     const int sector = i % total;
     const int b1 = a.s[0], b2 = b1 + a.s[1], b3 = b2 + a.s[2];
@@ -59,43 +61,57 @@ __device__ __forceinline__ float2 angle_cos_sin(const RopeMulti& a, int i, int64
         axis = sector < b1 ? 0 : sector < b2 ? 1 : sector < b3 ? 2 : 3;
         if (a.mode == 24) step = sector - (axis == 0 ? 0 : axis == 1 ? b1 : axis == 2 ? b2 : b3);
     }
-    const double f = exp2((double)step * a.log2_base_step) * a.freq_scale;
-    const double half_turns = (double)__ldg(a.pos + (int64_t)axis * a.tokens + tok) * f * 0.31830988618379067154;
-    const float r = (float)(half_turns - 2.0 * rint(0.5 * half_turns));   // in [-1, 1]
-    float sn, cs;
-    sincospif(r, &sn, &cs);
-    return make_float2(cs * a.attn_factor, sn * a.attn_factor);
+    *axis_out = axis;
+    // ten 64-bit products at most, where a 64-bit exp2 is a chain of some sixty operations
+    double f = a.first;
+#pragma unroll
+    for (int k = 0; k < 10; k++)
+        if (step >> k & 1) f *= a.power[k];
+    return f;
 }
 
-// V consecutive values as f32
+// V consecutive values of type T: 16 bytes, or one value
 template <typename T, int V>
 struct Pack {
-    float v[V];
+    uint32_t w[V == 1 ? 1 : 4];
     __device__ __forceinline__ void load(const char* p) {
-        if constexpr (V == 1) {
-            v[0] = (float)*reinterpret_cast<const T*>(p);
+        if constexpr (V > 1) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
         } else if constexpr (sizeof(T) == 4) {
-            const float4 w = *reinterpret_cast<const float4*>(p);
-            v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
         } else {
-            const uint4 w = *reinterpret_cast<const uint4*>(p);
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+            w[0] = *reinterpret_cast<const uint16_t*>(p);
+        }
+    }
+    __device__ __forceinline__ void store(char* p) const {
+        if constexpr (V > 1) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        else if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+        else *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+    }
+    __device__ __forceinline__ void get(float (&v)[V]) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int k = 0; k < V; k++) v[k] = __uint_as_float(w[k]);
+        } else if constexpr (V == 1) {
+            v[0] = __half2float(__ushort_as_half((unsigned short)w[0]));
+        } else {
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
                 v[2 * k] = f.x, v[2 * k + 1] = f.y;
             }
         }
     }
-    __device__ __forceinline__ void store(char* p) const {
-        if constexpr (V == 1) {
-            if constexpr (sizeof(T) == 4) *reinterpret_cast<float*>(p) = v[0];
-            else *reinterpret_cast<__half*>(p) = __float2half_rn(v[0]);
-        } else if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    __device__ __forceinline__ void set(const float (&v)[V]) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int k = 0; k < V; k++) w[k] = __float_as_uint(v[k]);
+        } else if constexpr (V == 1) {
+            w[0] = __half_as_ushort(__float2half_rn(v[0]));
         } else {
-            *reinterpret_cast<uint4*>(p) = make_uint4(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]),
-                                                      pack_half2(v[4], v[5]), pack_half2(v[6], v[7]));
+#pragma unroll
+            for (int k = 0; k < 4; k++) w[k] = pack_half2(v[2 * k], v[2 * k + 1]);
         }
     }
 };
@@ -103,7 +119,7 @@ struct Pack {
 // V: values a vector access moves (16 bytes), or 1 where rows are not 16-byte aligned or pairs do not
 // divide by it.
 template <typename T, int V>
-__global__ void __launch_bounds__(RM_THREADS) rope_multi_kernel(const RopeMulti a) {
+__global__ void __launch_bounds__(RM_THREADS, 4) rope_multi_kernel(const RopeMulti a) {
     grid_dep_wait();
     grid_dep_launch();
     __shared__ float2 table[RM_TABLE];
@@ -129,8 +145,16 @@ __global__ void __launch_bounds__(RM_THREADS) rope_multi_kernel(const RopeMulti 
             hi[u].load(p + a.gap * (int64_t)sizeof(T));
         }
         if (!made) {
-            for (int e = threadIdx.x; e < n_tok * a.pairs; e += RM_THREADS)
-                table[e] = angle_cos_sin(a, e % a.pairs, tok0 + e / a.pairs);
+            int last = -1, axis = 0;
+            double rate = 0.0;
+            for (int e = threadIdx.x; e < n_tok * a.pairs; e += RM_THREADS) {
+                const int tk = e / a.pairs, i = e - tk * a.pairs;
+                if (i != last) rate = half_turns_per_position(a, i, &axis), last = i;
+                const double turns = (double)__ldg(a.pos + (int64_t)axis * a.tokens + tok0 + tk) * rate;
+                float sn, cs;
+                sincospif((float)(turns - 2.0 * rint(0.5 * turns)), &sn, &cs);   // of a value in [-1, 1]
+                table[e] = make_float2(cs * a.attn_factor, sn * a.attn_factor);
+            }
             __syncthreads();
             made = true;
         }
@@ -139,16 +163,20 @@ __global__ void __launch_bounds__(RM_THREADS) rope_multi_kernel(const RopeMulti 
             const int it = base + u * RM_THREADS + (int)threadIdx.x;
             if (it >= n) continue;
             const int tk = it / per_tok, rest = it - tk * per_tok, h = rest / ppr, j = (rest - h * ppr) * V;
-            Pack<T, V> y0, y1;
+            float x0[V], x1[V], y0[V], y1[V];
+            lo[u].get(x0);
+            hi[u].get(x1);
 #pragma unroll
             for (int e = 0; e < V; e++) {
                 const float2 c = table[tk * a.pairs + j + e];
-                y0.v[e] = lo[u].v[e] * c.x - hi[u].v[e] * c.y;
-                y1.v[e] = lo[u].v[e] * c.y + hi[u].v[e] * c.x;
+                y0[e] = x0[e] * c.x - x1[e] * c.y;
+                y1[e] = x0[e] * c.y + x1[e] * c.x;
             }
+            lo[u].set(y0);
+            hi[u].set(y1);
             char* p = d + (((int64_t)tk * a.heads + h) * a.dim + j) * (int64_t)sizeof(T);
-            y0.store(p);
-            y1.store(p + a.gap * (int64_t)sizeof(T));
+            lo[u].store(p);
+            hi[u].store(p + a.gap * (int64_t)sizeof(T));
         }
     }
     const int m = n_tok * a.heads * tail;
@@ -198,12 +226,13 @@ int b200_rope_multi(int type, const void* x, const int64_t ne[4], const size_t n
     a.heads = (int)ne[1], a.dim = (int)ne[0], a.pairs = (int)pairs, a.gap = (int)pairs;
     for (int i = 0; i < 4; i++) a.s[i] = sections[i];
     a.mode = mode;
-    a.freq_scale = (double)freq_scale;
-    a.log2_base_step = -2.0 * log2((double)freq_base) / (double)n_dims;
+    a.first = (double)freq_scale * 0.31830988618379067154;
+    const double l2 = -2.0 * log2((double)freq_base) / (double)n_dims;
+    for (int k = 0; k < 10; k++) a.power[k] = exp2(l2 * (double)(1 << k));
     a.attn_factor = attn_factor;
-    // tokens a CTA: enough items for its threads, as far as the table holds them
+    // tokens a CTA: enough items and enough angles for its threads, as far as the table holds them
     const int64_t items = ne[1] * (pairs / (vec ? vw : 1));
-    int64_t tpc = std::max<int64_t>(1, (int64_t)RM_THREADS * RM_U / items);
+    int64_t tpc = std::max<int64_t>({1, (int64_t)RM_THREADS * RM_U / items, RM_THREADS / pairs});
     tpc = std::min({tpc, (int64_t)RM_MAX_TOKENS, (int64_t)RM_TABLE / pairs, ne[2]});
     while (tpc > 1 && (ne[2] + tpc - 1) / tpc * ne[3] < device_sm_count()) tpc = (tpc + 1) / 2;
     a.tpc = (int)tpc;

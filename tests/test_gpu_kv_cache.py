@@ -54,7 +54,7 @@ def values(rng, rows, n):
 
 @pytest.mark.parametrize("kind", [Q4_0, Q8_0])
 @pytest.mark.parametrize("n,n_rows,total", [(32, 1, 1), (64, 7, 9), (96, 33, 50), (1024, 1, 300), (1024, 512, 700),
-                                            (128, 3000, 3001), (2080, 65, 80)])
+                                            (128, 3000, 3001), (2080, 65, 80), (480, 21, 40), (5120, 3, 4)])
 def test_write_and_read_back(cuda, kind, n, n_rows, total):
     import torch
     import ggml_b200 as g
