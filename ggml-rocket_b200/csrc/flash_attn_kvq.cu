@@ -56,6 +56,8 @@ constexpr int KR_THREADS = 32 * KR_WARPS;
 constexpr int KR_KEYS = 32;            // a warp takes at a time
 constexpr int KR_BOX = 144;            // bytes of a key's row in a TMA tile
 constexpr int KR_MAX_TILES = 1024;     // tiles of a CTA's range (its list of live tiles)
+constexpr int KR_MAX_CLUSTER = 8;       // CTAs that join their parts through each other's shared memory
+constexpr int KR_DEAD = 0x8000;         // of a list entry: a masked tile that was fetched all the same
 constexpr int64_t KR_WAVES = 6;
 constexpr int64_t KR_MIN_SPLIT = 2048;   // keys of a part, where they are many
 // More query rows a KV head than this go to the tcgen05 kernel over fp16 tiles of the cache: the row kernel
@@ -76,10 +78,11 @@ struct KvqArgs {
     int m_vec;                         // rows 16-byte aligned
     void* dst;                         // [S][T][H][D]
     int dst_f16;
-    float* part;                       // [S][HK][rows][splits][D] outputs, then 3 floats a part
+    float* part;                       // [S][T][H][splits / cluster][D] outputs, then 3 floats a part
     float* stat;                       // {max (log2 units, relative), sum, mask reference}
     int T, H, KV, HK, G, S;
-    int splits, tiles_per_split;
+    int splits, tiles_per_split;       // CTAs that share a row's keys, and their ranges
+    int cluster;                       // CTAs of a cluster
     float scale, softcap;
     int* err;
 };
@@ -94,6 +97,11 @@ template <int BYTES>
 __device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool valid) {
     const int n = valid ? BYTES : 0;   // bytes behind n are zero-filled
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t a) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -175,7 +183,8 @@ struct KrCfg {
     static constexpr int OFF_LIST = OFF_BAR + 16 * STAGES + 16;
     static constexpr int SMEM = OFF_LIST + KR_MAX_TILES * 2;
     static constexpr int OUT = (KR_ROWS * D + 2 * KR_ROWS) * 4;   // a warp's result, in the ring's place
-    static_assert(KR_WARPS * OUT <= RING && OFF_BAR % 8 == 0 && OFF_Q % 16 == 0 && HALF % 128 == 0);
+    static constexpr int OFF_CTA = KR_WARPS * OUT;             // the CTA's: [head][row][D], then {max, sum} of each
+    static_assert(OFF_CTA + HPB * KR_ROWS * (D + 2) * 4 <= RING && OFF_CTA % 16 == 0 && OFF_BAR % 8 == 0 && OFF_Q % 16 == 0 && HALF % 128 == 0);
 };
 
 // MT: the most tokens a CTA's rows come from (1 or 8). MODE: 0 f16 q and result (q has no low half), 1 f16
@@ -190,6 +199,7 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     extern __shared__ __align__(128) uint8_t sm[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const int packs = a.HK / HPB;
+    const int crank = (int)(blockIdx.x % a.cluster);     // the CTA's rank in its cluster
     const int split = blockIdx.x, pack = blockIdx.y % packs, rt = blockIdx.y / packs, str = blockIdx.z;
     const int rows_all = a.T * a.G, row0 = rt * KR_ROWS;
     const int rows = min(KR_ROWS, rows_all - row0);
@@ -197,7 +207,7 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     const int n_tiles = (a.KV + C::TK - 1) / C::TK;
     const int tile0 = split * a.tiles_per_split, tile1 = min(n_tiles, tile0 + a.tiles_per_split);
     const int range = max(0, tile1 - tile0);
-    uint16_t* list = reinterpret_cast<uint16_t*>(sm + C::OFF_LIST);
+    uint16_t* list = reinterpret_cast<uint16_t*>(sm + C::OFF_LIST);          // tiles from tile0; KR_DEAD: masked
     float* refs = reinterpret_cast<float*>(sm + C::OFF_REF);               // [warp][8], then per row
     float* backs = reinterpret_cast<float*>(sm + C::OFF_BACK);             // [head][row]
     uint4* q_frag = reinterpret_cast<uint4*>(sm + C::OFF_Q);               // [head][k-step][lane]
@@ -221,65 +231,49 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     grid_dep_wait();
     grid_dep_launch();
 
+    // TMA: one thread brings tiles into the CTA's stages
+    int sent = 0;
+    auto send = [&](int tile, int st) {
+        const uint32_t d = smem_u32(sm) + st * C::STAGE;
+        mbar_arrive_expect_tx(full(st), C::STAGE);
+        tma_load_3d(d, &tm_k, full(st), pack * KR_BOX, tile * C::TK, str);
+        tma_load_3d(d + C::HALF, &tm_v, full(st), pack * KR_BOX, tile * C::TK, str);
+        sent++;
+    };
+    // The first tiles are under way before the mask says whether they are live (one that is not is waited for
+    // and passed over): a range of few tiles is all latency.
+    const int early = C::TMA ? min(range, C::STAGES - 1) : 0;
+    if (C::TMA && threadIdx.x == 0)
+        for (int i = 0; i < early; i++) send(tile0 + i, i);
+
     // ---- q (warp i: head i of the CTA): high and low halves of the row, times a power of two that brings
     // its maximum to 2^10, in shared memory for every warp of the head, a k-step at a time ----
-    if (warp < HPB) {
-        const int r = row0 + g;
-        const bool in = g < rows;
-        const int t = in ? r / a.G : 0, h = (pack * HPB + warp) * a.G + (in ? r - t * a.G : 0);
+    uint4 q_raw[2 * C::NB];                              // values 16 i + 4 t4 .. + 3 of row g, as they are stored
+#pragma unroll
+    for (int i = 0; i < 2 * C::NB; i++) q_raw[i] = make_uint4(0, 0, 0, 0);
+    if (warp < HPB && g < rows) {
+        const int t = (row0 + g) / a.G, h = (pack * HPB + warp) * a.G + row0 + g - t * a.G;
         const char* qp = a.q + (int64_t)str * a.q_s + (int64_t)t * a.q_t + (int64_t)h * a.q_h;
-        float x[C::NB][8];
-        float amax = 0.0f;
+        if (a.q_vec && a.q_f16) {
 #pragma unroll
-        for (int b = 0; b < C::NB; b++)
-#pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                const int d = 32 * b + 4 * e + 4 * t4;   // values 32 b + {0, 16} + 4 t4 ..
-#pragma unroll
-                for (int n = 0; n < 4; n++) x[b][e + n] = 0.0f;
-                if (!in) continue;
-                if (a.q_vec) {
-                    if (a.q_f16) {
-                        const uint2 v = *reinterpret_cast<const uint2*>(qp + 2 * d);
-                        const float2 lo = h2f(v.x), hi = h2f(v.y);
-                        x[b][e] = lo.x, x[b][e + 1] = lo.y, x[b][e + 2] = hi.x, x[b][e + 3] = hi.y;
-                    } else {
-                        const float4 v = *reinterpret_cast<const float4*>(qp + 4 * d);
-                        x[b][e] = v.x, x[b][e + 1] = v.y, x[b][e + 2] = v.z, x[b][e + 3] = v.w;
-                    }
-                } else {
-#pragma unroll
-                    for (int n = 0; n < 4; n++)
-                        x[b][e + n] = a.q_f16 ? __half2float(reinterpret_cast<const __half*>(qp)[d + n])
-                                              : reinterpret_cast<const float*>(qp)[d + n];
-                }
+            for (int i = 0; i < 2 * C::NB; i++) {
+                const uint2 v = *reinterpret_cast<const uint2*>(qp + 2 * (16 * i + 4 * t4));
+                q_raw[i].x = v.x, q_raw[i].y = v.y;
             }
+        } else if (a.q_vec) {
 #pragma unroll
-        for (int b = 0; b < C::NB; b++)
+            for (int i = 0; i < 2 * C::NB; i++) q_raw[i] = *reinterpret_cast<const uint4*>(qp + 4 * (16 * i + 4 * t4));
+        } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[b][e]));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        int ex = 0;
-        if (amax > 0.0f && amax <= 3.402823466e38f) frexpf(amax, &ex);
-        ex = max(-100, ex - 10);
-        const float mul = ldexpf(1.0f, -ex);
-        if (t4 == 0) backs[warp * KR_ROWS + g] = ldexpf(a.scale, ex);   // what undoes it, with the scale
+            for (int i = 0; i < 2 * C::NB; i++) {
+                uint32_t w[4];
 #pragma unroll
-        for (int b = 0; b < C::NB; b++)
-#pragma unroll
-            for (int st = 0; st < 2; st++) {             // k-step 2b + st: values 16 st + {0, 2}, then {1, 3}
-                float hi[4], lo[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float v = x[b][4 * st + e] * mul;
-                    hi[e] = __half2float(__float2half_rn(v));
-                    lo[e] = v - hi[e];
-                }
-                q_frag[(warp * 2 * C::NB + 2 * b + st) * 32 + lane] =
-                    make_uint4(pack_half2(hi[0], hi[2]), pack_half2(lo[0], lo[2]), pack_half2(hi[1], hi[3]),
-                               pack_half2(lo[1], lo[3]));
+                for (int n = 0; n < 4; n++)
+                    w[n] = a.q_f16 ? (uint32_t)reinterpret_cast<const uint16_t*>(qp)[16 * i + 4 * t4 + n]
+                                   : reinterpret_cast<const uint32_t*>(qp)[16 * i + 4 * t4 + n];
+                q_raw[i] = a.q_f16 ? make_uint4(w[0] | (w[1] << 16), w[2] | (w[3] << 16), 0, 0) : make_uint4(w[0], w[1], w[2], w[3]);
             }
+        }
     }
 
     // ---- the range's mask: live tiles and each token's largest mask value; eight keys a lane where the
@@ -324,26 +318,65 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             if (lane == 0) refs[warp * KR_ROWS + k] = top[k];
         }
     }
-    __syncthreads();
-    float ref_of[MT];                                    // the largest mask value, per token
+    // ---- q's halves ----
+    if (warp < HPB) {
+        float x[C::NB][8];
+        float amax = 0.0f;
 #pragma unroll
-    for (int k = 0; k < MT; k++) {
-        float r = -INFINITY;
-        if (mbase && k < n_tok)
+        for (int i = 0; i < 2 * C::NB; i++) {
+            const uint4 w = q_raw[i];
+            const float2 lo = h2f(w.x), hi = h2f(w.y);
+            float* d = &x[i >> 1][4 * (i & 1)];
+            d[0] = a.q_f16 ? lo.x : __uint_as_float(w.x);
+            d[1] = a.q_f16 ? lo.y : __uint_as_float(w.y);
+            d[2] = a.q_f16 ? hi.x : __uint_as_float(w.z);
+            d[3] = a.q_f16 ? hi.y : __uint_as_float(w.w);
+        }
 #pragma unroll
-            for (int w = 0; w < C::WARPS; w++) r = fmaxf(r, refs[w * KR_ROWS + k]);
-        ref_of[k] = fabsf(r) <= 65504.0f ? r : 0.0f;     // all masked (or an infinite mask): nothing to gain
+        for (int b = 0; b < C::NB; b++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[b][e]));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        int ex = 0;
+        if (amax > 0.0f && amax <= 3.402823466e38f) frexpf(amax, &ex);
+        ex = max(-100, ex - 10);
+        const float mul = ldexpf(1.0f, -ex);
+        if (t4 == 0) backs[warp * KR_ROWS + g] = ldexpf(a.scale, ex);   // what undoes it, with the scale
+#pragma unroll
+        for (int b = 0; b < C::NB; b++)
+#pragma unroll
+            for (int st = 0; st < 2; st++) {             // k-step 2b + st: values 16 st + {0, 2}, then {1, 3}
+                float hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float v = x[b][4 * st + e] * mul;
+                    hi[e] = __half2float(__float2half_rn(v));
+                    lo[e] = v - hi[e];
+                }
+                q_frag[(warp * 2 * C::NB + 2 * b + st) * 32 + lane] =
+                    make_uint4(pack_half2(hi[0], hi[2]), pack_half2(lo[0], lo[2]), pack_half2(hi[1], hi[3]),
+                               pack_half2(lo[1], lo[3]));
+            }
     }
+    __syncthreads();
     const int my_tok = MT == 1 ? 0 : min(row0 + g, rows_all - 1) / a.G - t_first;   // of this lane's row (g)
-    float* row_ref = refs + C::WARPS * KR_ROWS;
+    float* row_ref = refs + C::WARPS * KR_ROWS;          // per token, then per row
+    if (mbase && threadIdx.x < MT) {
+        float r = -INFINITY;
+        if ((int)threadIdx.x < n_tok)
+#pragma unroll
+            for (int w = 0; w < C::WARPS; w++) r = fmaxf(r, refs[w * KR_ROWS + threadIdx.x]);
+        row_ref[threadIdx.x] = r;
+    }
     if (mbase) {
         if (warp == C::WARPS - 1) {                      // the live tiles in order, in place
             int n = 0;
             for (int i0 = 0; i0 < range; i0 += 32) {
                 const int i = i0 + lane;
-                const bool on = i < range && list[i] != 0;
+                const bool is = i < range && list[i] != 0, on = is || i < early;
                 const uint32_t votes = __ballot_sync(0xffffffffu, on);
-                if (on) list[n + __popc(votes & ((1u << lane) - 1u))] = (uint16_t)i;
+                if (on) list[n + __popc(votes & ((1u << lane) - 1u))] = (uint16_t)(i | (is ? 0 : KR_DEAD));
                 n += __popc(votes);
                 __syncwarp();
             }
@@ -353,14 +386,20 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         for (int i = threadIdx.x; i < range; i += C::THREADS) list[i] = (uint16_t)i;
         if (threadIdx.x == 0) *n_live = range;
     }
+    __syncthreads();
+    const int live = *n_live;
+    float ref_of[MT];                                    // the largest mask value, per token
+#pragma unroll
+    for (int k = 0; k < MT; k++) {
+        const float r = mbase ? row_ref[k] : 0.0f;
+        ref_of[k] = fabsf(r) <= 65504.0f ? r : 0.0f;     // all masked (or an infinite mask): nothing to gain
+    }
     if (warp == 0 && t4 == 0) {
         float r = ref_of[0];
 #pragma unroll
         for (int k = 1; k < MT; k++) r = my_tok == k ? ref_of[k] : r;
-        row_ref[g] = r;
+        refs[g] = r;                                     // the warps' maxima have been read: per row from here on
     }
-    __syncthreads();
-    const int live = *n_live;
 
     // ---- a warp's 32 keys of every live tile ----
     const int hs = warp % HPB, part = warp / HPB;        // its head of the CTA's, its keys of the tile's
@@ -393,19 +432,9 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         }
         cp_async_commit();
     };
-    // TMA: one thread brings live tile e into a stage of the CTA's
-    int sent = 0;
-    auto send = [&](int st) {
-        if (sent >= live) return;
-        const int key0 = (tile0 + list[sent++]) * C::TK;
-        const uint32_t d = smem_u32(sm) + st * C::STAGE;
-        mbar_arrive_expect_tx(full(st), C::STAGE);
-        tma_load_3d(d, &tm_k, full(st), pack * KR_BOX, key0, str);
-        tma_load_3d(d + C::HALF, &tm_v, full(st), pack * KR_BOX, key0, str);
-    };
     if constexpr (C::TMA) {
         if (threadIdx.x == 0)
-            for (int i = 0; i < C::STAGES - 1; i++) send(i);
+            while (sent < min(live, C::STAGES - 1)) send(tile0 + (list[sent] & ~KR_DEAD), sent);
     } else {
 #pragma unroll
         for (int i = 0; i < C::STAGES - 1; i++) fetch(i, i);
@@ -421,7 +450,7 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 
     // the lane's key's mask bits in live tile e, per token; 0xfc00 (-inf) where there is no such key
     auto load_mask = [&](int e, uint16_t (&m)[MT]) {
-        const int key = e < live ? (tile0 + list[e]) * C::TK + part * KR_KEYS + lane : a.KV;
+        const int key = e < live ? (tile0 + (list[e] & ~KR_DEAD)) * C::TK + part * KR_KEYS + lane : a.KV;
 #pragma unroll
         for (int k = 0; k < MT; k++) {
             m[k] = key < a.KV ? 0 : 0xfc00;
@@ -433,6 +462,7 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 
     int stage = 0;
     uint32_t phase = 0;
+    bool gave_up = false;
     for (int e = 0; e < live; e++) {
         bool seen = false;
 #pragma unroll
@@ -448,13 +478,19 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             // the tile STAGES - 1 on, into the stage every warp has left behind
             if (threadIdx.x == 0) {
                 const int prev = stage == 0 ? C::STAGES - 1 : stage - 1;
-                if (e > 0 && sent < live &&
+                if (e > 0 && sent < live && !gave_up &&
                     !mbar_wait(empty(prev), stage == 0 ? phase ^ 1u : phase, a.err, ERR_WAIT_PRODUCER, abort_flag))
-                    sent = live;                         // an abort: the other waits end on its flag
-                send(prev);
+                    gave_up = true;                      // the other waits end on the abort flag
+                if (sent < live && !gave_up) send(tile0 + list[sent], prev);
             }
             __syncwarp();
             if (!mbar_wait(full(stage), phase, a.err, ERR_WAIT_STREAM, abort_flag)) break;
+            if (list[e] & KR_DEAD) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty(stage));
+                if (++stage == C::STAGES) stage = 0, phase ^= 1u;
+                continue;
+            }
             ks = ring + stage * C::STAGE + part * KR_KEYS * C::PITCH + hs * (18 * C::NB);
         } else {
             cp_async_wait<C::STAGES - 2>();
@@ -646,38 +682,93 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         wout[KR_ROWS * D + KR_ROWS + g] = run_sum;
     }
     cta_sync();
-    for (int i = threadIdx.x; i < HPB * rows * D; i += KR_THREADS) {
-        const int d = i % D, r = (i / D) % rows, head = i / (D * rows);
-        const float* first = reinterpret_cast<const float*>(sm + head * C::OUT);
-        constexpr int STEP = HPB * C::OUT / 4;           // to the head's next warp
-        float m = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < C::PARTS; w++) m = fmaxf(m, first[w * STEP + KR_ROWS * D + r]);
-        const float base = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f, acc = 0.0f;
-#pragma unroll
-        for (int w = 0; w < C::PARTS; w++) {
-            const float* p = first + w * STEP;
-            const float f = ex2(p[KR_ROWS * D + r] - base);
-            l = fmaf(p[KR_ROWS * D + KR_ROWS + r], f, l);
-            acc = fmaf(p[r * D + d], f, acc);
-        }
+    // A thread takes value d of rows r0, r0 + 128 / D, ..; rows are numbered 8 head + r here, those from `rows`
+    // on of each head left out.
+    float* cta_out = reinterpret_cast<float*>(sm + C::OFF_CTA);
+    float* cta_stat = cta_out + HPB * KR_ROWS * D;
+    constexpr int SIDE = KR_THREADS / D;
+    const int d = threadIdx.x % D, r0 = threadIdx.x / D;
+    const int parts = a.splits / a.cluster;
+    // value d of a row: the result, or one part of it
+    auto emit = [&](int head, int r, float acc, float l, float m, float ref) {
         const int row = row0 + r, t = row / a.G, h = (pack * HPB + head) * a.G + row - t * a.G;
         const int64_t at = ((int64_t)str * a.T + t) * a.H + h;
-        if (a.splits == 1) {
+        if (parts == 1) {
             const float y = l == 0.0f ? 0.0f : acc / l;
             if (a.dst_f16) static_cast<__half*>(a.dst)[at * D + d] = __float2half_rn(y);
             else static_cast<float*>(a.dst)[at * D + d] = y;
         } else {
-            const int64_t p = at * a.splits + split;
+            const int64_t p = at * parts + split / a.cluster;
             a.part[p * D + d] = acc;
             if (d == 0) {
                 a.stat[3 * p] = m;
                 a.stat[3 * p + 1] = l;
-                a.stat[3 * p + 2] = row_ref[r];
+                a.stat[3 * p + 2] = ref;
+            }
+        }
+    };
+#pragma unroll
+    for (int head = 0; head < HPB; head++) {
+        const float* first = reinterpret_cast<const float*>(sm + head * C::OUT);
+        constexpr int STEP = HPB * C::OUT / 4;           // to the head's next warp
+#pragma unroll 4
+        for (int r = r0; r < rows; r += SIDE) {
+            float m = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < C::PARTS; w++) m = fmaxf(m, first[w * STEP + KR_ROWS * D + r]);
+            const float base = m == -INFINITY ? 0.0f : m;
+            float l = 0.0f, acc = 0.0f;
+#pragma unroll
+            for (int w = 0; w < C::PARTS; w++) {
+                const float* p = first + w * STEP;
+                const float f = ex2(p[KR_ROWS * D + r] - base);
+                l = fmaf(p[KR_ROWS * D + KR_ROWS + r], f, l);
+                acc = fmaf(p[r * D + d], f, acc);
+            }
+            if (a.cluster == 1) {
+                emit(head, r, acc, l, m, refs[r]);
+            } else {
+                cta_out[(head * KR_ROWS + r) * D + d] = acc;
+                if (d == 0) cta_stat[2 * (head * KR_ROWS + r)] = m, cta_stat[2 * (head * KR_ROWS + r) + 1] = l;
             }
         }
     }
+    if (a.cluster == 1) return;
+    cluster_sync();
+
+    // ---- join the CTAs of the cluster, its rows shared out; maxima are compared as maximum plus mask
+    // reference, their differences formed apart, where they are exact ----
+    for (int hr = crank + r0 * a.cluster; hr < HPB * KR_ROWS; hr += SIDE * a.cluster) {
+        const int r = hr % KR_ROWS;
+        if (r >= rows) continue;
+        float top = -INFINITY, m_best = 0.0f, r_best = 0.0f;
+        float l_of[KR_MAX_CLUSTER], e_of[KR_MAX_CLUSTER], ref_at[KR_MAX_CLUSTER], x[KR_MAX_CLUSTER];
+#pragma unroll
+        for (int c = 0; c < KR_MAX_CLUSTER; c++) {
+            l_of[c] = 0.0f, e_of[c] = ref_at[c] = x[c] = 0.0f;
+            if (c >= a.cluster) continue;
+            const uint32_t st = mapa_shared(smem_u32(cta_stat + 2 * hr), c);
+            e_of[c] = ld_cluster_f32(st);
+            l_of[c] = ld_cluster_f32(st + 4);
+            ref_at[c] = ld_cluster_f32(mapa_shared(smem_u32(refs + r), c));
+            x[c] = ld_cluster_f32(mapa_shared(smem_u32(cta_out + hr * D + d), c));
+        }
+#pragma unroll
+        for (int c = 0; c < KR_MAX_CLUSTER; c++) {
+            const float v = e_of[c] + ref_at[c] * KR_LOG2E;
+            if (l_of[c] != 0.0f && v > top) top = v, m_best = e_of[c], r_best = ref_at[c];
+        }
+        float l = 0.0f, acc = 0.0f;
+#pragma unroll
+        for (int c = 0; c < KR_MAX_CLUSTER; c++) {
+            // l is 0 where no key is seen
+            const float f = l_of[c] == 0.0f ? 0.0f : ex2((e_of[c] - m_best) + (ref_at[c] - r_best) * KR_LOG2E);
+            l = fmaf(l_of[c], f, l);
+            acc = fmaf(x[c], f, acc);
+        }
+        emit(hr / KR_ROWS, r, acc, l, m_best, r_best);
+    }
+    cluster_sync();                                      // no CTA leaves while a peer reads its memory
 }
 
 // Joins the parts of a row: one CTA per (stream, token, head), its four warps taking the parts in turn.
@@ -740,7 +831,7 @@ __global__ void __launch_bounds__(128) kvq_join_kernel(const float* __restrict__
 
 struct KvqPlan {
     int heads;                                   // KV heads a CTA takes (1: the cp.async kernel)
-    int splits, tiles_per_split;
+    int splits, tiles_per_split, cluster;
     size_t part_off, stat_off, total;
 };
 
@@ -751,21 +842,40 @@ KvqPlan kvq_plan(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_
     const int64_t tk = KR_KEYS * KR_WARPS / p.heads;
     const int64_t rows = T * (H / HK), tiles = (KV + tk - 1) / tk;
     const int64_t ctas = S * (HK / p.heads) * ((rows + KR_ROWS - 1) / KR_ROWS);
-    // Three CTAs fit an SM. One wave of them when the keys are few; several where they are many, with at
-    // least KR_MIN_SPLIT keys each, so that streams of unequal length even out.
-    const int64_t slots = (int64_t)device_sm_count() * 3;
-    int64_t splits = std::max<int64_t>(1, slots / ctas);
-    splits = std::max(splits, std::min(KR_WAVES * slots / ctas, tiles * tk / KR_MIN_SPLIT));
-    splits = std::min(splits, tiles);
+    // Three CTAs fit an SM, seven eighths of that when they come in clusters. Where it leaves a CTA no more
+    // than four tiles, or where a row's keys are spread over sixteen CTAs or more, clusters join the parts
+    // (one stream x 16384 keys 24.2 -> 18.1 us, x 512 keys 9.3 -> 8.4). Otherwise CTAs stand alone: clusters
+    // wait for their slowest and for room in one GPC (32 streams x 16384 keys 167 us alone, 202 in clusters).
+    // Then one wave when the keys are few, several where they are many, with at least KR_MIN_SPLIT keys each,
+    // so that streams of unequal length even out.
+    const int64_t slots = (int64_t)device_sm_count() * 3, fit = slots * 7 / 8;
+    int64_t splits = 0;
+    p.cluster = 1;
+    for (int c = KR_MAX_CLUSTER; c > 1; c /= 2)
+        if (ctas * c <= fit && (tiles + c - 1) / c <= 4 && tiles > c / 2) {
+            p.cluster = c;
+            splits = c;
+            break;
+        }
+    if (!splits && ctas * 2 * KR_MAX_CLUSTER <= fit && tiles >= 2 * KR_MAX_CLUSTER) {
+        p.cluster = KR_MAX_CLUSTER;
+        splits = std::min(fit / ctas, tiles) / p.cluster * p.cluster;
+    }
+    if (!splits) {
+        splits = std::max<int64_t>(1, slots / ctas);
+        splits = std::max(splits, std::min(KR_WAVES * slots / ctas, tiles * tk / KR_MIN_SPLIT));
+        splits = std::min(splits, tiles);
+    }
     splits = std::max(splits, (tiles + KR_MAX_TILES - 1) / KR_MAX_TILES);
     const int64_t per = (tiles + splits - 1) / splits;
-    splits = (tiles + per - 1) / per;
+    splits = ((tiles + per - 1) / per + p.cluster - 1) / p.cluster * p.cluster;
     p.splits = (int)splits;
     p.tiles_per_split = (int)per;
+    const int64_t parts = splits / p.cluster;
     auto al = [](size_t x) { return (x + 255) & ~(size_t)255; };
     p.part_off = 0;
-    p.stat_off = splits > 1 ? al((size_t)(S * T * H * splits * D) * 4) : 0;
-    p.total = splits > 1 ? p.stat_off + al((size_t)(S * T * H * splits) * 12) : 256;
+    p.stat_off = parts > 1 ? al((size_t)(S * T * H * parts * D) * 4) : 0;
+    p.total = parts > 1 ? p.stat_off + al((size_t)(S * T * H * parts) * 12) : 256;
     return p;
 }
 
@@ -805,7 +915,7 @@ cudaError_t launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const KvqA
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) set[dev] = true;
     }
-    return launch_pdl(kvq_rows_kernel<D, MT, MODE, HPB>, grid, dim3(C::THREADS), C::SMEM, st, tk, tv, a);
+    return launch_pdl_cluster(kvq_rows_kernel<D, MT, MODE, HPB>, grid, dim3(C::THREADS), C::SMEM, st, a.cluster, tk, tv, a);
 }
 
 template <int D, int HPB>
@@ -822,9 +932,10 @@ cudaError_t launch_kvq(const CUtensorMap& tk, const CUtensorMap& tv, const KvqAr
     else
         e = mode == 0 ? launch_rows<D, 8, 0, HPB>(tk, tv, a, grid, st)
           : mode == 1 ? launch_rows<D, 8, 1, HPB>(tk, tv, a, grid, st) : launch_rows<D, 8, 2, HPB>(tk, tv, a, grid, st);
-    if (e != cudaSuccess || a.splits == 1) return e;
+    const int parts = a.splits / a.cluster;
+    if (e != cudaSuccess || parts == 1) return e;
     return launch_pdl(kvq_join_kernel<D>, dim3((unsigned)((int64_t)a.S * a.T * a.H)), dim3(128), 0, st,
-                      (const float*)a.part, (const float*)a.stat, a.splits, a.dst_f16, a.dst);
+                      (const float*)a.part, (const float*)a.stat, parts, a.dst_f16, a.dst);
 }
 
 bool kvq_dims_ok(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S) {
@@ -917,7 +1028,7 @@ int b200_flash_attn_kvq(int kv_type, int q_type, const void* q, const int64_t qn
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.part_off);
     a.stat = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.stat_off);
     a.T = (int)T, a.H = (int)H, a.KV = (int)KV, a.HK = (int)HK, a.G = (int)(H / HK), a.S = (int)S;
-    a.splits = p.splits, a.tiles_per_split = p.tiles_per_split;
+    a.splits = p.splits, a.tiles_per_split = p.tiles_per_split, a.cluster = p.cluster;
     a.scale = scale, a.softcap = softcap;
     a.err = dev_err;
     CUtensorMap tk{}, tv{};
