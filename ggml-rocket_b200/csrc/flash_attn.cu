@@ -883,9 +883,9 @@ struct FaQuantLayout {
 static FaQuantLayout fa_quant_layout(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S) {
     FaQuantLayout Q{};
     Q.L = fa_layout((int)D, (int)T, (int)H, (int)KV, (int)HK);
-    // few query tiles: the keys split until the SMs are filled twice, at least four blocks a part
+    // few query tiles: the keys split as far as the SMs hold a part each, at least four blocks a part
     const int64_t tiles = S * Q.L.n_hg * Q.L.n_tb;
-    int64_t splits = std::max<int64_t>(1, 2 * device_sm_count() / tiles);
+    int64_t splits = std::max<int64_t>(1, device_sm_count() / tiles);
     splits = std::min<int64_t>(splits, std::max<int64_t>(1, Q.L.n_kvb / 4));
     Q.kvb_per_split = (int)((Q.L.n_kvb + splits - 1) / splits);
     Q.splits = (Q.L.n_kvb + Q.kvb_per_split - 1) / Q.kvb_per_split;
