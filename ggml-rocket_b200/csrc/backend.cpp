@@ -139,8 +139,10 @@ int flash_attn_min_kv() {
     static const int kv = [] { const int x = knob_int("B200_FLASH_ATTN_MIN_KV", 1024); return x < 1 ? 1 : x; }();
     return kv;
 }
-// FLASH_ATTN_EXT over a quantized KV cache (Q8_0 / Q4_0 K or V): converted to fp16 tiles, then the
-// fp16 kernel (b200_kv_to_f16). Off by default: the reference declines these (F16 K / V only).
+// FLASH_ATTN_EXT over a quantized KV cache. Q4_0 K and V in device memory: read as they are stored, any
+// number of tokens and streams (b200_flash_attn_kvq). Otherwise Q8_0 / Q4_0 K or V converted to fp16
+// tiles, then the fp16 kernel (b200_kv_to_f16). Off by default: the reference declines these (F16 K / V
+// only).
 bool fa_quant_kv_on() {
     static const bool v = knob_on("B200_FA_QUANT_KV", false);
     return v;
@@ -160,7 +162,7 @@ bool fuse_on() {
     static const bool v = knob_on("B200_FUSE", true);
     return v;
 }
-// The glue ops (RMS_NORM, ADD, MUL, SILU, SWIGLU, ROPE, GET_ROWS, CPY). Off by default: the
+// The glue ops (RMS_NORM, ADD, MUL, SILU, SWIGLU, ROPE, GET_ROWS, SET_ROWS, CPY). Off by default: the
 // reference claims none of them; B200_GLUE=1 keeps a layer's activations on the device.
 bool glue_on() {
     static const bool v = knob_on("B200_GLUE", false);
@@ -178,12 +180,13 @@ size_t weight_budget_bytes(int device) {
 // tensor helpers (ggml semantics)
 // ------------------------------------------------------------------------------------------------
 
-enum : int { T_F32 = 0, T_F16 = 1, T_Q4_0 = 2, T_Q8_0 = 8, T_Q4_K = 12, T_Q6_K = 14, T_I32 = 26, T_BF16 = 30 };
+enum : int { T_F32 = 0, T_F16 = 1, T_Q4_0 = 2, T_Q8_0 = 8, T_Q4_K = 12, T_Q6_K = 14, T_I32 = 26, T_I64 = 27, T_BF16 = 30 };
 
 int64_t blck_size(int t) { return (t == T_Q8_0 || t == T_Q4_0) ? 32 : (t == T_Q4_K || t == T_Q6_K) ? 256 : 1; }
 size_t type_size(int t) {
     switch (t) {
         case T_F32: case T_I32: return 4;
+        case T_I64: return 8;
         case T_F16: case T_BF16: return 2;
         case T_Q4_0: return 18;   // a KV-cache type only (FLASH_ATTN_EXT); no weight route
         case T_Q8_0: return 34;
@@ -949,6 +952,32 @@ bool op_outputs_done(b200_backend* b, const std::vector<const b200_tensor*>& out
 static bool same_shape(const b200_tensor* a, const b200_tensor* b) {
     return a->ne[0] == b->ne[0] && a->ne[1] == b->ne[1] && a->ne[2] == b->ne[2] && a->ne[3] == b->ne[3];
 }
+// ggml's rope modes with sections: MROPE, VISION, IMROPE (b200_rope_multi)
+static bool rope_sections_mode(int mode) { return mode == 8 || mode == 24 || mode == 40; }
+static bool rope_multi_supported(const b200_tensor* op) {
+    const b200_tensor* a = op->src[0];
+    const b200_tensor* b = op->src[1];
+    const int n_dims = op->op_params[1], mode = op->op_params[2];
+    if (!b || op->src[2] || (a->type != T_F32 && a->type != T_F16) || op->type != a->type || b->type != T_I32 ||
+        !is_contiguous(op) || !same_shape(a, op) || !is_contiguous(b) || a->ne[3] != 1 || b->ne[0] != 4 * a->ne[2])
+        return false;
+    int64_t sum = 0;
+    for (int i = 0; i < 4; i++) {
+        const int sec = op->op_params[11 + i];
+        if (sec < 0 || sec > 65536) return false;
+        sum += sec;
+    }
+    const size_t es = type_size(a->type);
+    const int64_t pairs = mode == 24 ? n_dims : n_dims / 2;
+    return sum > 0 && n_dims > 0 && n_dims % 2 == 0 && n_dims <= a->ne[0] && (mode != 24 || 2 * (int64_t)n_dims == a->ne[0]) &&
+           pairs <= 1024 && a->ne[0] <= 4096 && a->ne[1] <= 65536 && a->nb[0] == es &&
+           (a->nb[1] | a->nb[2] | a->nb[3]) % es == 0 && op_param_f32(op, 7) == 0.0f && op_param_f32(op, 5) > 0.0f;
+}
+// A quantised cache type the device reads and writes row by row, its rows whole blocks.
+static bool kv_block_type(const b200_tensor* t) {
+    return (t->type == T_Q8_0 || t->type == T_Q4_0) && t->ne[0] % 32 == 0 && t->nb[0] == type_size(t->type) &&
+           (t->nb[1] | t->nb[2] | t->nb[3]) % 2 == 0 && (uintptr_t)t->data % 2 == 0;
+}
 static bool glue_supported(const b200_tensor* op) {
     const b200_tensor* a = op->src[0];
     const b200_tensor* b = op->src[1];
@@ -982,15 +1011,30 @@ static bool glue_supported(const b200_tensor* op) {
         }
         case B200_OP_ROPE: {
             const int n_dims = op->op_params[1], mode = op->op_params[2];
+            if (rope_sections_mode(mode)) return rope_multi_supported(op);
             return b && !op->src[2] && a->type == T_F32 && op->type == T_F32 && b->type == T_I32 &&
                    is_contiguous(op) && same_shape(a, op) && a->ne[3] == 1 && b->ne[0] == a->ne[2] &&
                    a->ne[0] % 2 == 0 && n_dims > 0 && n_dims % 2 == 0 && n_dims <= a->ne[0] &&
                    (mode == 0 || mode == 2) && op_param_f32(op, 7) == 0.0f && op_param_f32(op, 5) > 0.0f;
         }
         case B200_OP_GET_ROWS:
-            return b && (a->type == T_F32 || a->type == T_F16) && b->type == T_I32 && op->type == T_F32 &&
+            // quantised tables only where they already lie in device memory (a KV cache): a token
+            // embedding in host memory would be copied whole for a few rows
+            return b && (a->type == T_F32 || a->type == T_F16 || (kv_block_type(a) && a->on_device)) && b->type == T_I32 && op->type == T_F32 &&
                    is_contiguous(op) && op->ne[0] == a->ne[0] && op->ne[1] == b->ne[0] && op->ne[2] == b->ne[1] &&
                    op->ne[3] == b->ne[2] && b->ne[3] == 1 && b->ne[1] <= a->ne[2] && b->ne[2] <= a->ne[3];
+        case B200_OP_SET_ROWS: {
+            // op: the cache tensor itself (its rows that no index names stay as they are, so it has to lie
+            // in device memory); a: the new rows; b: their indices
+            const size_t unit = op->type == T_F32 ? 4 : 2;
+            return b && op->on_device && a->type == T_F32 && (b->type == T_I64 || b->type == T_I32) &&
+                   (op->type == T_F32 || op->type == T_F16 || kv_block_type(op)) && op->nb[0] == type_size(op->type) &&
+                   (op->nb[1] | op->nb[2] | op->nb[3]) % unit == 0 && (uintptr_t)op->data % unit == 0 && a->nb[0] == 4 &&
+                   (a->nb[1] | a->nb[2] | a->nb[3]) % 4 == 0 && (b->nb[0] | b->nb[1] | b->nb[2]) % type_size(b->type) == 0 &&
+                   a->ne[0] == op->ne[0] && a->ne[2] == op->ne[2] && a->ne[3] == op->ne[3] && b->ne[0] == a->ne[1] &&
+                   b->ne[1] > 0 && b->ne[2] > 0 && a->ne[2] % b->ne[1] == 0 && a->ne[3] % b->ne[2] == 0 && b->ne[3] == 1 &&
+                   a->ne[1] > 0 && a->ne[0] <= ((int64_t)1 << 30) && (a->ne[0] + 127) / 128 * a->ne[1] < ((int64_t)1 << 30);
+        }
         case B200_OP_SOFT_MAX:   // no mask, no ALiBi slope, no sinks
             return !b && !op->src[2] && a->type == T_F32 && op->type == T_F32 && is_contiguous(op) &&
                    same_shape(a, op) && op_param_f32(op, 1) == 0.0f;
@@ -1009,6 +1053,30 @@ static bool glue_supported(const b200_tensor* op) {
         default:
             return false;
     }
+}
+
+// FLASH_ATTN_EXT over Q4_0 K and V in device memory (b200_flash_attn_kvq): any number of tokens, keys and
+// streams. The floors of the fp16 route weigh copies between host and device, which such a cache has none of.
+static bool fa_kvq(const b200_tensor* op) {
+    const b200_tensor* q = op->src[0];
+    const b200_tensor* k = op->src[1];
+    const b200_tensor* v = op->src[2];
+    const b200_tensor* m = op->src[3];
+    if (!fa_quant_kv_on() || op->src[4] || op_param_f32(op, 1) != 0.0f) return false;
+    const int64_t D = q->ne[0], T = q->ne[1], H = q->ne[2], S = q->ne[3], KV = k->ne[1], HK = k->ne[2];
+    const size_t qe = type_size(q->type), unit = (size_t)D / 16;
+    if ((D != 64 && D != 128) || (q->type != T_F32 && q->type != T_F16)) return false;
+    auto cache_ok = [&](const b200_tensor* t) {
+        return t->type == T_Q4_0 && t->on_device && t->nb[0] == 18 && t->ne[0] == D && t->ne[1] == KV && t->ne[2] == HK &&
+               t->ne[3] == S && (t->nb[1] | t->nb[2] | t->nb[3]) % unit == 0 && (uintptr_t)t->data % unit == 0;
+    };
+    return T > 0 && T <= 65536 && S > 0 && S <= 65535 && HK > 0 && H > 0 && H % HK == 0 && KV > 0 &&
+           KV <= ((int64_t)1 << 30) && q->nb[0] == qe && (q->nb[1] | q->nb[2] | q->nb[3]) % qe == 0 && cache_ok(k) &&
+           cache_ok(v) && op->type == T_F32 && is_contiguous(op) && op->ne[0] == D && op->ne[1] == H && op->ne[2] == T &&
+           op->ne[3] == S && (!op->on_device || (uintptr_t)op->data % 16 == 0) && S * T * H <= INT32_MAX / 4 &&
+           T * (H / HK) <= (1 << 20) && HK * ((T * (H / HK) + 7) / 8) <= 65535 &&
+           (!m || (m->type == T_F16 && m->nb[0] == 2 && is_contiguous(m) && m->ne[0] >= KV && m->ne[1] >= T && m->ne[2] == 1 &&
+                   (m->ne[3] == S || m->ne[3] == 1)));
 }
 
 extern "C" bool ggml_backend_b200_supports_op(const b200_tensor* op) {
@@ -1086,6 +1154,7 @@ extern "C" bool ggml_backend_b200_supports_op(const b200_tensor* op) {
             if (!flash_attn_on() || !q || !k || !v) return false;
             if (!m && !flash_attn_unmasked()) return false;
             if (op->src[4]) return false;   // attention sinks: a different softmax (ggml-rocket.cpp:7703-7721)
+            if (fa_kvq(op)) return true;
             const float max_bias = op_param_f32(op, 1);
             const int64_t D = q->ne[0], T = q->ne[1], H = q->ne[2], DV = v->ne[0];
             const int64_t KV = k->ne[1], HK = k->ne[2];
@@ -1114,6 +1183,7 @@ extern "C" bool ggml_backend_b200_supports_op(const b200_tensor* op) {
         case B200_OP_GLU:
         case B200_OP_ROPE:
         case B200_OP_GET_ROWS:
+        case B200_OP_SET_ROWS:
         case B200_OP_CPY:
         case B200_OP_SOFT_MAX:
         case B200_OP_ARGSORT:
@@ -1159,8 +1229,8 @@ bool graph_finish(b200_backend* b) {
     if (h == 0) return true;
     if (h == B200_DEV_BAD_IDS) {
         logf("E", "graph_compute: a MUL_MAT_ID expert id outside [0, n_expert)\n");
-    } else if (h == 6) {   // the kernels' bounds-check code (GET_ROWS row index outside the table)
-        logf("E", "graph_compute: a GET_ROWS row index outside its table\n");
+    } else if (h == 6) {   // the kernels' bounds-check code (a GET_ROWS or SET_ROWS row index outside its table)
+        logf("E", "graph_compute: a GET_ROWS or SET_ROWS row index outside its table\n");
         b->device_errors++;
     } else {
         logf("E", "graph_compute: device error word %d\n", h);
@@ -1586,7 +1656,37 @@ int do_rope_cpy(b200_backend* b, const b200_tensor* r, const b200_tensor* c) {
     return B200_OK;
 }
 
+int do_flash_attn_kvq(b200_backend* b, b200_tensor* op) {
+    const b200_tensor* q = op->src[0];
+    const b200_tensor* k = op->src[1];
+    const b200_tensor* v = op->src[2];
+    const b200_tensor* m = op->src[3];
+    OpStaging stg;
+    stg.ins = {q, k, v, m};
+    stg.outs = {op};
+    const size_t need = b200_flash_attn_kvq_workspace_size(q->ne[0], q->ne[1], q->ne[2], k->ne[1], k->ne[2], q->ne[3]);
+    if (!op_reserve(b, stg)) return B200_E_CUDA;
+    if (!grow(&b->ws, &b->ws_bytes, need, b->stream)) return B200_E_CUDA;
+    bool ok = true;
+    const void* qd = stage_in(b, q, &ok);
+    const void* kd = stage_in(b, k, &ok);
+    const void* vd = stage_in(b, v, &ok);
+    const void* md = m ? stage_in(b, m, &ok) : nullptr;
+    char* dd = stage_out(b, op, false, &ok);
+    if (!ok || !op_inputs_ready(b)) return B200_E_CUDA;
+    const size_t mnb[4] = {2, m ? m->nb[1] : 0, 0, m && m->ne[3] > 1 ? m->nb[3] : 0};
+    const int rc = b200_flash_attn_kvq(k->type, q->type, qd, q->ne, q->nb, kd, k->ne, k->nb, vd, v->ne, v->nb, md, mnb,
+                                       op->type, dd, op_param_f32(op, 0), op_param_f32(op, 2), b->ws, b->ws_bytes, b->dev_err,
+                                       b->stream);
+    if (rc != B200_OK) return rc;
+    if (!op_outputs_done(b, stg.outs, {dd})) return B200_E_CUDA;
+    b->route_ops["fa"]++;
+    b->route_ops["fa_kvq"]++;
+    return B200_OK;
+}
+
 int do_flash_attn(b200_backend* b, b200_tensor* op) {
+    if (fa_kvq(op)) return do_flash_attn_kvq(b, op);
     const b200_tensor* q = op->src[0];
     const b200_tensor* k = op->src[1];
     const b200_tensor* v = op->src[2];
@@ -1697,13 +1797,23 @@ int do_glue(b200_backend* b, const b200_tensor* op) {
             break;
         }
         case B200_OP_ROPE:
+            if (rope_sections_mode(op->op_params[2])) {
+                rc = b200_rope_multi(a->type, sa, a->ne, a->nb, reinterpret_cast<const int32_t*>(sc), op->op_params[1],
+                                     op->op_params[2], &op->op_params[11], op_param_f32(op, 5), op_param_f32(op, 6),
+                                     op_param_f32(op, 8), d, st);
+                break;
+            }
             rc = b200_rope(reinterpret_cast<const float*>(sa), a->ne, a->nb, reinterpret_cast<const int32_t*>(sc),
                            op->op_params[1], op->op_params[2], op_param_f32(op, 5), op_param_f32(op, 6),
                            op_param_f32(op, 8), df, st);
             break;
         case B200_OP_GET_ROWS:
-            rc = b200_get_rows(a->type == T_F16 ? 1 : 0, sa, a->ne, a->nb, reinterpret_cast<const int32_t*>(sc), c->ne,
+            rc = b200_get_rows(a->type, sa, a->ne, a->nb, reinterpret_cast<const int32_t*>(sc), c->ne,
                                c->nb, df, b->dev_err, st);
+            break;
+        case B200_OP_SET_ROWS:
+            rc = b200_set_rows(reinterpret_cast<const float*>(sa), a->ne, a->nb, c->type, sc, c->ne, c->nb, op->type, d,
+                               op->ne, op->nb, b->dev_err, st);
             break;
         case B200_OP_CPY:
             rc = b200_cpy(a->type == T_F16 ? 1 : 0, sa, a->ne, a->nb, op->type == T_F16 ? 1 : 0, d, op->ne, op->nb, st);
@@ -1923,7 +2033,7 @@ int ggml_backend_b200_op_from_name(const char* name) {
         {"MUL_MAT_ID", B200_OP_MUL_MAT_ID}, {"FLASH_ATTN_EXT", B200_OP_FLASH_ATTN_EXT},
         {"RMS_NORM", B200_OP_RMS_NORM}, {"ADD", B200_OP_ADD},   {"MUL", B200_OP_MUL},
         {"UNARY", B200_OP_UNARY},       {"GLU", B200_OP_GLU},   {"ROPE", B200_OP_ROPE},
-        {"GET_ROWS", B200_OP_GET_ROWS}, {"CPY", B200_OP_CPY},   {"SOFT_MAX", B200_OP_SOFT_MAX},
+        {"GET_ROWS", B200_OP_GET_ROWS}, {"SET_ROWS", B200_OP_SET_ROWS}, {"CPY", B200_OP_CPY},   {"SOFT_MAX", B200_OP_SOFT_MAX},
         {"ARGSORT", B200_OP_ARGSORT},   {"SUM_ROWS", B200_OP_SUM_ROWS}, {"DIV", B200_OP_DIV},
     };
     for (const auto& e : map)
@@ -2184,6 +2294,7 @@ int ggml_backend_b200_graph_compute(b200_backend_t b, b200_tensor* const* nodes,
             case B200_OP_GLU:
             case B200_OP_ROPE:
             case B200_OP_GET_ROWS:
+            case B200_OP_SET_ROWS:
             case B200_OP_CPY:
             case B200_OP_SOFT_MAX:
             case B200_OP_ARGSORT:

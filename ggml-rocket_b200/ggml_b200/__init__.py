@@ -193,7 +193,7 @@ def mul_mat_plan(M, N, K, wtype=F16):
 
 OP_NONE, OP_RESHAPE, OP_VIEW, OP_PERMUTE, OP_TRANSPOSE, OP_MUL_MAT, OP_MUL_MAT_ID, OP_FLASH_ATTN_EXT, OP_OTHER = range(9)
 OP_RMS_NORM, OP_ADD, OP_MUL, OP_UNARY, OP_GLU, OP_ROPE, OP_GET_ROWS, OP_CPY = range(9, 17)
-OP_SOFT_MAX, OP_ARGSORT, OP_SUM_ROWS, OP_DIV = range(17, 21)
+OP_SOFT_MAX, OP_ARGSORT, OP_SUM_ROWS, OP_DIV, OP_SET_ROWS = range(17, 22)
 UNARY_SILU, GLU_SWIGLU = 1, 2
 STATUS_SUCCESS, STATUS_FAILED = 0, -1
 PREC_F32, PREC_BF16, PREC_F16, PREC_Q8, PREC_Q4 = 10, 15, 20, 30, 40
@@ -358,7 +358,7 @@ _SIGS.update({
 
 
 def _elem_size(t):
-    be, bb = BLOCK.get(t, (1, 4 if t == I32 else 0))
+    be, bb = BLOCK.get(t, (1, 4 if t == I32 else 8 if t == I64 else 0))
     return bb / be
 
 
@@ -372,7 +372,7 @@ def make_tensor(t, ne, data=None, op=OP_NONE, srcs=(), name="", on_device=False,
     for i in range(4):
         x.ne[i] = int(ne[i])
     if nb is None:
-        be, bb = BLOCK.get(t, (1, 4 if t == I32 else 4))
+        be, bb = BLOCK.get(t, (1, 8 if t == I64 else 4))
         nb0 = bb if be == 1 else bb
         nb1 = (ne[0] // be) * bb
         nb = [nb0, nb1, nb1 * ne[1], nb1 * ne[1] * ne[2]]

@@ -52,6 +52,7 @@ typedef enum {
     B200_OP_ARGSORT,     /* op_params[0]: 0 ascending, 1 descending (ggml_sort_order) */
     B200_OP_SUM_ROWS,
     B200_OP_DIV,
+    B200_OP_SET_ROWS,    /* the node is the cache itself; src[0] the new rows, src[1] their indices (B200_GLUE=1) */
 } b200_op;
 
 /* Sub-ops of UNARY and GLU, which a ggml adapter maps by name (ggml_unary_op_name /
