@@ -37,6 +37,12 @@ constexpr int FA_THREADS = 64 + 32 * FA_SOFTMAX_WARPS;   // warp 0 TMA, warp 1 M
 constexpr float FA_RESCALE_LOG2 = 8.0f;   // rescale O only when the row max grows by more than 2^8
 enum : uint8_t { MF_MIXED = 0, MF_ZERO = 1, MF_MASKED = 2 };
 
+// How the query tiles are shared out: CTAs below `whole` take a tile and all its keys; behind them come
+// `cut` CTAs a tile, with `per` key blocks each.
+struct FaUnits {
+    int whole, cut, per;
+};
+
 struct FaArgs {
     const float* qscale;       // [H*T] per-row divisor (1 unless out of fp16 range)
     const uint16_t* mask;      // F16 mask or nullptr
@@ -50,16 +56,23 @@ struct FaArgs {
     // the extended form only (several streams, parts of the keys, f16 results; q16 not scaled)
     int64_t m_stream;          // mask stride of a stream, elements
     float scale;
-    int splits, kvb_per_split;
+    FaUnits units;
     int dst_f16;
-    float* part;               // [S][T][H][splits][DV] outputs not divided by their sums (splits > 1)
-    float* stat;               // {max in log2 units, sum, 0} of every part
+    float* part;               // [unit - whole][rows of a unit][DV] outputs not divided by their sums
+    float* stat;               // {max in log2 units, sum} of each of their rows
 };
 
 __device__ __forceinline__ float ex2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// cap * tanh(s / cap) through one exponential and one reciprocal, within cap * 2^-21: inlined into an unrolled
+// loop, the library's tanhf makes code that the instruction cache does not hold.
+__device__ __forceinline__ float capped(float s, float cap, float inv_cap) {
+    const float t = ex2_approx(s * inv_cap * 2.885390082f);          // e^(2 s / cap)
+    return cap - 2.0f * cap * __frcp_rn(1.0f + t);
 }
 
 // Shared-memory descriptor of an MN-major operand in 128-byte-swizzled rows: 64 MN elements per
@@ -236,8 +249,19 @@ struct FaCfg {
     static constexpr uint32_t IDESC_O = idesc_f16_f32_bmn(FA_ROWS, DV);
 };
 
-// EXT: streams in blockIdx.y (heads of q16 and of K / V numbered stream by stream), a part of the keys in
-// blockIdx.z, scores scaled after the product, a key whose mask is -inf left out whatever its score.
+// A CTA's tile (numbered stream by stream, heavier token blocks first) and its range of key blocks.
+struct FaUnit {
+    int tile, first, end, slot;     // slot: of its part, -1 for a whole tile
+};
+__device__ __forceinline__ FaUnit fa_unit(const FaUnits& u, int n_kvb) {
+    const int b = (int)blockIdx.x;
+    if (b < u.whole) return {b, 0, n_kvb, -1};
+    const int i = b - u.whole, piece = i % u.cut;
+    return {u.whole + i / u.cut, min(n_kvb, piece * u.per), min(n_kvb, (piece + 1) * u.per), i};
+}
+
+// EXT: several streams (heads of q16 and of K / V numbered stream by stream), tiles whose keys CTAs share,
+// scores scaled after the product, a key whose mask is -inf left out whatever its score.
 template <int D, int DV, bool EXT>
 __global__ void __launch_bounds__(FA_THREADS, 1)
 fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -265,14 +289,15 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // heavier (later) token blocks first
-    const int tb = args.n_tb - 1 - (int)(blockIdx.x / args.n_hg);
-    const int hg = (int)(blockIdx.x % args.n_hg);
+    const int per_stream = EXT ? args.n_tb * args.n_hg : 0;
+    const FaUnit un = EXT ? fa_unit(args.units, args.n_kvb) : FaUnit{(int)blockIdx.x, 0, args.n_kvb, -1};
+    const int str = EXT ? un.tile / per_stream : 0, tile = EXT ? un.tile % per_stream : un.tile;
+    const int tb = args.n_tb - 1 - tile / args.n_hg;
+    const int hg = tile % args.n_hg;
     const int G = args.H / args.HK;
     const int hk = (hg * args.GP) / G;
-    const int str = EXT ? (int)blockIdx.y : 0;
     const uint8_t* flags = args.flags + ((int64_t)str * args.n_tb + tb) * args.n_kvb;
-    const int j_first = EXT ? (int)blockIdx.z * args.kvb_per_split : 0;
-    const int j_end = EXT ? min(args.n_kvb, j_first + args.kvb_per_split) : args.n_kvb;
+    const int j_first = un.first, j_end = un.end;
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
@@ -464,7 +489,7 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
             const uint8_t fl = flags[j];
             if (fl == MF_MASKED) continue;
             const bool use_mask = (fl == MF_MIXED) && (mrow != nullptr);
-            const bool general = use_mask || softcap != 0.0f || (j + 1) * FA_KB > args.KV;
+            const bool general = use_mask || softcap != 0.0f || (j + 1) * FA_KB > args.KV || (EXT && !(args.scale >= 0.0f));
             const int s = i & 1;
             const uint32_t ph = (uint32_t)(i >> 1) & 1u;
             if (!mbar_wait(s_full(s), ph, args.err, ERR_WAIT_EPILOGUE, abort_flag)) { ok = false; break; }
@@ -496,7 +521,7 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
 #pragma unroll
                     for (int e = 0; e < 32; e++) {
                         float sv = x[c0 + e] * qs;
-                        if (softcap != 0.0f) sv = softcap * tanhf(sv / softcap);
+                        if (softcap != 0.0f) sv = EXT ? capped(sv, softcap, 1.0f / softcap) : softcap * tanhf(sv / softcap);
                         sv *= LOG2E;
                         if (use_mask) {
                             const uint32_t mw = (&mv[e >> 3].x)[(e & 7) >> 1];
@@ -584,14 +609,12 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
         for (int k = 0; k < FA_SPLIT; k++) l_tot += sums[k];
         if constexpr (EXT) {
             if (ok) {                                    // tcgen05.ld is a whole warp's: rows past T load too
-                const int64_t row = ((int64_t)str * args.T + t) * args.H + h;
-                const bool whole = args.splits == 1;
-                const int64_t at = whole ? row : row * args.splits + blockIdx.z;
+                const bool whole = un.slot < 0;
+                const int64_t at = whole ? ((int64_t)str * args.T + t) * args.H + h : (int64_t)un.slot * FA_ROWS + r;
                 const float inv = whole ? 1.0f / l_tot : 1.0f;
-                if (!whole && pt == 0 && row_valid) {
-                    args.stat[3 * at] = m;
-                    args.stat[3 * at + 1] = l_tot;
-                    args.stat[3 * at + 2] = 0.0f;
+                if (!whole && pt == 0) {
+                    args.stat[2 * at] = m;
+                    args.stat[2 * at + 1] = l_tot;
                 }
 #pragma unroll
                 for (int c0 = 0; c0 < OPT; c0 += 16) {
@@ -603,7 +626,7 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
                     float y[16];
 #pragma unroll
                     for (int e = 0; e < 16; e++) y[e] = have_o && l_tot != 0.0f ? __uint_as_float(ov[e]) * inv : 0.0f;
-                    if (!row_valid) {
+                    if (whole && !row_valid) {
                     } else if (whole && args.dst_f16) {
                         uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<__half*>(args.dst) + at * DV + pt * OPT + c0);
                         out[0] = make_uint4(pack_half2(y[0], y[1]), pack_half2(y[2], y[3]), pack_half2(y[4], y[5]), pack_half2(y[6], y[7]));
@@ -644,6 +667,50 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, C::TMEM_COLS);
+    }
+}
+
+// Joins the parts of the tiles that several CTAs shared: one warp per row of such a tile.
+template <int D>
+__global__ void __launch_bounds__(256) fa_join_kernel(const FaArgs args, int n_rows) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const int id = (int)(blockIdx.x * 8 + (threadIdx.x >> 5)), lane = threadIdx.x & 31;
+    if (id >= n_rows) return;
+    const int cut_tile = id / FA_ROWS, r = id % FA_ROWS;
+    const int gt = args.units.whole + cut_tile, per_stream = args.n_tb * args.n_hg;
+    const int str = gt / per_stream, tile = gt % per_stream;
+    const int tb = args.n_tb - 1 - tile / args.n_hg;
+    const int t = tb * args.TQ + r % args.TQ, h = tile % args.n_hg * args.GP + r / args.TQ;
+    if (t >= args.T) return;
+    const int cut = args.units.cut;
+    const int64_t first = (int64_t)cut_tile * cut * FA_ROWS + r;   // of part k: + k * FA_ROWS
+    float top = -INFINITY;
+    for (int k = lane; k < cut; k += 32) {
+        const float* st = args.stat + 2 * (first + (int64_t)k * FA_ROWS);
+        if (st[1] != 0.0f) top = fmaxf(top, st[0]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (top == -INFINITY) top = 0.0f;
+    constexpr int PER = D / 32;
+    float acc[PER] = {}, l_all = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < cut; k++) {
+        const int64_t at = first + (int64_t)k * FA_ROWS;
+        const float l = args.stat[2 * at + 1];
+        const float f = l == 0.0f ? 0.0f : ex2_approx(args.stat[2 * at] - top);   // l is 0 where no key is seen
+        l_all = fmaf(l, f, l_all);
+        const float* p = args.part + at * D + lane * PER;
+#pragma unroll
+        for (int e = 0; e < PER; e++) acc[e] = fmaf(p[e], f, acc[e]);
+    }
+    const int64_t at = (((int64_t)str * args.T + t) * args.H + h) * D + lane * PER;
+#pragma unroll
+    for (int e = 0; e < PER; e++) {
+        const float y = l_all == 0.0f ? 0.0f : acc[e] / l_all;
+        if (args.dst_f16) reinterpret_cast<__half*>(args.dst)[at + e] = __float2half_rn(y);
+        else args.dst[at + e] = y;
     }
 }
 
@@ -876,19 +943,30 @@ __global__ void __launch_bounds__(256) fa_quant_prep_kernel(const FaQuantPrep a)
 
 struct FaQuantLayout {
     FaLayout L;
-    int splits, kvb_per_split;
+    int cut_tiles;              // tiles whose keys CTAs share
+    FaUnits units;
     size_t q16_off, qs_off, flags_off, k_off, v_off, part_off, stat_off, total;
 };
 
 static FaQuantLayout fa_quant_layout(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S) {
     FaQuantLayout Q{};
     Q.L = fa_layout((int)D, (int)T, (int)H, (int)KV, (int)HK);
-    // few query tiles: the keys split as far as the SMs hold a part each, at least four blocks a part
-    const int64_t tiles = S * Q.L.n_hg * Q.L.n_tb;
-    int64_t splits = std::max<int64_t>(1, device_sm_count() / tiles);
-    splits = std::min<int64_t>(splits, std::max<int64_t>(1, Q.L.n_kvb / 4));
-    Q.kvb_per_split = (int)((Q.L.n_kvb + splits - 1) / splits);
-    Q.splits = (Q.L.n_kvb + Q.kvb_per_split - 1) / Q.kvb_per_split;
+    // Whole tiles for as many full waves as there are; the tiles left over are cut into pieces of at least
+    // four key blocks, so that their waves take the least time. In key blocks: the pieces' waves, then about
+    // four for the join's launch and one for every 5.6 MB of parts it writes and reads.
+    const int64_t tiles = S * Q.L.n_hg * Q.L.n_tb, sms = device_sm_count();
+    const int64_t left = tiles % sms, part = D * 8 * FA_ROWS;
+    int cut = 1;
+    double best = left ? (double)Q.L.n_kvb : 0.0;
+    for (int64_t k = 2; left && k <= 64 && Q.L.n_kvb >= 4 * k; k++) {
+        const double cost = (double)((left * k + sms - 1) / sms * ((Q.L.n_kvb + k - 1) / k)) + 4.0 + (double)(left * k * part) / 5.6e6;
+        if (cost < best) best = cost, cut = (int)k;
+    }
+    Q.cut_tiles = cut > 1 ? (int)left : 0;
+    Q.units.whole = (int)(tiles - Q.cut_tiles);
+    Q.units.per = (Q.L.n_kvb + cut - 1) / cut;
+    Q.units.cut = cut;
+    const int64_t rows = (int64_t)Q.cut_tiles * cut * FA_ROWS;
     auto al = [](size_t x) { return (x + 255) & ~(size_t)255; };
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += al(n); return o; };
@@ -897,8 +975,8 @@ static FaQuantLayout fa_quant_layout(int64_t D, int64_t T, int64_t H, int64_t KV
     Q.flags_off = take((size_t)S * Q.L.n_tb * Q.L.n_kvb);
     Q.k_off = take((size_t)(S * HK * KV * D) * 2);
     Q.v_off = take((size_t)(S * HK * KV * D) * 2);
-    Q.part_off = take(Q.splits > 1 ? (size_t)(S * T * H * Q.splits * D) * 4 : 0);
-    Q.stat_off = take(Q.splits > 1 ? (size_t)(S * T * H * Q.splits) * 12 : 0);
+    Q.part_off = take((size_t)(rows * D) * 4);
+    Q.stat_off = take((size_t)rows * 8);
     Q.total = at;
     return Q;
 }
@@ -907,7 +985,7 @@ size_t fa_quant_workspace(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t H
     return fa_quant_layout(D, T, H, KV, HK, S).total;
 }
 
-cudaError_t fa_quant_run(const FaQuantArgs& q, char* ws, int* splits, float** part, float** stat, cudaStream_t st) {
+cudaError_t fa_quant_run(const FaQuantArgs& q, char* ws, cudaStream_t st) {
     const FaQuantLayout Q = fa_quant_layout(q.D, q.T, q.H, q.KV, q.HK, q.S);
     const FaLayout& L = Q.L;
     FaQuantPrep p{};
@@ -947,13 +1025,17 @@ cudaError_t fa_quant_run(const FaQuantArgs& q, char* ws, int* splits, float** pa
     a.dst = static_cast<float*>(q.dst);
     a.T = q.T, a.H = q.H, a.KV = q.KV, a.HK = q.HK, a.GP = L.GP, a.TQ = L.TQ, a.n_hg = L.n_hg, a.n_tb = L.n_tb, a.n_kvb = L.n_kvb;
     a.softcap = q.softcap, a.scale = q.scale, a.dst_f16 = q.dst_f16;
-    a.splits = Q.splits, a.kvb_per_split = Q.kvb_per_split;
+    a.units = Q.units;
     a.part = reinterpret_cast<float*>(ws + Q.part_off);
     a.stat = reinterpret_cast<float*>(ws + Q.stat_off);
     a.err = q.err;
-    *splits = Q.splits, *part = a.part, *stat = a.stat;
-    const dim3 fgrid((unsigned)(L.n_hg * L.n_tb), (unsigned)q.S, (unsigned)Q.splits);
-    return q.D == 64 ? launch_fa<64, 64, true>(tq, tk, tv, a, fgrid, st) : launch_fa<128, 128, true>(tq, tk, tv, a, fgrid, st);
+    const dim3 fgrid((unsigned)(Q.units.whole + Q.cut_tiles * Q.units.cut));
+    e = q.D == 64 ? launch_fa<64, 64, true>(tq, tk, tv, a, fgrid, st) : launch_fa<128, 128, true>(tq, tk, tv, a, fgrid, st);
+    if (e != cudaSuccess || Q.cut_tiles == 0) return e;
+    const int rows = Q.cut_tiles * FA_ROWS;
+    const dim3 jgrid((unsigned)((rows + 7) / 8));
+    return q.D == 64 ? launch_pdl(fa_join_kernel<64>, jgrid, dim3(256), 0, st, a, rows)
+                     : launch_pdl(fa_join_kernel<128>, jgrid, dim3(256), 0, st, a, rows);
 }
 
 }  // namespace b200

@@ -484,7 +484,9 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                 if (sent < live && !gave_up) send(tile0 + list[sent], prev);
             }
             __syncwarp();
-            if (!mbar_wait(full(stage), phase, a.err, ERR_WAIT_STREAM, abort_flag)) break;
+            // a wait that gives up may do so for some lanes alone: the warp leaves together
+            const bool got = mbar_wait(full(stage), phase, a.err, ERR_WAIT_STREAM, abort_flag);
+            if (__any_sync(0xffffffffu, !got)) break;
             if (list[e] & KR_DEAD) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(empty(stage));
@@ -994,14 +996,7 @@ int b200_flash_attn_kvq(int kv_type, int q_type, const void* q, const int64_t qn
         f.dst = dst, f.dst_f16 = dst_type == 1;
         f.D = (int)D, f.T = (int)T, f.H = (int)H, f.KV = (int)KV, f.HK = (int)HK, f.S = (int)S;
         f.scale = scale, f.softcap = softcap, f.err = dev_err;
-        int splits = 1;
-        float *part = nullptr, *stat = nullptr;
-        cudaError_t e = fa_quant_run(f, static_cast<char*>(workspace), &splits, &part, &stat, st);
-        if (e == cudaSuccess && splits > 1) {
-            const dim3 rows((unsigned)(S * T * H)), block(128);
-            e = D == 64 ? launch_pdl(kvq_join_kernel<64>, rows, block, 0, st, (const float*)part, (const float*)stat, splits, f.dst_f16, dst)
-                        : launch_pdl(kvq_join_kernel<128>, rows, block, 0, st, (const float*)part, (const float*)stat, splits, f.dst_f16, dst);
-        }
+        const cudaError_t e = fa_quant_run(f, static_cast<char*>(workspace), st);
         return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? B200_OK : B200_E_CUDA;
     }
     const int64_t row = D / 32 * 18;

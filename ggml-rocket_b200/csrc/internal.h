@@ -72,8 +72,7 @@ int mul_mat_vec_tiles(int wtype, const void* w_packed, int64_t N, int64_t K, con
 bool weight_type_supported(int type, int64_t K);
 // Attention of prompts over a Q4_0 cache (flash_attn.cu): the cache and q brought to fp16 in the workspace
 // (256-byte aligned, fa_quant_workspace bytes), then the tcgen05 kernel over every stream. Strides in bytes
-// (token or key, head, stream). Writes dst (16-byte aligned) when *splits comes back as 1; else the parts of
-// every row, outputs not divided by their sums and {max in log2 units, sum, 0}, in [S][T][H][splits] order.
+// (token or key, head, stream); dst 16-byte aligned.
 struct FaQuantArgs {
     const char* q;
     int64_t q_t, q_h, q_s;
@@ -92,7 +91,7 @@ struct FaQuantArgs {
     int* err;
 };
 size_t fa_quant_workspace(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S);
-cudaError_t fa_quant_run(const FaQuantArgs& q, char* ws, int* splits, float** part, float** stat, cudaStream_t st);
+cudaError_t fa_quant_run(const FaQuantArgs& q, char* ws, cudaStream_t st);
 // b200_get_rows over a Q4_0 (2) / Q8_0 (8) table (kv_cache.cu); pointers, shapes and idx checked before.
 int get_rows_quant_impl(int src_type, const void* src, const int64_t sne[4], const size_t snb[4], const int32_t* idx,
                         const int64_t ine[4], const size_t inb[4], float* dst, int* dev_err, cudaStream_t st);

@@ -172,6 +172,9 @@ PROMPTS = [
     (3, 17, 8, 2, 128, 2000),        # parts of the keys over several CTAs
     (1, 512, 8, 2, 128, 4096),
     (1, 9, 32, 4, 64, 20000),
+    (1, 300, 32, 8, 128, 5000),      # an odd number of token blocks
+    (2, 1100, 8, 8, 64, 1100),
+    (1, 700, 64, 8, 128, 900),       # more tiles than a wave: whole ones, then cut ones
 ]
 
 
@@ -187,6 +190,7 @@ def test_prompts_against_definition(cuda, S, T, H, HK, D, KV, f16):
     assert float((out.double() - want).norm() / want.norm()) < 2e-3     # random roundings: far below the bound
     check(run(q, k, v, None, scale, f16), q, k, v, None, scale)
     check(run(q, k, v, None, scale, f16, softcap=5.0), q, k, v, None, scale, softcap=5.0)
+    check(run(q, k, v, m, -3 * scale, f16), q, k, v, m, -3 * scale)
 
 
 @pytest.mark.parametrize("f16", [False, True])
