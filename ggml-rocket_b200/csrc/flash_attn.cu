@@ -670,41 +670,58 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
     }
 }
 
-// Joins the parts of the tiles that several CTAs shared: one warp per row of such a tile.
-template <int D>
+// Joins the parts of the tiles that several CTAs shared: W warps per row of such a tile take its parts in turn.
+template <int D, int W>
 __global__ void __launch_bounds__(256) fa_join_kernel(const FaArgs args, int n_rows) {
     grid_dep_wait();
     grid_dep_launch();
-    const int id = (int)(blockIdx.x * 8 + (threadIdx.x >> 5)), lane = threadIdx.x & 31;
-    if (id >= n_rows) return;
+    __shared__ float sums[8][D + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int id = (int)(blockIdx.x * (8 / W) + warp / W), w = warp % W;
     const int cut_tile = id / FA_ROWS, r = id % FA_ROWS;
     const int gt = args.units.whole + cut_tile, per_stream = args.n_tb * args.n_hg;
     const int str = gt / per_stream, tile = gt % per_stream;
     const int tb = args.n_tb - 1 - tile / args.n_hg;
     const int t = tb * args.TQ + r % args.TQ, h = tile % args.n_hg * args.GP + r / args.TQ;
-    if (t >= args.T) return;
+    const bool in = id < n_rows && t < args.T;
     const int cut = args.units.cut;
     const int64_t first = (int64_t)cut_tile * cut * FA_ROWS + r;   // of part k: + k * FA_ROWS
-    float top = -INFINITY;
-    for (int k = lane; k < cut; k += 32) {
-        const float* st = args.stat + 2 * (first + (int64_t)k * FA_ROWS);
-        if (st[1] != 0.0f) top = fmaxf(top, st[0]);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (top == -INFINITY) top = 0.0f;
     constexpr int PER = D / 32;
     float acc[PER] = {}, l_all = 0.0f;
-#pragma unroll 4
-    for (int k = 0; k < cut; k++) {
-        const int64_t at = first + (int64_t)k * FA_ROWS;
-        const float l = args.stat[2 * at + 1];
-        const float f = l == 0.0f ? 0.0f : ex2_approx(args.stat[2 * at] - top);   // l is 0 where no key is seen
-        l_all = fmaf(l, f, l_all);
-        const float* p = args.part + at * D + lane * PER;
+    if (in) {
+        float top = -INFINITY;
+        for (int k = lane; k < cut; k += 32) {
+            const float* st = args.stat + 2 * (first + (int64_t)k * FA_ROWS);
+            if (st[1] != 0.0f) top = fmaxf(top, st[0]);
+        }
 #pragma unroll
-        for (int e = 0; e < PER; e++) acc[e] = fmaf(p[e], f, acc[e]);
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (top == -INFINITY) top = 0.0f;
+#pragma unroll 4
+        for (int k = w; k < cut; k += W) {
+            const int64_t at = first + (int64_t)k * FA_ROWS;
+            const float l = args.stat[2 * at + 1];
+            const float f = l == 0.0f ? 0.0f : ex2_approx(args.stat[2 * at] - top);   // l is 0 where no key is seen
+            l_all = fmaf(l, f, l_all);
+            const float* p = args.part + at * D + lane * PER;
+#pragma unroll
+            for (int e = 0; e < PER; e++) acc[e] = fmaf(p[e], f, acc[e]);
+        }
     }
+    if constexpr (W > 1) {
+#pragma unroll
+        for (int e = 0; e < PER; e++) sums[warp][lane * PER + e] = acc[e];
+        if (lane == 0) sums[warp][D] = l_all;
+        __syncthreads();
+        if (w != 0) return;
+        for (int o = 1; o < W; o++) {
+#pragma unroll
+            for (int e = 0; e < PER; e++) acc[e] += sums[warp + o][lane * PER + e];
+            l_all += sums[warp + o][D];
+        }
+        l_all = __shfl_sync(0xffffffffu, l_all, 0);
+    }
+    if (!in) return;
     const int64_t at = (((int64_t)str * args.T + t) * args.H + h) * D + lane * PER;
 #pragma unroll
     for (int e = 0; e < PER; e++) {
@@ -875,12 +892,18 @@ __global__ void __launch_bounds__(256) fa_quant_prep_kernel(const FaQuantPrep a)
         const char* src = a.q + s * a.q_s + h * a.q_h + t * a.q_t;
         constexpr int PER = D / 32;
         float x[PER], amax = 0.0f;
+        if (a.q_f16) {
+            uint16_t w[PER];
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            x[i] = a.q_f16 ? __half2float(reinterpret_cast<const __half*>(src)[lane * PER + i])
-                           : reinterpret_cast<const float*>(src)[lane * PER + i];
-            amax = fmaxf(amax, fabsf(x[i]));
+            for (int i = 0; i < PER; i++) w[i] = reinterpret_cast<const uint16_t*>(src)[lane * PER + i];
+#pragma unroll
+            for (int i = 0; i < PER; i++) x[i] = __half2float(__ushort_as_half(w[i]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; i++) x[i] = reinterpret_cast<const float*>(src)[lane * PER + i];
         }
+#pragma unroll
+        for (int i = 0; i < PER; i++) amax = fmaxf(amax, fabsf(x[i]));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         // f32 rows are brought near 1 as well, so that small ones keep fp16's full precision
@@ -1033,9 +1056,11 @@ cudaError_t fa_quant_run(const FaQuantArgs& q, char* ws, cudaStream_t st) {
     e = q.D == 64 ? launch_fa<64, 64, true>(tq, tk, tv, a, fgrid, st) : launch_fa<128, 128, true>(tq, tk, tv, a, fgrid, st);
     if (e != cudaSuccess || Q.cut_tiles == 0) return e;
     const int rows = Q.cut_tiles * FA_ROWS;
-    const dim3 jgrid((unsigned)((rows + 7) / 8));
-    return q.D == 64 ? launch_pdl(fa_join_kernel<64>, jgrid, dim3(256), 0, st, a, rows)
-                     : launch_pdl(fa_join_kernel<128>, jgrid, dim3(256), 0, st, a, rows);
+    auto join = [&](auto kernel, int warps) {
+        return launch_pdl(kernel, dim3((unsigned)((rows * warps + 7) / 8)), dim3(256), 0, st, a, rows);
+    };
+    if (Q.units.cut <= 4) return q.D == 64 ? join(fa_join_kernel<64, 1>, 1) : join(fa_join_kernel<128, 1>, 1);
+    return q.D == 64 ? join(fa_join_kernel<64, 4>, 4) : join(fa_join_kernel<128, 4>, 4);
 }
 
 }  // namespace b200
