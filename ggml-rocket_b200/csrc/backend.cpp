@@ -1027,6 +1027,9 @@ static bool glue_supported(const b200_tensor* op) {
             // op: the cache tensor itself (its rows that no index names stay as they are, so it has to lie
             // in device memory); a: the new rows; b: their indices
             const size_t unit = op->type == T_F32 ? 4 : 2;
+            const size_t row = is_quantized(op->type) ? (size_t)(op->ne[0] / 32) * type_size(op->type) : (size_t)op->ne[0] * type_size(op->type);
+            for (int i = 1; i < 4; i++)
+                if (op->ne[i] > 1 && op->nb[i] < row) return false;   // rows that lie in one another
             return b && op->on_device && a->type == T_F32 && (b->type == T_I64 || b->type == T_I32) &&
                    (op->type == T_F32 || op->type == T_F16 || kv_block_type(op)) && op->nb[0] == type_size(op->type) &&
                    (op->nb[1] | op->nb[2] | op->nb[3]) % unit == 0 && (uintptr_t)op->data % unit == 0 && a->nb[0] == 4 &&
@@ -1070,11 +1073,9 @@ static bool fa_kvq(const b200_tensor* op) {
         return t->type == T_Q4_0 && t->on_device && t->nb[0] == 18 && t->ne[0] == D && t->ne[1] == KV && t->ne[2] == HK &&
                t->ne[3] == S && (t->nb[1] | t->nb[2] | t->nb[3]) % unit == 0 && (uintptr_t)t->data % unit == 0;
     };
-    return T > 0 && T <= 65536 && S > 0 && S <= 65535 && HK > 0 && H > 0 && H % HK == 0 && KV > 0 &&
-           KV <= ((int64_t)1 << 30) && q->nb[0] == qe && (q->nb[1] | q->nb[2] | q->nb[3]) % qe == 0 && cache_ok(k) &&
+    return b200_flash_attn_kvq_workspace_size(D, T, H, KV, HK, S) > 0 && q->nb[0] == qe && (q->nb[1] | q->nb[2] | q->nb[3]) % qe == 0 && cache_ok(k) &&
            cache_ok(v) && op->type == T_F32 && is_contiguous(op) && op->ne[0] == D && op->ne[1] == H && op->ne[2] == T &&
-           op->ne[3] == S && (!op->on_device || (uintptr_t)op->data % 16 == 0) && S * T * H <= INT32_MAX / 4 &&
-           T * (H / HK) <= (1 << 20) && HK * ((T * (H / HK) + 7) / 8) <= 65535 &&
+           op->ne[3] == S && (!op->on_device || (uintptr_t)op->data % 16 == 0) &&
            (!m || (m->type == T_F16 && m->nb[0] == 2 && is_contiguous(m) && m->ne[0] >= KV && m->ne[1] >= T && m->ne[2] == 1 &&
                    (m->ne[3] == S || m->ne[3] == 1)));
 }

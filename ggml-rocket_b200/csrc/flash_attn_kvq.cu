@@ -940,8 +940,15 @@ cudaError_t launch_kvq(const CUtensorMap& tk, const CUtensorMap& tv, const KvqAr
                       (const float*)a.part, (const float*)a.stat, parts, a.dst_f16, a.dst);
 }
 
-bool kvq_dims_ok(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S) {
-    return (D == 64 || D == 128) && T > 0 && H > 0 && KV > 0 && HK > 0 && S > 0 && H % HK == 0;
+// The sizes the grids and 32-bit counters hold.
+bool kvq_sizes_ok(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S) {
+    if ((D != 64 && D != 128) || T <= 0 || T > 65536 || H <= 0 || H > (1 << 20) || KV <= 0 || KV > (1ll << 30) || HK <= 0 ||
+        S <= 0 || S > 65535 || H % HK != 0)
+        return false;
+    const int64_t rows = T * (H / HK);
+    if (rows > (1 << 20) || S * T * H > INT32_MAX / 4 || HK * ((rows + KR_ROWS - 1) / KR_ROWS) > 65535) return false;
+    // mask blocks of the prompt path: a token at least and 128 keys each
+    return rows <= KR_MAX_ROWS || S * T * ((KV + 127) / 128) <= INT32_MAX;
 }
 
 }  // namespace
@@ -952,7 +959,7 @@ extern "C" {
 
 size_t b200_flash_attn_kvq_workspace_size(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S) {
     using namespace b200;
-    if (!kvq_dims_ok(D, T, H, KV, HK, S)) return 0;
+    if (!kvq_sizes_ok(D, T, H, KV, HK, S)) return 0;
     if (T * (H / HK) > KR_MAX_ROWS) return fa_quant_workspace(D, T, H, KV, HK, S);
     return std::max(kvq_plan(D, T, H, KV, HK, S, true).total, kvq_plan(D, T, H, KV, HK, S, false).total);
 }
@@ -972,9 +979,7 @@ int b200_flash_attn_kvq(int kv_type, int q_type, const void* q, const int64_t qn
         return B200_E_INVALID;
     if (kv_type != 2 || (q_type != 0 && q_type != 1) || (dst_type != 0 && dst_type != 1)) return B200_E_UNSUPPORTED;
     const size_t qe = q_type == 1 ? 2 : 4, unit = (size_t)D / 16;
-    if (!kvq_dims_ok(D, T, H, KV, HK, S) || T > 65536 || S > 65535 || KV > (1ll << 30) || T * (H / HK) > (1 << 20) || S * T * H > INT32_MAX / 4 ||
-        HK * ((T * (H / HK) + KR_ROWS - 1) / KR_ROWS) > 65535)
-        return B200_E_UNSUPPORTED;
+    if (!kvq_sizes_ok(D, T, H, KV, HK, S)) return B200_E_UNSUPPORTED;
     auto off = [](const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; };
     if (qnb[0] != qe || (qnb[1] | qnb[2] | qnb[3]) % qe != 0 || off(q, qe) || knb[0] != 18 || vnb[0] != 18 ||
         (knb[1] | knb[2] | knb[3] | vnb[1] | vnb[2] | vnb[3]) % unit != 0 || off(k, unit) || off(v, unit) ||

@@ -212,7 +212,7 @@ int b200_rope_multi(int type, const void* x, const int64_t ne[4], const size_t n
     RopeMulti a{};
     const int64_t pairs = mode == 24 ? n_dims : n_dims / 2;
     if ((int64_t)nb[0] != es || (nb[1] | nb[2] | nb[3]) % es != 0 || reinterpret_cast<uintptr_t>(x) % es != 0 ||
-        reinterpret_cast<uintptr_t>(dst) % es != 0 || pairs > RM_TABLE || ne[0] > 4096 || ne[1] > 65536 ||
+        reinterpret_cast<uintptr_t>(dst) % es != 0 || reinterpret_cast<uintptr_t>(pos) % 4 != 0 || pairs > RM_TABLE || ne[0] > 4096 || ne[1] > 65536 ||
         ne[3] > 65535)
         return B200_E_UNSUPPORTED;
     const int vw = (int)(16 / es);

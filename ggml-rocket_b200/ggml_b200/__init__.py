@@ -640,6 +640,12 @@ def _type_of(t, what):
     return ty
 
 
+def _err_of(dev_err, what):
+    if _type_of(dev_err, what) != I32 or dev_err.numel() < 1:
+        raise B200Error(f"{what}: dev_err is an int32 tensor of one element")
+    return dev_err.data_ptr()
+
+
 def _stream_of(stream, dev):
     return _raw_stream(dev) if stream is None else stream.cuda_stream
 
@@ -657,6 +663,8 @@ def _dims(t):
 
 def _dims_q(t, kind, what):
     """The same for a uint8 tensor whose innermost dim holds the blocks of one row of a quantised type."""
+    if kind not in BLOCK:
+        raise B200Error(f"{what}: type {kind} is not supported")
     block, size = BLOCK[kind]
     ne, nb = _dims(t)
     if t.element_size() != 1 or nb[0] != 1 or ne[0] % size:
@@ -696,7 +704,7 @@ def set_rows(src, idx, dst, dst_type, dev_err, stream=None):
     else:
         dne, dnb = _dims_q(dst, dst_type, "set_rows")
     rc = lib().b200_set_rows(src.data_ptr(), _ne4(*sne), _ne4(*snb), _type_of(idx, "set_rows"), idx.data_ptr(), _ne4(*ine),
-                             _ne4(*inb), dst_type, dst.data_ptr(), _ne4(*dne), _ne4(*dnb), dev_err.data_ptr(),
+                             _ne4(*inb), dst_type, dst.data_ptr(), _ne4(*dne), _ne4(*dnb), _err_of(dev_err, "set_rows"),
                              _stream_of(stream, dev))
     if rc:
         check(rc, "set_rows")
@@ -718,7 +726,7 @@ def get_rows(src, src_type, idx, dst, dev_err, stream=None):
             dst.numel() != sne[0] * idx.numel():
         raise B200Error("get_rows: idx is int32, dst contiguous f32 with a row for every index")
     rc = lib().b200_get_rows(src_type, src.data_ptr(), _ne4(*sne), _ne4(*snb), idx.data_ptr(), _ne4(*ine), _ne4(*inb),
-                             dst.data_ptr(), dev_err.data_ptr(), _stream_of(stream, dev))
+                             dst.data_ptr(), _err_of(dev_err, "get_rows"), _stream_of(stream, dev))
     if rc:
         check(rc, "get_rows")
     return dst
@@ -752,7 +760,7 @@ def flash_attn_kvq(kv_type, q, k, v, mask, dst, scale, workspace, dev_err, softc
         kv_type, _type_of(q, "flash_attn_kvq"), q.data_ptr(), _ne4(D, T, H, S), _ne4(qd * es, qt * es, qh * es, qs * es),
         k.data_ptr(), _ne4(kn, kkv, khk, kst), _ne4(k0, kr, kh, ks), v.data_ptr(), _ne4(vn, vkv, vhk, vst),
         _ne4(v0, vr, vh, vs), mp, mnb, _type_of(dst, "flash_attn_kvq"), dst.data_ptr(), scale, softcap,
-        workspace.data_ptr(), workspace.numel() * workspace.element_size(), dev_err.data_ptr(), _stream_of(stream, dev))
+        workspace.data_ptr(), workspace.numel() * workspace.element_size(), _err_of(dev_err, "flash_attn_kvq"), _stream_of(stream, dev))
     if rc:
         check(rc, "flash_attn_kvq")
     return dst

@@ -290,11 +290,11 @@ int b200_get_rows(int src_type, const void * src, const int64_t sne[4], const si
                   const int64_t ine[4], const size_t inb[4], float * dst, int * dev_err, void * stream);
 /* SET_ROWS, a KV cache's write: dst[:, idx[i, j % ine[1], k % ine[2]], j, k] = src[:, i, j, k], src F32
  * [n, n_rows, ..], idx I32 (26) or I64 (27) [n_rows, ..], dst a view of F32 (0), F16 (1), Q4_0 (2) or
- * Q8_0 (8) rows with any strides (multiples of 2 bytes, 4 for F32), quantised as ggml's reference
- * encoders do, bit for bit (n a multiple of 32 for those). Rows that no index names stay as they are; of
- * several source rows for one destination row the last stays, as if written in order. An index outside
- * dst's rows records a device error and its row is not written. A block that holds a NaN or an infinity
- * is stored with a NaN scale (ggml leaves it undefined). */
+ * Q8_0 (8) rows with any strides (multiples of 2 bytes, 4 for F32; rows at least a row's bytes apart),
+ * quantised as ggml's reference encoders do, bit for bit (n a multiple of 32 for those). Rows that no
+ * index names stay as they are; of several source rows for one destination row the last stays, as if
+ * written in order. An index outside dst's rows records a device error and its row is not written. A
+ * block that holds a NaN or an infinity is stored with a NaN scale (ggml leaves it undefined). */
 int b200_set_rows(const float * src, const int64_t sne[4], const size_t snb[4], int idx_type, const void * idx,
                   const int64_t ine[4], const size_t inb[4], int dst_type, void * dst, const int64_t dne[4],
                   const size_t dnb[4], int * dev_err, void * stream);

@@ -346,3 +346,29 @@ def test_cache_past_32_bits(cuda):
     vv = big.as_strided((S, KV, HK, 72), (KV * stride, stride, 72, 1), 4096)
     kv.copy_(k), vv.copy_(v)
     check(run(q, kv, vv, None, 0.1), q, k, v, None, 0.1)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("S,T,H,HK,D,KV", [
+    (1, 1, 40, 1, 128, 777),         # single tokens whose KV head serves more rows than the row kernel takes
+    (1, 1, 256, 1, 64, 300),
+    (2, 1, 33, 1, 64, 5),
+    (300, 1, 4, 1, 64, 40),          # more streams than SMs
+    (70, 2, 64, 2, 64, 129),
+    (1, 16, 2, 1, 128, 1),           # as many rows as the row kernel takes, one key; and two more
+    (1, 17, 2, 1, 128, 1),
+    (1, 64, 6, 3, 64, 20),           # more tokens than keys
+    (2, 1, 4, 2, 128, 127),
+])
+def test_shapes_at_the_ends(cuda, S, T, H, HK, D, KV, f16):
+    """A random mask, its first row of every stream hidden whole, its last key of every other row visible."""
+    import torch
+    q, k, v = inputs(S, T, H, HK, D, KV, seed=5, q_f16=f16)
+    scale = 1 / math.sqrt(D)
+    gen = torch.Generator(device="cuda").manual_seed(S + T + KV)
+    m = torch.randn(S, T, KV, device="cuda", generator=gen).half()
+    m[torch.rand(S, T, KV, device="cuda", generator=gen) < 0.5] = NEG
+    m[:, 1:, -1] = 0.0
+    m[:, 0] = NEG
+    check(run(q, k, v, m, scale, f16), q, k, v, m, scale)
+    check(run(q, k, v, None, scale, f16), q, k, v, None, scale)

@@ -237,3 +237,28 @@ def test_replayed_graph_and_side_stream(cuda):
     g.set_rows(x, idx, side, Q4_0, err, stream=st)
     st.synchronize()
     assert np.array_equal(side[9:14].cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("kind", [Q4_0, Q8_0])
+@pytest.mark.parametrize("n,n_rows,total", [(16384, 3, 4), (1 << 20, 1, 1), (32, 70000, 70001)])
+def test_widest_and_most_rows(cuda, kind, n, n_rows, total):
+    """Rows of many CTAs, many rows of one block; indices every second element of a longer vector."""
+    import torch
+    import ggml_b200 as g
+    rng = np.random.default_rng(n_rows)
+    x = rng.standard_normal((n_rows, n)).astype(np.float32)
+    where = rng.permutation(total)[:n_rows].astype(np.int32)
+    idx = torch.from_numpy(np.repeat(where, 2)).cuda()[::2]
+    blocks = np.zeros((total, n // 32 * (34 if kind == Q8_0 else 18)), np.uint8)
+    d = torch.from_numpy(blocks).cuda()
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    g.set_rows(torch.from_numpy(x).cuda(), idx, d, kind, err)
+    blocks[where] = encode(x, kind)
+    back = torch.empty(n_rows, n, device="cuda")
+    g.get_rows(d, kind, idx, back, err)
+    torch.cuda.synchronize()
+    assert int(err.item()) == 0
+    assert np.array_equal(d.cpu().numpy(), blocks)
+    assert np.array_equal(back.cpu().numpy(), decode(blocks[where], kind), equal_nan=True)
+    with pytest.raises(g.B200Error, match="dev_err"):
+        g.set_rows(torch.from_numpy(x).cuda(), idx, d, kind, err.float())

@@ -140,3 +140,19 @@ def test_replayed_graph_reads_new_inputs(cuda):
     graph.replay()
     torch.cuda.synchronize()
     check(out, x, pos, 128, 8, [16, 24, 24, 0], 1e4)
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("tokens,heads,dim,n_dims,mode,sections", [
+    (1, 700, 64, 64, 40, [11, 11, 10, 0]),         # many heads of one token
+    (20000, 1, 32, 32, 8, [6, 5, 5, 0]),           # many tokens of one head
+    (2, 2, 4096, 64, 8, [16, 8, 8, 0]),            # nearly all of the head copied
+    (9, 3, 2048, 1024, 24, [512, 512, 0, 0]),
+])
+def test_sizes_at_the_ends(cuda, tokens, heads, dim, n_dims, mode, sections, half):
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(tokens + dim)
+    x = torch.randn(tokens, heads, dim, device="cuda", generator=gen)
+    x = x.half() if half else x
+    pos = torch.randint(0, 200000, (4, tokens), device="cuda", generator=gen, dtype=torch.int32)
+    check(run(x, pos, n_dims, mode, sections, 1e6), x, pos, n_dims, mode, sections, 1e6)

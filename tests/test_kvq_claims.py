@@ -18,10 +18,10 @@ def rope(mode=8, sections=(16, 24, 24, 0), n_dims=128, ptokens=12, t=g.F32, dt=N
     x = T(t, [128, 8, 3])
     return T(t if dt is None else dt, [128, 8, 3], op=g.OP_ROPE, srcs=[x, T(g.I32, [ptokens]), src2],
              op_params=[0, n_dims, mode, 0, 4096, 10000.0, 1.0, ext, 1.0, 32.0, 1.0] + list(sections))
-def set_rows(dt=g.Q4_0, n=256, rows=5, it=g.I64, dev=True, n_idx=None, st=g.F32, data=DEV):
+def set_rows(dt=g.Q4_0, n=256, rows=5, it=g.I64, dev=True, n_idx=None, st=g.F32, data=DEV, nb=None):
     a, i = T(st, [n, rows]), T(it, [rows if n_idx is None else n_idx])
     c = T(dt, [n, 100], data, on_device=dev)
-    return T(dt, [n, 100], data, op=g.OP_SET_ROWS, srcs=[a, i, c], on_device=dev)
+    return T(dt, [n, 100], data, nb=nb, op=g.OP_SET_ROWS, srcs=[a, i, c], on_device=dev)
 def get_rows(t=g.Q4_0, dev=True, n=256):
     return T(g.F32, [n, 4], op=g.OP_GET_ROWS, srcs=[T(t, [n, 100], DEV if dev else None, on_device=dev), T(g.I32, [4])])
 def fa(tokens=1, kv=64, D=128, H=8, HK=2, S=1, kt=g.Q4_0, vt=g.Q4_0, dev=True, mask=True, sinks=False, bias=0.0, data=DEV, qt=g.F32, ms=None):
@@ -39,9 +39,10 @@ r = {
     "rope": [rope(), rope(40), rope(24, (32, 32, 0, 0), 64), rope(t=g.F16)],
     "rope_no": [rope(ptokens=3), rope(sections=(0, 0, 0, 0)), rope(24), rope(ext=1.0), rope(9), rope(t=g.BF16), rope(n_dims=130),
                 rope(sections=(-1, 24, 24, 0)), rope(src2=T(g.F32, [64])), rope(dt=g.F16)],
-    "set": [set_rows(), set_rows(g.Q8_0), set_rows(g.F16), set_rows(g.F32, n=7), set_rows(it=g.I32)],
+    "set": [set_rows(), set_rows(g.Q8_0), set_rows(g.F16), set_rows(g.F32, n=7), set_rows(it=g.I32),
+            set_rows(nb=[18, 162, 16200, 16200])],
     "set_no": [set_rows(dev=False), set_rows(n=48), set_rows(g.Q4_K), set_rows(n_idx=4), set_rows(it=g.F32), set_rows(st=g.F16),
-               set_rows(data=DEV + 1)],
+               set_rows(data=DEV + 1), set_rows(nb=[18, 126, 14400, 14400])],
     "get": [get_rows(), get_rows(g.Q8_0)],
     "get_no": [get_rows(dev=False), get_rows(g.Q4_K), get_rows(g.Q8_0, dev=False)],
     "fa": [fa(), fa(tokens=7, kv=1), fa(D=64, S=5), fa(tokens=600, kv=700, S=2, ms=1), fa(qt=g.F16)],

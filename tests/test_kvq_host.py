@@ -83,3 +83,38 @@ def test_flash_attn_kvq():
     assert call(mnb=(4, 128, 128, 128)) == NO and call(mask=ODD) == NO and call(dst=ctypes.c_void_p((1 << 20) + 2)) == NO
     assert call(kne=(128, 1 << 31, 8, 1), vne=(128, 1 << 31, 8, 1)) == NO
     assert call(ws=None) == WS and call(wsb=16) == WS and call(ws=ctypes.c_void_p((1 << 20) + 16)) == WS
+
+
+def test_sizes_past_the_counters():
+    """Sizes whose grids or 32-bit counters would not hold the work have no workspace and are refused."""
+    size = g.lib().b200_flash_attn_kvq_workspace_size
+    assert size(64, 65536, 1, (1 << 22) - 128, 1, 1) > 0      # 2^31 - 2^16 mask blocks of a token and 128 keys
+    assert size(64, 65536, 1, 1 << 22, 1, 1) == 0              # 2^31
+    assert size(64, 1, 1, 1 << 30, 1, 65535) > 0               # few rows: no such blocks
+    assert size(64, 65537, 1, 64, 1, 1) == 0 and size(64, 1, 1, (1 << 30) + 1, 1, 1) == 0
+    assert size(64, 1, 1, 64, 1, 65536) == 0 and size(128, 1, 65536 * 32, 64, 65536, 1) == 0
+
+
+def test_more_refusals():
+    """A misaligned position tensor, rows of a cache that lie in one another, sizes past 32 bits."""
+    lib = g.lib()
+    s = (ctypes.c_int32 * 4)(16, 24, 24, 0)
+    assert lib.b200_rope_multi(0, P, ne(128, 4, 3), nb(4, 512, 2048, 6144), ctypes.c_void_p((1 << 20) + 2), 128, 8, s, 1e4,
+                               1.0, 1.0, P, None) == NO
+
+    def call(sne=(64, 5), snb=(4, 256, 1280, 1280), dne=(64, 9), dnb=(18, 36, 324, 324)):
+        return lib.b200_set_rows(P, ne(*sne), nb(*snb), 27, P, ne(sne[1]), nb(8, 0, 0, 0), 2, P, ne(*dne), nb(*dnb), P, None)
+
+    assert call(dnb=(18, 18, 324, 324)) == BAD and call(dnb=(18, 0, 324, 324)) == BAD
+    assert call(sne=(64, 5, 2), dne=(64, 9, 2), dnb=(18, 36, 0, 0)) == BAD
+    assert call(sne=(64, 1 << 62)) == NO and call(sne=(1 << 40, 1 << 30), dne=(1 << 40, 9), dnb=(18, 1 << 40, 1 << 50, 0)) == NO
+
+
+def test_wrapper_types():
+    """The wrappers name a type they do not take, before any CUDA call."""
+    import pytest
+    import torch
+    with pytest.raises(g.B200Error, match="type 99"):
+        g._dims_q(torch.zeros(2, 36, dtype=torch.uint8), 99, "set_rows")
+    with pytest.raises(g.B200Error, match="whole blocks"):
+        g._dims_q(torch.zeros(2, 35, dtype=torch.uint8), g.Q4_0, "set_rows")
