@@ -51,6 +51,8 @@ struct FaArgs {
     const uint8_t* flags;      // [n_tb][n_kvb]
     float* dst;                // [T][H][DV]
     int T, H, KV, HK, GP, TQ, n_hg, n_tb, n_kvb;
+    int S;                     // EXT: streams
+    const __half* q16;         // EXT: [S][H][T][D]
     float softcap;
     int* err;
     // the extended form only (several streams, parts of the keys, f16 results; q16 not scaled)
@@ -61,6 +63,13 @@ struct FaArgs {
     float* part;               // [unit - whole][rows of a unit][DV] outputs not divided by their sums
     float* stat;               // {max in log2 units, sum} of each of their rows
 };
+
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 
 __device__ __forceinline__ float ex2_approx(float x) {
     float y;
@@ -226,25 +235,29 @@ __device__ __forceinline__ void tmem_st_p(uint32_t taddr, const uint32_t (&w)[N]
 // ---------------------------------------------------------------------------------------------
 // The attention kernel.
 // ---------------------------------------------------------------------------------------------
-template <int D, int DV>
+template <int D, int DV, bool EXT = false>
 struct FaCfg {
     static constexpr int Q_BYTES = FA_ROWS * D * 2;
     static constexpr int K_BYTES = FA_KB * D * 2;
     static constexpr int V_BYTES = FA_KB * DV * 2;
     static constexpr int OFF_Q = 0;
-    static constexpr int OFF_K = OFF_Q + Q_BYTES;
+    static constexpr int OFF_K = EXT ? 0 : OFF_Q + Q_BYTES;   // EXT keeps Q in TMEM
     static constexpr int OFF_V = OFF_K + 2 * K_BYTES;
+    // EXT: one ring of tiles in the order the products take them, high and low halves of K and V alike
+    static constexpr int RING = EXT ? (D == 128 ? 6 : 10) : 0;
     // exchange between the FA_SPLIT threads of a row: maxima [2][SPLIT][128] f32 and their
     // sequence numbers (same shape, int), then sums [SPLIT][128] + sequence numbers
     static constexpr int XCH_MAX = 2 * FA_SPLIT * 128 * 4;
     static constexpr int XCH_SUM = FA_SPLIT * 128 * 4;
-    static constexpr int OFF_XCH = OFF_V + 2 * V_BYTES;
+    static constexpr int OFF_XCH = EXT ? OFF_K + RING * K_BYTES : OFF_V + 2 * V_BYTES;
     static constexpr int OFF_BAR = OFF_XCH + 2 * XCH_MAX + 2 * XCH_SUM;
     static constexpr int SMEM = OFF_BAR + 256 + 1024;
     // TMEM columns: S0 [0,128) | S1 [128,256) | O [256, 256+DV) | P0 [384,448) | P1 [448,512)
     // (P is fp16, two keys per 32-bit column, read by the P.V MMA as its A operand)
     static constexpr uint32_t TMEM_COLS = 512;
-    static constexpr uint32_t P_TMEM0 = 384;
+    // EXT: Q [384, 384+D/2), one P buffer [448,512)
+    static constexpr uint32_t P_TMEM0 = EXT ? 448 : 384;
+    static constexpr uint32_t Q_TMEM0 = 384;
     static constexpr uint32_t IDESC_S = idesc_f16_f32(FA_ROWS, FA_KB);
     static constexpr uint32_t IDESC_O = idesc_f16_f32_bmn(FA_ROWS, DV);
 };
@@ -266,7 +279,7 @@ template <int D, int DV, bool EXT>
 __global__ void __launch_bounds__(FA_THREADS, 1)
 fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
           const __grid_constant__ CUtensorMap tmV, const FaArgs args) {
-    using C = FaCfg<D, DV>;
+    using C = FaCfg<D, DV, EXT>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = smem_u32(smem_raw);
     uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
@@ -277,15 +290,19 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
     auto k_empty = [&](int s) { return bar + 8u * (3 + s); };
     auto v_full = [&](int s) { return bar + 8u * (5 + s); };
     auto v_empty = [&](int s) { return bar + 8u * (7 + s); };
-    auto s_full = [&](int s) { return bar + 8u * (9 + s); };
-    auto s_empty = [&](int s) { return bar + 8u * (11 + s); };
+    // EXT: a ring's barriers in the place of K's and V's
+    constexpr int X = EXT ? 2 * C::RING - 8 : 0;
+    auto full = [&](int slot) { return bar + 8u * (1 + slot); };
+    auto empty = [&](int slot) { return bar + 8u * (1 + C::RING + slot); };
+    auto s_full = [&](int s) { return bar + 8u * (X + 9 + s); };
+    auto s_empty = [&](int s) { return bar + 8u * (X + 11 + s); };
     // P of blocks b, b+2, ... written (per parity: a softmax warp may run one block ahead of
     // another, never two, because P buffer b is reused only after the P.V two blocks back)
-    auto p_full = [&](int b) { return bar + 8u * (17 + b); };
-    auto pv_done = [&](int b) { return bar + 8u * (14 + b); };   // P.V of blocks b, b+2, ... completed
-    const uint32_t drain = bar + 8u * 16;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_BAR + 8 * 19);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_BAR + 8 * 19 + 4);
+    auto p_full = [&](int b) { return bar + 8u * (X + 17 + b); };
+    auto pv_done = [&](int b) { return bar + 8u * (X + 14 + b); };   // P.V of blocks b, b+2, ... completed
+    const uint32_t drain = bar + 8u * (X + 16);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_BAR + 8 * (X + 19));
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_BAR + 8 * (X + 19) + 4);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // heavier (later) token blocks first
@@ -300,12 +317,18 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
     const int j_first = un.first, j_end = un.end;
 
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 1);
+        mbar_init(q_full, EXT ? FA_SOFTMAX_WARPS : 1);
+        if constexpr (EXT) {
+            for (int n = 0; n < 2 * C::RING; n++) mbar_init(full(n), 1);
+        } else {
+            for (int s = 0; s < 2; s++) {
+                mbar_init(k_full(s), 1);
+                mbar_init(k_empty(s), 1);
+                mbar_init(v_full(s), 1);
+                mbar_init(v_empty(s), 1);
+            }
+        }
         for (int s = 0; s < 2; s++) {
-            mbar_init(k_full(s), 1);
-            mbar_init(k_empty(s), 1);
-            mbar_init(v_full(s), 1);
-            mbar_init(v_empty(s), 1);
             mbar_init(s_full(s), 1);
             mbar_init(s_empty(s), FA_SOFTMAX_WARPS);
         }
@@ -341,10 +364,41 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
 
     if (warp == 0) {
         if (lane == 0) {
-            mbar_arrive_expect_tx(q_full, C::Q_BYTES);
-            for (int c = 0; c < D / 64; c++)
-                tma_load_3d(sb + C::OFF_Q + c * (FA_ROWS * 128), &tmQ, q_full, c * 64, tb * args.TQ,
-                            str * args.H + hg * args.GP);
+            if constexpr (!EXT) {
+                mbar_arrive_expect_tx(q_full, C::Q_BYTES);
+                for (int c = 0; c < D / 64; c++)
+                    tma_load_3d(sb + C::OFF_Q + c * (FA_ROWS * 128), &tmQ, q_full, c * 64, tb * args.TQ,
+                                str * args.H + hg * args.GP);
+            }
+            if constexpr (EXT) {
+                // tiles in the order of the products: K of a block, then V of the one before
+                int n = 0, prev = -1;
+                bool ok = true;
+                auto push = [&](const CUtensorMap* map, int j) {
+                    for (int half = 0; half < 2 && ok; half++) {
+                        const int slot = n % C::RING;
+                        ok = mbar_wait(empty(slot), ((uint32_t)(n / C::RING) & 1u) ^ 1u, args.err, ERR_WAIT_PRODUCER, abort_flag);
+                        if (!ok) break;
+                        mbar_arrive_expect_tx(full(slot), C::K_BYTES);
+                        for (int c = 0; c < D / 64; c++)
+                            tma_load_3d(sb + C::OFF_K + slot * C::K_BYTES + c * (FA_KB * 128), map, full(slot), c * 64, j * FA_KB,
+                                        (half * args.S + str) * args.HK + hk);
+                        n++;
+                    }
+                };
+                for (int j = j_first; j < j_end && ok; j++) {
+                    if (flags[j] == MF_MASKED) continue;
+                    push(&tmK, j);
+                    if (prev >= 0) push(&tmV, prev);
+                    prev = j;
+                }
+                if (prev >= 0) push(&tmV, prev);
+                if (!ok) {   // let every copy already issued land before the CTA exits
+                    bool drained = true;
+                    for (int i = max(0, n - C::RING); i < n; i++) drained &= mbar_drain(full(i % C::RING), (uint32_t)(i / C::RING) & 1u);
+                    if (!drained) atomicCAS(args.err, 0, ERR_WAIT_DRAIN);
+                }
+            } else {
             int i = 0;
             bool ok = true;
             int k_issued[2] = {-1, -1}, v_issued[2] = {-1, -1};
@@ -372,7 +426,62 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
                 }
                 if (!drained) atomicCAS(args.err, 0, ERR_WAIT_DRAIN);
             }
+            }
         }
+    } else if (EXT && warp == 1) {
+        // The whole warp walks the blocks and one lane issues: addresses and descriptors stay in uniform registers.
+        const bool lead = elect_one();
+        auto wait = [&](uint32_t b, uint32_t parity) {
+            return __all_sync(0xffffffffu, mbar_wait(b, parity, args.err, ERR_WAIT_MMA, abort_flag));
+        };
+        int n_active = 0, slot = 0;                      // slot: the ring's next tile
+        uint32_t turn = 0;
+        // the two tiles of K or V: A (TMEM) times their 16-row steps onto d
+        auto product = [&](uint32_t d, uint32_t a, bool v, uint32_t first, uint32_t done) {
+            for (int half = 0; half < 2; half++) {
+                if (!wait(full(slot), turn)) return false;
+                tc_fence_after();
+                const uint32_t tile = sb + C::OFF_K + slot * C::K_BYTES;
+                const uint64_t desc = v ? sdesc_mn_sw128(tile, FA_KB * 128) : sdesc_k_sw128(tile);
+                const uint32_t later = half == 0 ? first : 1u;
+                if (lead) {
+                    if (v) {
+#pragma unroll
+                        for (int ks = 0; ks < FA_KB / 16; ks++)
+                            mma_f16_ts(d, a + 8u * ks, desc + (uint64_t)(ks * 2048 / 16), C::IDESC_O, ks > 0 ? 1u : later);
+                    } else {
+#pragma unroll
+                        for (int ks = 0; ks < D / 16; ks++)
+                            mma_f16_ts(d, a + 8u * ks, desc + (uint64_t)(((ks >> 2) * (FA_KB * 128) + (ks & 3) * 32) / 16),
+                                       C::IDESC_S, ks > 0 ? 1u : later);
+                    }
+                    mma_commit(empty(slot));
+                    if (half == 1) mma_commit(done);
+                }
+                __syncwarp();
+                if (++slot == C::RING) slot = 0, turn ^= 1u;
+            }
+            return true;
+        };
+        auto issue_pv = [&](int i) {
+            return wait(p_full(i & 1), (uint32_t)(i >> 1) & 1u) &&
+                   product(tmem + 256, tmem + C::P_TMEM0, true, i > 0 ? 1u : 0u, pv_done(i & 1));
+        };
+        bool ok = wait(q_full, 0);
+        tc_fence_after();
+        for (int j = j_first; j < j_end && ok; j++) {
+            if (flags[j] == MF_MASKED) continue;
+            const int i = n_active, s = i & 1;
+            ok = wait(s_empty(s), ((uint32_t)(i >> 1) & 1u) ^ 1u) &&
+                 product(tmem + (uint32_t)(s * FA_KB), tmem + C::Q_TMEM0, false, 0u, s_full(s));
+            if (!ok) break;
+            n_active++;
+            if (i > 0) ok = issue_pv(i - 1);
+        }
+        if (ok && n_active > 0) issue_pv(n_active - 1);
+        if (lead) mma_commit(drain);
+        __syncwarp();
+        if (!__all_sync(0xffffffffu, mbar_drain(drain, 0)) && lead) atomicCAS(args.err, 0, ERR_WAIT_DRAIN);
     } else if (warp == 1) {
         if (lane == 0) {
             bool ok = mbar_wait(q_full, 0, args.err, ERR_WAIT_MMA, abort_flag);
@@ -481,6 +590,20 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
             for (int k = 0; k < FA_SPLIT; k++) vals[k] = v[k * 128 + r];
             return true;
         };
+        if constexpr (EXT) {                             // Q's row, this thread's half of it, to TMEM
+            const uint4* src = reinterpret_cast<const uint4*>(args.q16 + (((int64_t)str * args.H + h) * args.T + (row_valid ? t : 0)) * D + pt * (D / 2));
+            uint32_t w[D / 4];
+#pragma unroll
+            for (int n = 0; n < D / 16; n++) {
+                const uint4 v = row_valid ? src[n] : make_uint4(0, 0, 0, 0);
+                w[4 * n] = v.x, w[4 * n + 1] = v.y, w[4 * n + 2] = v.z, w[4 * n + 3] = v.w;
+            }
+            tmem_st_p<D / 4>(tmem + lane_base + C::Q_TMEM0 + (uint32_t)(pt * (D / 4)), w);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
         float m = -INFINITY;                             // running max (log2 units)
         float l = 0.0f;                                  // this thread's partial row sum
         int i = 0;
@@ -584,12 +707,13 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
                     pw[e >> 1] = pack_half2(p0, p1);
                 }
             }
-            // P buffer (i & 1) is free once the P.V of block i-2 has completed
-            if (i >= 2) {
-                if (!wait_pv(i - 2)) { ok = false; break; }
+            // P buffer (i & 1) is free once the P.V of block i-2 has completed (EXT: the one buffer, of block i-1)
+            constexpr int BACK = EXT ? 1 : 2;
+            if (i >= BACK) {
+                if (!wait_pv(i - BACK)) { ok = false; break; }
                 tc_fence_after();
             }
-            tmem_st_p<KPT / 2>(p_lane + (uint32_t)(64 * (i & 1)), pw);
+            tmem_st_p<KPT / 2>(p_lane + (uint32_t)(EXT ? 0 : 64 * (i & 1)), pw);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -764,7 +888,7 @@ static FaLayout fa_layout(int D, int T, int H, int KV, int HK) {
 template <int D, int DV, bool EXT = false>
 static cudaError_t launch_fa(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const FaArgs& a,
                              dim3 grid, cudaStream_t st) {
-    using C = FaCfg<D, DV>;
+    using C = FaCfg<D, DV, EXT>;
     static bool set[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -858,26 +982,31 @@ struct FaQuantPrep {
     int64_t k_r, k_h, k_s;
     const uint8_t* v;
     int64_t v_r, v_h, v_s;
-    __half* k16;
+    __half* k16;                 // [2: rounded values, what rounding left][S][HK][KV][D]
     __half* v16;
     int T, H, KV, HK, S, TQ, n_kvb, n_tb, q_ctas, m_ctas, m_grid;
 };
 
-// The eight values of bytes b of a Q4_0 block as fp16, each code * d rounded once: low nibbles, high nibbles.
-__device__ __forceinline__ void q4_0_values(uint32_t b, uint32_t d2, uint2* lo, uint2* hi) {
+// The eight values of bytes b of a Q4_0 block: code * d as fp16 and what that rounding leaves, exact in fp16
+// again (four bits times eleven); low nibbles, high nibbles.
+__device__ __forceinline__ void q4_0_values(uint32_t b, uint32_t d2, uint2 (&lo)[2], uint2 (&hi)[2]) {
     const __half2 c1032 = __half2half2(__ushort_as_half(0x6408)), c72 = __half2half2(__ushort_as_half(0x5480));
     const __half2 d = *reinterpret_cast<const __half2*>(&d2);
     const uint32_t u = b >> 8;
     const uint32_t w[4] = {(b & 0x000f000fu) | 0x64006400u, (u & 0x000f000fu) | 0x64006400u,
                            (b & 0x00f000f0u) | 0x54005400u, (u & 0x00f000f0u) | 0x54005400u};
-    uint32_t x[4];
+    uint32_t x[4], r[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const __half2 h = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&w[i]), i < 2 ? c1032 : c72), d);
+        const __half2 c = __hsub2(*reinterpret_cast<const __half2*>(&w[i]), i < 2 ? c1032 : c72);
+        const __half2 h = __hmul2(c, d), l = __hfma2(c, d, __hneg2(h));
         x[i] = *reinterpret_cast<const uint32_t*>(&h);
+        r[i] = *reinterpret_cast<const uint32_t*>(&l);
     }
-    *lo = make_uint2(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[0], x[1], 0x7632));
-    *hi = make_uint2(__byte_perm(x[2], x[3], 0x5410), __byte_perm(x[2], x[3], 0x7632));
+    lo[0] = make_uint2(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[0], x[1], 0x7632));
+    hi[0] = make_uint2(__byte_perm(x[2], x[3], 0x5410), __byte_perm(x[2], x[3], 0x7632));
+    lo[1] = make_uint2(__byte_perm(r[0], r[1], 0x5410), __byte_perm(r[0], r[1], 0x7632));
+    hi[1] = make_uint2(__byte_perm(r[2], r[3], 0x5410), __byte_perm(r[2], r[3], 0x7632));
 }
 
 template <int D>
@@ -952,15 +1081,20 @@ __global__ void __launch_bounds__(256) fa_quant_prep_kernel(const FaQuantPrep a)
         if ((votes >> ((threadIdx.x & 31) / LANES * LANES)) & (LANES == 32 ? 0xffffffffu : (1u << LANES) - 1u))
             dk = 0x7e00u, dv = 0u;
         if (!in) continue;
-        uint2 lo, hi;
-        q4_0_values(kw, dk | (dk << 16), &lo, &hi);
-        __half* ko = a.k16 + r * D + 32 * b + 4 * p;
-        *reinterpret_cast<uint2*>(ko) = lo;
-        *reinterpret_cast<uint2*>(ko + 16) = hi;
-        q4_0_values(vw, dv | (dv << 16), &lo, &hi);
-        __half* vo = a.v16 + r * D + 32 * b + 4 * p;
-        *reinterpret_cast<uint2*>(vo) = lo;
-        *reinterpret_cast<uint2*>(vo + 16) = hi;
+        uint2 lo[2], hi[2];
+        q4_0_values(kw, dk | (dk << 16), lo, hi);
+        const int64_t at = r * D + 32 * b + 4 * p;
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            *reinterpret_cast<uint2*>(a.k16 + n * rows * D + at) = lo[n];
+            *reinterpret_cast<uint2*>(a.k16 + n * rows * D + at + 16) = hi[n];
+        }
+        q4_0_values(vw, dv | (dv << 16), lo, hi);
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            *reinterpret_cast<uint2*>(a.v16 + n * rows * D + at) = lo[n];
+            *reinterpret_cast<uint2*>(a.v16 + n * rows * D + at + 16) = hi[n];
+        }
     }
 }
 
@@ -996,8 +1130,8 @@ static FaQuantLayout fa_quant_layout(int64_t D, int64_t T, int64_t H, int64_t KV
     Q.q16_off = take((size_t)(S * H * T * D) * 2);
     Q.qs_off = take((size_t)(S * H * T) * 4);
     Q.flags_off = take((size_t)S * Q.L.n_tb * Q.L.n_kvb);
-    Q.k_off = take((size_t)(S * HK * KV * D) * 2);
-    Q.v_off = take((size_t)(S * HK * KV * D) * 2);
+    Q.k_off = take((size_t)(S * HK * KV * D) * 4);
+    Q.v_off = take((size_t)(S * HK * KV * D) * 4);
     Q.part_off = take((size_t)(rows * D) * 4);
     Q.stat_off = take((size_t)rows * 8);
     Q.total = at;
@@ -1037,16 +1171,16 @@ cudaError_t fa_quant_run(const FaQuantArgs& q, char* ws, cudaStream_t st) {
     const uint64_t D = (uint64_t)q.D, row = D * 2;
     CUtensorMap tq, tk, tv;
     if (!make_tmap_3d_f16(&tq, p.q16, D, q.T, (uint64_t)q.S * q.H, row, (uint64_t)q.T * row, 64, L.TQ, L.GP) ||
-        !make_tmap_3d_f16(&tk, p.k16, D, q.KV, (uint64_t)q.S * q.HK, row, (uint64_t)q.KV * row, 64, FA_KB, 1) ||
-        !make_tmap_3d_f16(&tv, p.v16, D, q.KV, (uint64_t)q.S * q.HK, row, (uint64_t)q.KV * row, 64, FA_KB, 1))
+        !make_tmap_3d_f16(&tk, p.k16, D, q.KV, 2 * (uint64_t)q.S * q.HK, row, (uint64_t)q.KV * row, 64, FA_KB, 1) ||
+        !make_tmap_3d_f16(&tv, p.v16, D, q.KV, 2 * (uint64_t)q.S * q.HK, row, (uint64_t)q.KV * row, 64, FA_KB, 1))
         return cudaErrorInvalidValue;
     FaArgs a{};
-    a.qscale = p.qscale;
+    a.qscale = p.qscale, a.q16 = p.q16;
     a.mask = p.mask;
     a.m_stride = p.m_stride, a.m_stream = p.m_stream, a.mask_vec = q.m_vec != 0;
     a.flags = p.flags;
     a.dst = static_cast<float*>(q.dst);
-    a.T = q.T, a.H = q.H, a.KV = q.KV, a.HK = q.HK, a.GP = L.GP, a.TQ = L.TQ, a.n_hg = L.n_hg, a.n_tb = L.n_tb, a.n_kvb = L.n_kvb;
+    a.S = q.S, a.T = q.T, a.H = q.H, a.KV = q.KV, a.HK = q.HK, a.GP = L.GP, a.TQ = L.TQ, a.n_hg = L.n_hg, a.n_tb = L.n_tb, a.n_kvb = L.n_kvb;
     a.softcap = q.softcap, a.scale = q.scale, a.dst_f16 = q.dst_f16;
     a.units = Q.units;
     a.part = reinterpret_cast<float*>(ws + Q.part_off);
