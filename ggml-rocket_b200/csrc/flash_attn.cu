@@ -1138,6 +1138,11 @@ static FaQuantLayout fa_quant_layout(int64_t D, int64_t T, int64_t H, int64_t KV
     return Q;
 }
 
+int64_t fa_quant_tiles(int64_t T, int64_t H, int64_t HK) {
+    const FaLayout L = fa_layout(64, (int)T, (int)H, 1, (int)HK);
+    return (int64_t)L.n_hg * L.n_tb;
+}
+
 size_t fa_quant_workspace(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S) {
     return fa_quant_layout(D, T, H, KV, HK, S).total;
 }

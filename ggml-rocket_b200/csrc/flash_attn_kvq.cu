@@ -60,9 +60,6 @@ constexpr int KR_MAX_CLUSTER = 8;       // CTAs that join their parts through ea
 constexpr int KR_DEAD = 0x8000;         // of a list entry: a masked tile that was fetched all the same
 constexpr int64_t KR_WAVES = 6;
 constexpr int64_t KR_MIN_SPLIT = 2048;   // keys of a part, where they are many
-// More query rows a KV head than this go to the tcgen05 kernel over fp16 tiles of the cache: the row kernel
-// reads the cache again for every 8 rows, the tiles cost two passes over it whatever the rows.
-constexpr int64_t KR_MAX_ROWS = 32;
 constexpr float KR_LOG2E = 1.4426950408889634f;
 
 struct KvqArgs {
@@ -940,6 +937,16 @@ cudaError_t launch_kvq(const CUtensorMap& tk, const CUtensorMap& tv, const KvqAr
                       (const float*)a.part, (const float*)a.stat, parts, a.dst_f16, a.dst);
 }
 
+// Whether the row kernels take the call, or the tcgen05 kernel over fp16 tiles of the cache. With 32 heads of
+// 128 over 8 KV heads and 16384 keys the row kernels take 15 us and 0.9 us for every 8 rows of a KV head; the
+// other 50 us to make the tiles and 1.25 us for every query tile it has (128 rows, of several heads where
+// a power of two of them shares a KV head). 12 tokens: 56 against 63 us, 16: 69 against 64; 5 tokens of 56
+// heads 55 against 121. 4096 keys cross at the same place (12 tokens 23.5 against 26.7, 24: 35 against 28).
+bool by_rows(int64_t T, int64_t H, int64_t HK) {
+    const int64_t row_tiles = HK * ((T * (H / HK) + KR_ROWS - 1) / KR_ROWS);
+    return 5 * row_tiles <= 25 * HK + 7 * fa_quant_tiles(T, H, HK);
+}
+
 // The sizes the grids and 32-bit counters hold.
 bool kvq_sizes_ok(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S) {
     if ((D != 64 && D != 128) || T <= 0 || T > 65536 || H <= 0 || H > (1 << 20) || KV <= 0 || KV > (1ll << 30) || HK <= 0 ||
@@ -948,7 +955,7 @@ bool kvq_sizes_ok(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64
     const int64_t rows = T * (H / HK);
     if (rows > (1 << 20) || S * T * H > INT32_MAX / 4 || HK * ((rows + KR_ROWS - 1) / KR_ROWS) > 65535) return false;
     // mask blocks of the prompt path: a token at least and 128 keys each
-    return rows <= KR_MAX_ROWS || S * T * ((KV + 127) / 128) <= INT32_MAX;
+    return by_rows(T, H, HK) || S * T * ((KV + 127) / 128) <= INT32_MAX;
 }
 
 }  // namespace
@@ -960,7 +967,7 @@ extern "C" {
 size_t b200_flash_attn_kvq_workspace_size(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S) {
     using namespace b200;
     if (!kvq_sizes_ok(D, T, H, KV, HK, S)) return 0;
-    if (T * (H / HK) > KR_MAX_ROWS) return fa_quant_workspace(D, T, H, KV, HK, S);
+    if (!by_rows(T, H, HK)) return fa_quant_workspace(D, T, H, KV, HK, S);
     return std::max(kvq_plan(D, T, H, KV, HK, S, true).total, kvq_plan(D, T, H, KV, HK, S, false).total);
 }
 
@@ -989,7 +996,7 @@ int b200_flash_attn_kvq(int kv_type, int q_type, const void* q, const int64_t qn
     const size_t need = b200_flash_attn_kvq_workspace_size(D, T, H, KV, HK, S);
     if (!workspace || workspace_bytes < need || off(workspace, 256)) return B200_E_WORKSPACE;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (T * (H / HK) > KR_MAX_ROWS) {
+    if (!by_rows(T, H, HK)) {
         FaQuantArgs f{};
         f.q = static_cast<const char*>(q);
         f.q_t = (int64_t)qnb[1], f.q_h = (int64_t)qnb[2], f.q_s = (int64_t)qnb[3], f.q_f16 = q_type == 1;

@@ -90,6 +90,8 @@ struct FaQuantArgs {
     float scale, softcap;
     int* err;
 };
+// Its query tiles of a stream.
+int64_t fa_quant_tiles(int64_t T, int64_t H, int64_t HK);
 size_t fa_quant_workspace(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S);
 cudaError_t fa_quant_run(const FaQuantArgs& q, char* ws, cudaStream_t st);
 // b200_get_rows over a Q4_0 (2) / Q8_0 (8) table (kv_cache.cu); pointers, shapes and idx checked before.

@@ -178,12 +178,13 @@ int    b200_kv_to_f16(int type, const void * src, int64_t D, int64_t KV, int64_t
  *   dst[:, h, t, s] = sum_j softmax_j(S[j]) v[:, j, h / (H / HK), s],
  *   S[j] = softcap * tanh(scale * q.k / softcap) (scale * q.k when softcap == 0) + mask[s][t][j]
  * A key whose mask is -inf takes no part, whatever its bytes hold; a row with no other key is zeros. D in
- * {64, 128}, H % HK == 0, KV <= 2^30, dst 16-byte aligned. With at most 32 query rows a KV head (T * H / HK)
- * the cache's codes enter the products exactly, and an F32 dst has fp32's accuracy (an F16 dst rounds the
- * softmax weights to fp16). With more the cache is brought to fp16 in the workspace once (values beyond
- * +-65504 become no numbers) and q, the weights and both products' operands are fp16, as in
- * b200_flash_attn_ext. The workspace (256-byte aligned, b200_flash_attn_kvq_workspace_size bytes) holds
- * that and the parts of rows whose keys several CTAs share; calls sharing one must not overlap on the GPU.
+ * {64, 128}, H % HK == 0, KV <= 2^30, dst 16-byte aligned. With at most 48 query rows a KV head (T * H / HK),
+ * and with more where that is faster, the cache's codes enter the products exactly, and an F32 dst has fp32's
+ * accuracy (an F16 dst rounds the softmax weights to fp16). Otherwise the cache is brought to pairs of fp16
+ * tiles in the workspace once, which hold its values exactly (those beyond +-65504 become no numbers), and q
+ * and the softmax weights are rounded to fp16. The workspace (256-byte aligned,
+ * b200_flash_attn_kvq_workspace_size bytes; the calling device's) holds that and the parts of rows whose
+ * keys several CTAs share; calls sharing one must not overlap on the GPU.
  * No ALiBi, no sinks. */
 size_t b200_flash_attn_kvq_workspace_size(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S);
 int    b200_flash_attn_kvq(int kv_type, int q_type, const void * q, const int64_t qne[4], const size_t qnb[4],

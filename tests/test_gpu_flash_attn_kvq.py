@@ -359,6 +359,10 @@ def test_cache_past_32_bits(cuda):
     (1, 17, 2, 1, 128, 1),
     (1, 64, 6, 3, 64, 20),           # more tokens than keys
     (2, 1, 4, 2, 128, 127),
+    (1, 12, 8, 2, 128, 700),         # either side of the row kernels' last size
+    (1, 13, 8, 2, 128, 700),
+    (2, 16, 14, 2, 64, 900),         # a group of seven: rows for longer
+    (1, 100, 7, 1, 128, 300),
 ])
 def test_shapes_at_the_ends(cuda, S, T, H, HK, D, KV, f16):
     """A random mask, its first row of every stream hidden whole, its last key of every other row visible."""
