@@ -15,6 +15,7 @@
 //              whole key range, rescaled in place only when a row max grows by more than 2^8.
 //              K and V tiles arrive by TMA straight from the op's strided cache views, two
 //              stages deep.
+// Further down: the same over a Q4_0 cache and several streams (b200_flash_attn_kvq's larger calls).
 #include <algorithm>
 #include <cstdint>
 #include <cstring>
@@ -274,7 +275,14 @@ __device__ __forceinline__ FaUnit fa_unit(const FaUnits& u, int n_kvb) {
 }
 
 // EXT: several streams (heads of q16 and of K / V numbered stream by stream), tiles whose keys CTAs share,
-// scores scaled after the product, a key whose mask is -inf left out whatever its score.
+// scores scaled after the product, a key whose mask is -inf left out whatever its score, and K and V as two
+// halves each: a value of a Q4_0 cache, a 4-bit code times an 11-bit scale, is no fp16 number, and rounding it
+// to one doubles the error of an fp16 result (4.4e-4 of it against 2.9e-4, of which 2.1e-4 are its own
+// rounding). So S = Q (K_hi + K_lo)^T, O += P (V_hi + V_lo): twice the products. Q lies in TMEM, which
+// leaves shared memory's bandwidth to the tiles and its room to a longer ring (933 -> 868 us, 2048 tokens x
+// 16384 keys, 32 heads over 8); the products are issued from a converged warp (868 -> 673): by one lane of a
+// divergent one, each took its operands to uniform registers first, and the tensor core waited for the issue.
+// Now it is busy two thirds of the time; the rest is the chain scores - softmax - P within a block.
 template <int D, int DV, bool EXT>
 __global__ void __launch_bounds__(FA_THREADS, 1)
 fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -967,7 +975,9 @@ int flash_attn_impl(const float* q, int64_t q_nb1, int64_t q_nb2, const void* k,
 
 // Set-up pass of one launch: CTAs [0, q_ctas) bring q to fp16 (one warp a row, a power-of-two divisor for
 // rows beyond fp16's range; not scaled, so that f16 values stay exact), the next m_ctas classify the mask,
-// the rest bring the cache to fp16: four lanes a block of 32 values, each eight of them.
+// the rest bring the cache to pairs of fp16 tiles: four lanes a block of 32 values, each eight of them. Bound by
+// HBM and L2: 16384 keys, 8 KV heads of 128, 2048 tokens of 32 heads, 56 us for 19 MB of cache, 67 MB of mask
+// and 17 MB of q read and 151 MB written (4.5 TB/s); making the tiles costs the call once what every query tile would else pay.
 struct FaQuantPrep {
     const char* q;
     int64_t q_t, q_h, q_s;

