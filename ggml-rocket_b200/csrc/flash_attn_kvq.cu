@@ -852,7 +852,8 @@ KvqPlan kvq_plan(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_
     // (one stream x 16384 keys 24.2 -> 18.1 us, x 512 keys 9.3 -> 8.4). Otherwise CTAs stand alone: clusters
     // wait for their slowest and for room in one GPC (32 streams x 16384 keys 167 us alone, 202 in clusters).
     // Then one wave when the keys are few, several where they are many, with at least KR_MIN_SPLIT keys each,
-    // so that streams of unequal length even out.
+    // so that streams of unequal length even out, and up to two waves with half as many (8 streams x 16384
+    // keys 57.5 -> 53.0 us, 32 x 5000 79 -> 68; for every wave it is slower: 32 x 16384 166 -> 170).
     const int64_t slots = (int64_t)device_sm_count() * 3, fit = slots * 7 / 8;
     int64_t splits = 0;
     p.cluster = 1;
@@ -869,6 +870,7 @@ KvqPlan kvq_plan(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_
     if (!splits) {
         splits = std::max<int64_t>(1, slots / ctas);
         splits = std::max(splits, std::min(KR_WAVES * slots / ctas, tiles * tk / KR_MIN_SPLIT));
+        splits = std::max(splits, std::min(2 * slots / ctas, 2 * tiles * tk / KR_MIN_SPLIT));
         splits = std::min(splits, tiles);
     }
     splits = std::max(splits, (tiles + KR_MAX_TILES - 1) / KR_MAX_TILES);
