@@ -347,7 +347,7 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
         mbar_init(drain, 1);
         *abort_flag = 0;
         fence_barrier_init();
-        tma_prefetch_desc(&tmQ);
+        if constexpr (!EXT) tma_prefetch_desc(&tmQ);
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
     }
@@ -407,33 +407,33 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
                     if (!drained) atomicCAS(args.err, 0, ERR_WAIT_DRAIN);
                 }
             } else {
-            int i = 0;
-            bool ok = true;
-            int k_issued[2] = {-1, -1}, v_issued[2] = {-1, -1};
-            for (int j = j_first; j < j_end && ok; j++) {
-                if (flags[j] == MF_MASKED) continue;
-                const int s = i & 1;
-                const uint32_t ph = (uint32_t)(i >> 1) & 1u;
-                if (!mbar_wait(k_empty(s), ph ^ 1u, args.err, ERR_WAIT_PRODUCER, abort_flag)) { ok = false; break; }
-                k_issued[s] = (int)ph;
-                mbar_arrive_expect_tx(k_full(s), C::K_BYTES);
-                for (int c = 0; c < D / 64; c++)
-                    tma_load_3d(sb + C::OFF_K + s * C::K_BYTES + c * (FA_KB * 128), &tmK, k_full(s), c * 64, j * FA_KB, str * args.HK + hk);
-                if (!mbar_wait(v_empty(s), ph ^ 1u, args.err, ERR_WAIT_PRODUCER, abort_flag)) { ok = false; break; }
-                v_issued[s] = (int)ph;
-                mbar_arrive_expect_tx(v_full(s), C::V_BYTES);
-                for (int c = 0; c < DV / 64; c++)
-                    tma_load_3d(sb + C::OFF_V + s * C::V_BYTES + c * (FA_KB * 128), &tmV, v_full(s), c * 64, j * FA_KB, str * args.HK + hk);
-                i++;
-            }
-            if (!ok) {   // let every copy already issued land before the CTA exits
-                bool drained = mbar_drain(q_full, 0);
-                for (int s = 0; s < 2; s++) {
-                    if (k_issued[s] >= 0) drained &= mbar_drain(k_full(s), (uint32_t)k_issued[s]);
-                    if (v_issued[s] >= 0) drained &= mbar_drain(v_full(s), (uint32_t)v_issued[s]);
+                int i = 0;
+                bool ok = true;
+                int k_issued[2] = {-1, -1}, v_issued[2] = {-1, -1};
+                for (int j = j_first; j < j_end && ok; j++) {
+                    if (flags[j] == MF_MASKED) continue;
+                    const int s = i & 1;
+                    const uint32_t ph = (uint32_t)(i >> 1) & 1u;
+                    if (!mbar_wait(k_empty(s), ph ^ 1u, args.err, ERR_WAIT_PRODUCER, abort_flag)) { ok = false; break; }
+                    k_issued[s] = (int)ph;
+                    mbar_arrive_expect_tx(k_full(s), C::K_BYTES);
+                    for (int c = 0; c < D / 64; c++)
+                        tma_load_3d(sb + C::OFF_K + s * C::K_BYTES + c * (FA_KB * 128), &tmK, k_full(s), c * 64, j * FA_KB, str * args.HK + hk);
+                    if (!mbar_wait(v_empty(s), ph ^ 1u, args.err, ERR_WAIT_PRODUCER, abort_flag)) { ok = false; break; }
+                    v_issued[s] = (int)ph;
+                    mbar_arrive_expect_tx(v_full(s), C::V_BYTES);
+                    for (int c = 0; c < DV / 64; c++)
+                        tma_load_3d(sb + C::OFF_V + s * C::V_BYTES + c * (FA_KB * 128), &tmV, v_full(s), c * 64, j * FA_KB, str * args.HK + hk);
+                    i++;
                 }
-                if (!drained) atomicCAS(args.err, 0, ERR_WAIT_DRAIN);
-            }
+                if (!ok) {   // let every copy already issued land before the CTA exits
+                    bool drained = mbar_drain(q_full, 0);
+                    for (int s = 0; s < 2; s++) {
+                        if (k_issued[s] >= 0) drained &= mbar_drain(k_full(s), (uint32_t)k_issued[s]);
+                        if (v_issued[s] >= 0) drained &= mbar_drain(v_full(s), (uint32_t)v_issued[s]);
+                    }
+                    if (!drained) atomicCAS(args.err, 0, ERR_WAIT_DRAIN);
+                }
             }
         }
     } else if (EXT && warp == 1) {
@@ -1184,9 +1184,8 @@ cudaError_t fa_quant_run(const FaQuantArgs& q, char* ws, cudaStream_t st) {
                               : launch_pdl(fa_quant_prep_kernel<128>, grid, block, 0, st, p);
     if (e != cudaSuccess) return e;
     const uint64_t D = (uint64_t)q.D, row = D * 2;
-    CUtensorMap tq, tk, tv;
-    if (!make_tmap_3d_f16(&tq, p.q16, D, q.T, (uint64_t)q.S * q.H, row, (uint64_t)q.T * row, 64, L.TQ, L.GP) ||
-        !make_tmap_3d_f16(&tk, p.k16, D, q.KV, 2 * (uint64_t)q.S * q.HK, row, (uint64_t)q.KV * row, 64, FA_KB, 1) ||
+    CUtensorMap tk, tv;
+    if (!make_tmap_3d_f16(&tk, p.k16, D, q.KV, 2 * (uint64_t)q.S * q.HK, row, (uint64_t)q.KV * row, 64, FA_KB, 1) ||
         !make_tmap_3d_f16(&tv, p.v16, D, q.KV, 2 * (uint64_t)q.S * q.HK, row, (uint64_t)q.KV * row, 64, FA_KB, 1))
         return cudaErrorInvalidValue;
     FaArgs a{};
@@ -1202,7 +1201,8 @@ cudaError_t fa_quant_run(const FaQuantArgs& q, char* ws, cudaStream_t st) {
     a.stat = reinterpret_cast<float*>(ws + Q.stat_off);
     a.err = q.err;
     const dim3 fgrid((unsigned)(Q.units.whole + Q.cut_tiles * Q.units.cut));
-    e = q.D == 64 ? launch_fa<64, 64, true>(tq, tk, tv, a, fgrid, st) : launch_fa<128, 128, true>(tq, tk, tv, a, fgrid, st);
+    // no map of Q, whose rows the softmax threads bring to TMEM: K's stands in its place, unused
+    e = q.D == 64 ? launch_fa<64, 64, true>(tk, tk, tv, a, fgrid, st) : launch_fa<128, 128, true>(tk, tk, tv, a, fgrid, st);
     if (e != cudaSuccess || Q.cut_tiles == 0) return e;
     const int rows = Q.cut_tiles * FA_ROWS;
     auto join = [&](auto kernel, int warps) {
