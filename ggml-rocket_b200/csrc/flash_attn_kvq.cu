@@ -16,10 +16,10 @@
 //   O^T = V^T P^T the codes are the A operand (16 head dimensions x 16 keys), P times the value
 //                 scales the B operand, straight from the score fragments' layout.
 //
-// P * scale is brought into fp16's range by a power of two per 32 keys (their largest value scale) and,
-// for an f32 result, split into a high and a low half as well; for an fp16 result its rounding (2^-12)
-// stays below the result's own. Sums, maxima and outputs are fp32 throughout; the output sums of 32
-// keys are added to the running ones by an fp32 FMA.
+// P * scale is brought into fp16's range by a power of two per 32 keys (their largest value scale) and
+// split into a high and a low half as well, for an fp16 result too: P rounded to fp16 alone takes its error
+// from 2.1e-4, its own rounding, to as much as 3e-4. Sums, maxima and outputs are fp32 throughout; the output
+// sums of 32 keys are added to the running ones by an fp32 FMA.
 //
 // Scores are in log2 units, taken relative to the largest mask value of the row in the CTA's range,
 // whose difference to a key's mask is exact in fp32 also when every mask value is fp16's lowest.
@@ -38,7 +38,8 @@
 //
 // Bound by the issue of instructions, not by HBM: about 30 a key and KV head (decoding the codes, their
 // fragments, the softmax). 64 streams x 32000 keys, 8 KV heads of 128: 554 us, 3.2 TB/s of cache, 0.49 of
-// the measured copy bandwidth, 63 % of the issue slots; 32 streams of 8192 to 16384 keys 164 us (2.8 TB/s).
+// the measured copy bandwidth, 63 % of the issue slots; 32 streams of 8192 to 16384 keys 178 us (2.6 TB/s; 164
+// with softmax weights of fp16, which an fp16 result showed).
 // A single stream is latency: 16384 keys 17.2 us, 512 keys 7.4 us, of which some 4 are launch, mask and q.
 #include <algorithm>
 #include <cmath>
@@ -190,15 +191,13 @@ struct KrCfg {
     static_assert(OFF_CTA + HPB * KR_ROWS * (D + 2) * 4 <= RING && OFF_CTA % 16 == 0 && OFF_BAR % 8 == 0 && OFF_Q % 16 == 0 && HALF % 128 == 0);
 };
 
-// MT: the most tokens a CTA's rows come from (1 or 8). MODE: 0 f16 q and result (q has no low half), 1 f16
-// result, 2 f32 result (P split in two halves). Leaving the codes' offsets in the MMA and starting its sums
+// MT: the most tokens a CTA's rows come from (1 or 8). QLO: q is f32 (an f16 q has no low half). Leaving the codes' offsets in the MMA and starting its sums
 // from minus the offset times sum(q), sum(P) saves the fp16 subtractions but measured slower (562 against
 // 554 us over 64 streams x 32000 keys): they use a pipe that is idle.
-template <int D, int MT, int MODE, int HPB>
+template <int D, int MT, bool QLO, int HPB>
 __global__ void __launch_bounds__(KrCfg<D, MT, HPB>::THREADS, 3)
 kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const KvqArgs a) {
     using C = KrCfg<D, MT, HPB>;
-    constexpr bool EXACT = MODE == 2, QLO = MODE > 0;
     extern __shared__ __align__(128) uint8_t sm[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const int packs = a.HK / HPB;
@@ -616,10 +615,8 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                     w1 = s[j][1] == 0.0f ? 0.0f : w1;
                 }
                 ph[j] = pack_half2(w0, w1);
-                if constexpr (EXACT) {
-                    const float2 h = h2f(ph[j]);
-                    pl[j] = pack_half2(w0 - h.x, w1 - h.y);
-                }
+                const float2 h = h2f(ph[j]);
+                pl[j] = pack_half2(w0 - h.x, w1 - h.y);
             }
             float ot[2][4];
 #pragma unroll
@@ -633,8 +630,7 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                 for (int m = 0; m < 2; m++) {
                     if (jj > 0) mma_16816(ot[m], f0[2 * m], f0[2 * m + 1], f1[2 * m], f1[2 * m + 1], ph[2 * jj], ph[2 * jj + 1]);
                     else mma_16816_first(ot[m], f0[2 * m], f0[2 * m + 1], f1[2 * m], f1[2 * m + 1], ph[0], ph[1]);
-                    if constexpr (EXACT)
-                        mma_16816(ot[m], f0[2 * m], f0[2 * m + 1], f1[2 * m], f1[2 * m + 1], pl[2 * jj], pl[2 * jj + 1]);
+                    mma_16816(ot[m], f0[2 * m], f0[2 * m + 1], f1[2 * m], f1[2 * m + 1], pl[2 * jj], pl[2 * jj + 1]);
                 }
             }
 #pragma unroll
@@ -910,19 +906,19 @@ bool make_cache_map(CUtensorMap* map, const void* base, int64_t row_bytes, int64
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, int MT, int MODE, int HPB>
+template <int D, int MT, bool QLO, int HPB>
 cudaError_t launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const KvqArgs& a, dim3 grid, cudaStream_t st) {
     using C = KrCfg<D, MT, HPB>;
     static bool set[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !set[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(kvq_rows_kernel<D, MT, MODE, HPB>,
+        const cudaError_t e = cudaFuncSetAttribute(kvq_rows_kernel<D, MT, QLO, HPB>,
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) set[dev] = true;
     }
-    return launch_pdl_cluster(kvq_rows_kernel<D, MT, MODE, HPB>, grid, dim3(C::THREADS), C::SMEM, st, a.cluster, tk, tv, a);
+    return launch_pdl_cluster(kvq_rows_kernel<D, MT, QLO, HPB>, grid, dim3(C::THREADS), C::SMEM, st, a.cluster, tk, tv, a);
 }
 
 template <int D, int HPB>
@@ -931,14 +927,9 @@ cudaError_t launch_kvq(const CUtensorMap& tk, const CUtensorMap& tv, const KvqAr
     const dim3 grid((unsigned)a.splits, (unsigned)(a.HK / HPB * ((rows + KR_ROWS - 1) / KR_ROWS)), (unsigned)a.S);
     // one token a CTA: its mask is one row, and keys it hides are hidden from all the CTA's rows
     const bool one = a.T == 1 || a.G % KR_ROWS == 0;
-    const int mode = a.dst_f16 ? (a.q_f16 ? 0 : 1) : 2;
     cudaError_t e;
-    if (one)
-        e = mode == 0 ? launch_rows<D, 1, 0, HPB>(tk, tv, a, grid, st)
-          : mode == 1 ? launch_rows<D, 1, 1, HPB>(tk, tv, a, grid, st) : launch_rows<D, 1, 2, HPB>(tk, tv, a, grid, st);
-    else
-        e = mode == 0 ? launch_rows<D, 8, 0, HPB>(tk, tv, a, grid, st)
-          : mode == 1 ? launch_rows<D, 8, 1, HPB>(tk, tv, a, grid, st) : launch_rows<D, 8, 2, HPB>(tk, tv, a, grid, st);
+    if (one) e = a.q_f16 ? launch_rows<D, 1, false, HPB>(tk, tv, a, grid, st) : launch_rows<D, 1, true, HPB>(tk, tv, a, grid, st);
+    else e = a.q_f16 ? launch_rows<D, 8, false, HPB>(tk, tv, a, grid, st) : launch_rows<D, 8, true, HPB>(tk, tv, a, grid, st);
     const int parts = a.splits / a.cluster;
     if (e != cudaSuccess || parts == 1) return e;
     return launch_pdl(kvq_join_kernel<D>, dim3((unsigned)((int64_t)a.S * a.T * a.H)), dim3(128), 0, st,

@@ -180,7 +180,7 @@ int    b200_kv_to_f16(int type, const void * src, int64_t D, int64_t KV, int64_t
  * A key whose mask is -inf takes no part, whatever its bytes hold; a row with no other key is zeros. D in
  * {64, 128}, H % HK == 0, KV <= 2^30, dst 16-byte aligned. With at most 48 query rows a KV head (T * H / HK),
  * and with more where that is faster, the cache's codes enter the products exactly, and an F32 dst has fp32's
- * accuracy (an F16 dst rounds the softmax weights to fp16). Otherwise the cache is brought to pairs of fp16
+ * accuracy (an F16 dst adds its own rounding alone). Otherwise the cache is brought to pairs of fp16
  * tiles in the workspace once, which hold its values exactly (those beyond +-65504 become no numbers), and q
  * and the softmax weights are rounded to fp16. The workspace (256-byte aligned,
  * b200_flash_attn_kvq_workspace_size bytes; the calling device's) holds that and the parts of rows whose

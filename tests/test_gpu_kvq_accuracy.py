@@ -1,0 +1,45 @@
+"""How near b200_flash_attn_kvq comes to its definition in 64 bits, whichever kernel takes the call.
+
+Tolerance, per element. Let A be the largest scale * sum_i |q_i k_i| of a row, B the same with the row's
+largest |q| in the place of q_i, V the largest |v|, N the number of keys.
+- q lies in two fp16 halves: what they leave is 2^-22 of the row's largest value, B 2^-22 of a score.
+- The exact products are added in fp32, the tensor core truncating: at most 32 steps of 2^-23 of A, with the
+  product of the two low halves left out (2^-22 A) and the roundings of scale, cap and log2(e) well inside.
+- ex2 is within 2^-22; a weight's two halves leave 2^-22 of it; the row's sum rounds a few times.
+So a weight is off by e = A 2^-18 + B 2^-22 + 2^-20, relative. Outputs are ratios of two sums of such weights:
+2 e V, and the sums are added in at most 3 N / 16 + 32 steps of 2^-23 of V. An f16 result adds its own rounding,
+half a step: 2^-11 of the value, 2^-25 in the subnormal range."""
+import math
+
+import pytest
+
+from test_gpu_flash_attn_kvq import causal, decode64, inputs, reference, run
+
+pytestmark = pytest.mark.gpu
+
+
+def check(out, q, k, v, mask, scale, softcap=0.0, key=None):
+    import torch
+    want, A, vmax = reference(q, k, v, mask, scale, softcap)
+    G = q.shape[2] // k.shape[2]
+    ks = decode64(k).abs().sum(-1).amax(1).repeat_interleave(G, 1)          # [S, H]: sum |k_i| of the largest key
+    B = abs(scale) * q.double().abs().amax(-1) * ks[:, None]                # [S, T, H]
+    e = A * 2.0 ** -18 + B[..., None] * 2.0 ** -22 + 2.0 ** -20
+    tol = (2 * e + (3 * k.shape[1] / 16 + 32) * 2.0 ** -23) * vmax
+    if out.dtype == torch.float16:
+        tol = tol + 2.0 ** -11 * want.abs() + 2.0 ** -25
+    d = (out.double() - want).abs()
+    assert bool((d <= tol).all()), (float((d - tol).max()), float((d / tol).max()))
+
+
+@pytest.mark.parametrize("q_f16", [False, True])
+@pytest.mark.parametrize("S,T,H,HK,D,KV", [
+    (40, 1, 8, 2, 128, 3),
+    (40, 1, 8, 2, 64, 9),
+    (40, 2, 8, 2, 128, 8),           # rows of two tokens in a tile
+    (40, 1, 3, 1, 128, 5),           # a head alone in its cache row
+])
+def test_f16_results_of_few_rows_lose_their_own_rounding_alone(cuda, S, T, H, HK, D, KV, q_f16):
+    """Few keys, so that the softmax weights' rounding does not average out."""
+    q, k, v = inputs(S, T, H, HK, D, KV, seed=3, q_f16=q_f16)
+    check(run(q, k, v, None, 1 / 128, True), q, k, v, None, 1 / 128)
