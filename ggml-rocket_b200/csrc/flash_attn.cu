@@ -567,10 +567,14 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
         volatile int* xls = reinterpret_cast<volatile int*>(smem + C::OFF_XCH + 2 * C::XCH_MAX + C::XCH_SUM);
         // this thread's keys of a block are P columns [KPT/2*pt, KPT/2*(pt+1)) of the P buffer
         const uint32_t p_lane = tmem + lane_base + C::P_TMEM0 + (uint32_t)(pt * (KPT / 2));
-        // wait until the P.V MMA of block k has completed (pv_done[k & 1], completion k >> 1)
-        auto wait_pv = [&](int k) {
-            return mbar_wait(pv_done(k & 1), (uint32_t)(k >> 1) & 1u, args.err, ERR_WAIT_EPILOGUE, abort_flag);
+        // A wait may give up in some lanes of a warp alone; votes, tcgen05.ld and .st take all of them, so the
+        // warp goes on, or leaves, together.
+        auto together = [](bool got) { return __all_sync(0xffffffffu, got) != 0; };
+        auto wait = [&](uint32_t b, uint32_t parity) {
+            return together(mbar_wait(b, parity, args.err, ERR_WAIT_EPILOGUE, abort_flag));
         };
+        // wait until the P.V MMA of block k has completed (pv_done[k & 1], completion k >> 1)
+        auto wait_pv = [&](int k) { return wait(pv_done(k & 1), (uint32_t)(k >> 1) & 1u); };
         // Publish a value to the other threads of this row and wait for theirs: a bounded spin on
         // sequence numbers in shared memory (the threads are in different warps). vals[k] gets
         // part k's value.
@@ -623,7 +627,7 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
             const bool general = use_mask || softcap != 0.0f || (j + 1) * FA_KB > args.KV || (EXT && !(args.scale >= 0.0f));
             const int s = i & 1;
             const uint32_t ph = (uint32_t)(i >> 1) & 1u;
-            if (!mbar_wait(s_full(s), ph, args.err, ERR_WAIT_EPILOGUE, abort_flag)) { ok = false; break; }
+            if (!wait(s_full(s), ph)) { ok = false; break; }
             tc_fence_after();
             float x[KPT];
 #pragma unroll
@@ -668,7 +672,7 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
             }
             // the row max over all parts (double-buffered by block parity)
             float maxes[FA_SPLIT];
-            if (!exchange(xv + (i & 1) * (FA_SPLIT * 128), xs + (i & 1) * (FA_SPLIT * 128), bmax, i + 1, maxes)) {
+            if (!together(exchange(xv + (i & 1) * (FA_SPLIT * 128), xs + (i & 1) * (FA_SPLIT * 128), bmax, i + 1, maxes))) {
                 ok = false;
                 break;
             }
@@ -735,7 +739,7 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
         }
         // row sum over all parts, added in part order so every thread of the row agrees
         float sums[FA_SPLIT];
-        if (ok && !exchange(xl, xls, l, 1, sums)) ok = false;
+        if (ok && !together(exchange(xl, xls, l, 1, sums))) ok = false;
         float l_tot = 0.0f;
 #pragma unroll
         for (int k = 0; k < FA_SPLIT; k++) l_tot += sums[k];
