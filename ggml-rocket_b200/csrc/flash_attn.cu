@@ -45,7 +45,7 @@ struct FaUnits {
 };
 
 struct FaArgs {
-    const float* qscale;       // [H*T] per-row divisor (1 unless out of fp16 range)
+    const float* qscale;       // [H*T] per-row divisor (1 unless out of fp16 range); EXT: [S*H*T], times the scale
     const uint16_t* mask;      // F16 mask or nullptr
     int64_t m_stride;          // mask row stride, elements
     bool mask_vec;             // rows 16-byte aligned: 16-byte loads
@@ -552,8 +552,7 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
         const int h = hg * args.GP + g;
         const int t = tb * args.TQ + tq;
         const bool row_valid = t < args.T;
-        const float qs = (row_valid ? __ldg(args.qscale + ((int64_t)str * args.H + h) * args.T + t) : 1.0f) *
-                         (EXT ? args.scale : 1.0f);
+        const float qs = row_valid ? __ldg(args.qscale + ((int64_t)str * args.H + h) * args.T + t) : 1.0f;
         const uint16_t* mrow = (args.mask && row_valid) ? args.mask + (EXT ? str * args.m_stream : 0) + (int64_t)t * args.m_stride
                                                         : nullptr;
         const float LOG2E = 1.4426950408889634f;
@@ -987,7 +986,7 @@ struct FaQuantPrep {
     int64_t q_t, q_h, q_s;
     int q_f16;
     __half* q16;
-    float* qscale;
+    float* qscale;               // per row: the scale times the divisor
     const uint16_t* mask;
     int64_t m_stride, m_stream;
     int mask_vec;
@@ -999,6 +998,7 @@ struct FaQuantPrep {
     __half* k16;                 // [2: rounded values, what rounding left][S][HK][KV][D]
     __half* v16;
     int T, H, KV, HK, S, TQ, n_kvb, n_tb, q_ctas, m_ctas, m_grid;
+    float scale;
 };
 
 // The eight values of bytes b of a Q4_0 block: code * d as fp16 and what that rounding leaves, exact in fp16
@@ -1052,11 +1052,11 @@ __global__ void __launch_bounds__(256) fa_quant_prep_kernel(const FaQuantPrep a)
         // f32 rows are brought near 1 as well, so that small ones keep fp16's full precision
         int e = 0;
         if (!a.q_f16 && amax > 0.0f && amax <= 3.402823466e38f) frexpf(amax, &e);
-        e = max(-100, e);
+        e = max(-126, e);
 #pragma unroll
         for (int i = 0; i < PER; i += 2)
             *reinterpret_cast<uint32_t*>(a.q16 + row * D + lane * PER + i) = pack_half2(ldexpf(x[i], -e), ldexpf(x[i + 1], -e));
-        if (lane == 0) a.qscale[row] = ldexpf(1.0f, e);
+        if (lane == 0) a.qscale[row] = ldexpf(a.scale, e);   // the scale within: 2^128 alone would be no f32 number
         return;
     }
     const int mi = (int)blockIdx.x - a.q_ctas;
@@ -1175,7 +1175,7 @@ cudaError_t fa_quant_run(const FaQuantArgs& q, char* ws, cudaStream_t st) {
     p.v = reinterpret_cast<const uint8_t*>(q.v), p.v_r = q.v_r, p.v_h = q.v_h, p.v_s = q.v_s;
     p.k16 = reinterpret_cast<__half*>(ws + Q.k_off);
     p.v16 = reinterpret_cast<__half*>(ws + Q.v_off);
-    p.T = q.T, p.H = q.H, p.KV = q.KV, p.HK = q.HK, p.S = q.S;
+    p.T = q.T, p.H = q.H, p.KV = q.KV, p.HK = q.HK, p.S = q.S, p.scale = q.scale;
     p.TQ = L.TQ, p.n_kvb = L.n_kvb, p.n_tb = L.n_tb;
     const int sms = device_sm_count();
     p.q_ctas = (int)(((int64_t)q.S * q.H * q.T + 7) / 8);

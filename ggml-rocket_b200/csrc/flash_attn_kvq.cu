@@ -342,7 +342,7 @@ kvq_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         int ex = 0;
         if (amax > 0.0f && amax <= 3.402823466e38f) frexpf(amax, &ex);
-        ex = max(-100, ex - 10);
+        ex = max(-126, ex - 10);                         // 2^126: the largest power whose inverse is a normal number
         const float mul = ldexpf(1.0f, -ex);
         if (t4 == 0) backs[warp * KR_ROWS + g] = ldexpf(a.scale, ex);   // what undoes it, with the scale
 #pragma unroll

@@ -13,6 +13,7 @@ import math
 
 import pytest
 
+from test_gpu_flash_attn_kvq import check as loose
 from test_gpu_flash_attn_kvq import causal, decode64, inputs, reference, run
 
 pytestmark = pytest.mark.gpu
@@ -43,3 +44,11 @@ def test_f16_results_of_few_rows_lose_their_own_rounding_alone(cuda, S, T, H, HK
     """Few keys, so that the softmax weights' rounding does not average out."""
     q, k, v = inputs(S, T, H, HK, D, KV, seed=3, q_f16=q_f16)
     check(run(q, k, v, None, 1 / 128, True), q, k, v, None, 1 / 128)
+
+
+@pytest.mark.parametrize("T", [1, 60])
+def test_queries_at_the_end_of_f32(cuda, T):
+    """The largest |q| at 2^127 and above, and among f32's smallest, with a scale that brings them back."""
+    q, k, v = inputs(1, T, 8, 2, 128, 300)
+    for qq, scale in ((q.sign() * 3e38, 1e-39), (q / q.abs().max() * 3.4e38, 2e-39), (q * 1e-38, 1e37)):
+        loose(run(qq, k, v, None, scale), qq, k, v, None, scale)
