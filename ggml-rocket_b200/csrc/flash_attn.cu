@@ -53,7 +53,7 @@ struct FaArgs {
     float* dst;                // [T][H][DV]
     int T, H, KV, HK, GP, TQ, n_hg, n_tb, n_kvb;
     int S;                     // EXT: streams
-    const __half* q16;         // EXT: [S][H][T][D]
+    const __half* q16;         // EXT: [S][H][T][D], an f32 q's low halves behind them
     float softcap;
     int* err;
     // the extended form only (several streams, parts of the keys, f16 results; q16 not scaled)
@@ -256,9 +256,10 @@ struct FaCfg {
     // TMEM columns: S0 [0,128) | S1 [128,256) | O [256, 256+DV) | P0 [384,448) | P1 [448,512)
     // (P is fp16, two keys per 32-bit column, read by the P.V MMA as its A operand)
     static constexpr uint32_t TMEM_COLS = 512;
-    // EXT: Q [384, 384+D/2), one P buffer [448,512)
-    static constexpr uint32_t P_TMEM0 = EXT ? 448 : 384;
-    static constexpr uint32_t Q_TMEM0 = 384;
+    static constexpr uint32_t P_TMEM0 = 384;
+    // EXT: Q's high halves [384, 384+D/2), its low ones [448, 448+D/2). P takes the place of the scores it is
+    // made of: keys 64 pt .. 64 pt + 63 as columns 64 pt (high halves) and 64 pt + 32 (low halves) of S's 128.
+    static constexpr uint32_t Q_TMEM0 = 384, Q_LO = 64, P_LO = 32;
     static constexpr uint32_t IDESC_S = idesc_f16_f32(FA_ROWS, FA_KB);
     static constexpr uint32_t IDESC_O = idesc_f16_f32_bmn(FA_ROWS, DV);
 };
@@ -275,15 +276,15 @@ __device__ __forceinline__ FaUnit fa_unit(const FaUnits& u, int n_kvb) {
 }
 
 // EXT: several streams (heads of q16 and of K / V numbered stream by stream), tiles whose keys CTAs share,
-// scores scaled after the product, a key whose mask is -inf left out whatever its score, and K and V as two
-// halves each: a value of a Q4_0 cache, a 4-bit code times an 11-bit scale, is no fp16 number, and rounding it
-// to one doubles the error of an fp16 result (4.4e-4 of it against 2.9e-4, of which 2.1e-4 are its own
-// rounding). So S = Q (K_hi + K_lo)^T, O += P (V_hi + V_lo): twice the products. Q lies in TMEM, which
-// leaves shared memory's bandwidth to the tiles and its room to a longer ring (933 -> 868 us, 2048 tokens x
-// 16384 keys, 32 heads over 8); the products are issued from a converged warp (868 -> 673): by one lane of a
+// scores scaled after the product, a key whose mask is -inf left out whatever its score, and every operand to
+// 22 bits as two fp16 halves: K and V (a 4-bit code times an 11-bit scale is no fp16 number), the softmax
+// weights P and, where it is f32 (QLO), q. S = Q_hi K_hi + Q_lo K_hi + Q_hi K_lo, O likewise of P and V: the
+// products of two low halves are below 2^-22. Operands rounded to fp16 took an fp16 result's error from 2.1e-4,
+// its own rounding, to 4.4e-4, and with P alone rounded to 2.9e-4. Q and P lie in TMEM, which leaves shared
+// memory's bandwidth and its room to the ring of tiles; P takes the columns of the scores it is made of, so the
+// next scores but one wait for its product. The products are issued from a converged warp: by one lane of a
 // divergent one, each took its operands to uniform registers first, and the tensor core waited for the issue.
-// Now it is busy two thirds of the time; the rest is the chain scores - softmax - P within a block.
-template <int D, int DV, bool EXT>
+template <int D, int DV, bool EXT, bool QLO>
 __global__ void __launch_bounds__(FA_THREADS, 1)
 fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
           const __grid_constant__ CUtensorMap tmV, const FaArgs args) {
@@ -444,24 +445,28 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
         };
         int n_active = 0, slot = 0;                      // slot: the ring's next tile
         uint32_t turn = 0;
-        // the two tiles of K or V: A (TMEM) times their 16-row steps onto d
-        auto product = [&](uint32_t d, uint32_t a, bool v, uint32_t first, uint32_t done) {
+        // the two tiles of K or V: the high half takes A's high and (lo) low halves, the low one A's high ones
+        auto product = [&](uint32_t d, uint32_t a, bool v, bool lo, uint32_t first, uint32_t done) {
             for (int half = 0; half < 2; half++) {
                 if (!wait(full(slot), turn)) return false;
                 tc_fence_after();
                 const uint32_t tile = sb + C::OFF_K + slot * C::K_BYTES;
                 const uint64_t desc = v ? sdesc_mn_sw128(tile, FA_KB * 128) : sdesc_k_sw128(tile);
-                const uint32_t later = half == 0 ? first : 1u;
                 if (lead) {
-                    if (v) {
+                    for (int part = 0; part < (half == 0 && lo ? 2 : 1); part++) {
+                        const uint32_t later = half == 0 && part == 0 ? first : 1u;
+                        if (v) {
 #pragma unroll
-                        for (int ks = 0; ks < FA_KB / 16; ks++)
-                            mma_f16_ts(d, a + 8u * ks, desc + (uint64_t)(ks * 2048 / 16), C::IDESC_O, ks > 0 ? 1u : later);
-                    } else {
+                            for (int ks = 0; ks < FA_KB / 16; ks++)
+                                mma_f16_ts(d, a + C::P_LO * part + 8u * (ks & 3) + 64u * (ks >> 2),
+                                           desc + (uint64_t)(ks * 2048 / 16), C::IDESC_O, ks > 0 ? 1u : later);
+                        } else {
 #pragma unroll
-                        for (int ks = 0; ks < D / 16; ks++)
-                            mma_f16_ts(d, a + 8u * ks, desc + (uint64_t)(((ks >> 2) * (FA_KB * 128) + (ks & 3) * 32) / 16),
-                                       C::IDESC_S, ks > 0 ? 1u : later);
+                            for (int ks = 0; ks < D / 16; ks++)
+                                mma_f16_ts(d, a + C::Q_LO * part + 8u * ks,
+                                           desc + (uint64_t)(((ks >> 2) * (FA_KB * 128) + (ks & 3) * 32) / 16), C::IDESC_S,
+                                           ks > 0 ? 1u : later);
+                        }
                     }
                     mma_commit(empty(slot));
                     if (half == 1) mma_commit(done);
@@ -473,15 +478,16 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
         };
         auto issue_pv = [&](int i) {
             return wait(p_full(i & 1), (uint32_t)(i >> 1) & 1u) &&
-                   product(tmem + 256, tmem + C::P_TMEM0, true, i > 0 ? 1u : 0u, pv_done(i & 1));
+                   product(tmem + 256, tmem + (uint32_t)(i & 1) * FA_KB, true, true, i > 0 ? 1u : 0u, pv_done(i & 1));
         };
         bool ok = wait(q_full, 0);
         tc_fence_after();
         for (int j = j_first; j < j_end && ok; j++) {
             if (flags[j] == MF_MASKED) continue;
             const int i = n_active, s = i & 1;
-            ok = wait(s_empty(s), ((uint32_t)(i >> 1) & 1u) ^ 1u) &&
-                 product(tmem + (uint32_t)(s * FA_KB), tmem + C::Q_TMEM0, false, 0u, s_full(s));
+            // the buffer held P of block i - 2 last
+            ok = (i < 2 || wait(pv_done(s), ((uint32_t)(i >> 1) & 1u) ^ 1u)) &&
+                 product(tmem + (uint32_t)(s * FA_KB), tmem + C::Q_TMEM0, false, QLO, 0u, s_full(s));
             if (!ok) break;
             n_active++;
             if (i > 0) ok = issue_pv(i - 1);
@@ -602,14 +608,18 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
             return true;
         };
         if constexpr (EXT) {                             // Q's row, this thread's half of it, to TMEM
-            const uint4* src = reinterpret_cast<const uint4*>(args.q16 + (((int64_t)str * args.H + h) * args.T + (row_valid ? t : 0)) * D + pt * (D / 2));
-            uint32_t w[D / 4];
 #pragma unroll
-            for (int n = 0; n < D / 16; n++) {
-                const uint4 v = row_valid ? src[n] : make_uint4(0, 0, 0, 0);
-                w[4 * n] = v.x, w[4 * n + 1] = v.y, w[4 * n + 2] = v.z, w[4 * n + 3] = v.w;
+            for (int part = 0; part < (QLO ? 2 : 1); part++) {
+                const uint4* src = reinterpret_cast<const uint4*>(
+                    args.q16 + ((((int64_t)part * args.S + str) * args.H + h) * args.T + (row_valid ? t : 0)) * D + pt * (D / 2));
+                uint32_t w[D / 4];
+#pragma unroll
+                for (int n = 0; n < D / 16; n++) {
+                    const uint4 v = row_valid ? src[n] : make_uint4(0, 0, 0, 0);
+                    w[4 * n] = v.x, w[4 * n + 1] = v.y, w[4 * n + 2] = v.z, w[4 * n + 3] = v.w;
+                }
+                tmem_st_p<D / 4>(tmem + lane_base + C::Q_TMEM0 + C::Q_LO * part + (uint32_t)(pt * (D / 4)), w);
             }
-            tmem_st_p<D / 4>(tmem + lane_base + C::Q_TMEM0 + (uint32_t)(pt * (D / 4)), w);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -637,10 +647,12 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
 #pragma unroll
                 for (int e = 0; e < 32; e++) x[c0 + e] = __uint_as_float(rv[e]);
             }
-            // S is in registers: the buffer may take the next Q.K^T
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(s_empty(s));
+            if constexpr (!EXT) {
+                // S is in registers: the buffer may take the next Q.K^T
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_empty(s));
+            }
             const int k0 = j * FA_KB + pt * KPT;
             float bmax = -INFINITY;
             if (!general) {
@@ -700,31 +712,46 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
             l *= alpha;
             m = m_new;
             const float mu = (m == -INFINITY) ? 0.0f : m;
-            uint32_t pw[KPT / 2];
-            if (!general) {
+            if constexpr (EXT) {
+                uint32_t ph[KPT / 2], pl[KPT / 2];
 #pragma unroll
                 for (int e = 0; e < KPT; e += 2) {
-                    const float p0 = ex2_approx(fmaf(x[e], c2, -mu));
-                    const float p1 = ex2_approx(fmaf(x[e + 1], c2, -mu));
+                    const float p0 = ex2_approx(general ? x[e] - mu : fmaf(x[e], c2, -mu));
+                    const float p1 = ex2_approx(general ? x[e + 1] - mu : fmaf(x[e + 1], c2, -mu));
                     l += p0 + p1;
-                    pw[e >> 1] = pack_half2(p0, p1);
+                    ph[e >> 1] = pack_half2(p0, p1);
+                    const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&ph[e >> 1]));
+                    pl[e >> 1] = pack_half2(p0 - hi.x, p1 - hi.y);
                 }
+                const uint32_t p_at = tmem + lane_base + (uint32_t)(s * FA_KB + pt * KPT);
+                tmem_st_p<KPT / 2>(p_at, ph);
+                tmem_st_p<KPT / 2>(p_at + C::P_LO, pl);
             } else {
+                uint32_t pw[KPT / 2];
+                if (!general) {
 #pragma unroll
-                for (int e = 0; e < KPT; e += 2) {
-                    const float p0 = ex2_approx(x[e] - mu);
-                    const float p1 = ex2_approx(x[e + 1] - mu);
-                    l += p0 + p1;
-                    pw[e >> 1] = pack_half2(p0, p1);
+                    for (int e = 0; e < KPT; e += 2) {
+                        const float p0 = ex2_approx(fmaf(x[e], c2, -mu));
+                        const float p1 = ex2_approx(fmaf(x[e + 1], c2, -mu));
+                        l += p0 + p1;
+                        pw[e >> 1] = pack_half2(p0, p1);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < KPT; e += 2) {
+                        const float p0 = ex2_approx(x[e] - mu);
+                        const float p1 = ex2_approx(x[e + 1] - mu);
+                        l += p0 + p1;
+                        pw[e >> 1] = pack_half2(p0, p1);
+                    }
                 }
+                // P buffer (i & 1) is free once the P.V of block i-2 has completed
+                if (i >= 2) {
+                    if (!wait_pv(i - 2)) { ok = false; break; }
+                    tc_fence_after();
+                }
+                tmem_st_p<KPT / 2>(p_lane + (uint32_t)(64 * (i & 1)), pw);
             }
-            // P buffer (i & 1) is free once the P.V of block i-2 has completed (EXT: the one buffer, of block i-1)
-            constexpr int BACK = EXT ? 1 : 2;
-            if (i >= BACK) {
-                if (!wait_pv(i - BACK)) { ok = false; break; }
-                tc_fence_after();
-            }
-            tmem_st_p<KPT / 2>(p_lane + (uint32_t)(EXT ? 0 : 64 * (i & 1)), pw);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -896,7 +923,7 @@ static FaLayout fa_layout(int D, int T, int H, int KV, int HK) {
     return L;
 }
 
-template <int D, int DV, bool EXT = false>
+template <int D, int DV, bool EXT = false, bool QLO = false>
 static cudaError_t launch_fa(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const FaArgs& a,
                              dim3 grid, cudaStream_t st) {
     using C = FaCfg<D, DV, EXT>;
@@ -904,11 +931,11 @@ static cudaError_t launch_fa(const CUtensorMap& tq, const CUtensorMap& tk, const
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 0 && dev < 64 && !set[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(fa_kernel<D, DV, EXT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        cudaError_t e = cudaFuncSetAttribute(fa_kernel<D, DV, EXT, QLO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) return e;
         set[dev] = true;
     }
-    return launch_pdl(fa_kernel<D, DV, EXT>, grid, dim3(FA_THREADS), C::SMEM, st, tq, tk, tv, a);
+    return launch_pdl(fa_kernel<D, DV, EXT, QLO>, grid, dim3(FA_THREADS), C::SMEM, st, tq, tk, tv, a);
 }
 
 int flash_attn_impl(const float* q, int64_t q_nb1, int64_t q_nb2, const void* k, int64_t k_nb1, int64_t k_nb2,
@@ -976,8 +1003,8 @@ int flash_attn_impl(const float* q, int64_t q_nb1, int64_t q_nb2, const void* k,
 
 // ---- the kernels over several streams, from a Q4_0 cache brought to fp16 tiles (b200_flash_attn_kvq) ----
 
-// Set-up pass of one launch: CTAs [0, q_ctas) bring q to fp16 (one warp a row, a power-of-two divisor for
-// rows beyond fp16's range; not scaled, so that f16 values stay exact), the next m_ctas classify the mask,
+// Set-up pass of one launch: CTAs [0, q_ctas) bring q to fp16 (one warp a row; f32 rows as two halves, times a
+// power of two that brings them near 1; not scaled, so that f16 values stay exact), the next m_ctas classify the mask,
 // the rest bring the cache to pairs of fp16 tiles: four lanes a block of 32 values, each eight of them. Bound by
 // HBM and L2: 16384 keys, 8 KV heads of 128, 2048 tokens of 32 heads, 56 us for 19 MB of cache, 67 MB of mask
 // and 17 MB of q read and 151 MB written (4.5 TB/s); making the tiles costs the call once what every query tile would else pay.
@@ -985,7 +1012,7 @@ struct FaQuantPrep {
     const char* q;
     int64_t q_t, q_h, q_s;
     int q_f16;
-    __half* q16;
+    __half* q16;                 // [1, f32: 2 halves][S][H][T][D]
     float* qscale;               // per row: the scale times the divisor
     const uint16_t* mask;
     int64_t m_stride, m_stream;
@@ -1049,13 +1076,19 @@ __global__ void __launch_bounds__(256) fa_quant_prep_kernel(const FaQuantPrep a)
         for (int i = 0; i < PER; i++) amax = fmaxf(amax, fabsf(x[i]));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        // f32 rows are brought near 1 as well, so that small ones keep fp16's full precision
+        // f32 rows are brought near 1 as well, so that their halves keep fp16's full precision
         int e = 0;
         if (!a.q_f16 && amax > 0.0f && amax <= 3.402823466e38f) frexpf(amax, &e);
         e = max(-126, e);
 #pragma unroll
-        for (int i = 0; i < PER; i += 2)
-            *reinterpret_cast<uint32_t*>(a.q16 + row * D + lane * PER + i) = pack_half2(ldexpf(x[i], -e), ldexpf(x[i + 1], -e));
+        for (int i = 0; i < PER; i += 2) {
+            const float x0 = ldexpf(x[i], -e), x1 = ldexpf(x[i + 1], -e);
+            const uint32_t hi = pack_half2(x0, x1);
+            const float2 h2 = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+            uint32_t* dst = reinterpret_cast<uint32_t*>(a.q16 + row * D + lane * PER + i);
+            *dst = hi;
+            if (!a.q_f16) dst[(int64_t)a.S * a.H * a.T * D / 2] = pack_half2(x0 - h2.x, x1 - h2.y);
+        }
         if (lane == 0) a.qscale[row] = ldexpf(a.scale, e);   // the scale within: 2^128 alone would be no f32 number
         return;
     }
@@ -1141,7 +1174,7 @@ static FaQuantLayout fa_quant_layout(int64_t D, int64_t T, int64_t H, int64_t KV
     auto al = [](size_t x) { return (x + 255) & ~(size_t)255; };
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += al(n); return o; };
-    Q.q16_off = take((size_t)(S * H * T * D) * 2);
+    Q.q16_off = take((size_t)(S * H * T * D) * 4);
     Q.qs_off = take((size_t)(S * H * T) * 4);
     Q.flags_off = take((size_t)S * Q.L.n_tb * Q.L.n_kvb);
     Q.k_off = take((size_t)(S * HK * KV * D) * 4);
@@ -1206,7 +1239,8 @@ cudaError_t fa_quant_run(const FaQuantArgs& q, char* ws, cudaStream_t st) {
     a.err = q.err;
     const dim3 fgrid((unsigned)(Q.units.whole + Q.cut_tiles * Q.units.cut));
     // no map of Q, whose rows the softmax threads bring to TMEM: K's stands in its place, unused
-    e = q.D == 64 ? launch_fa<64, 64, true>(tk, tk, tv, a, fgrid, st) : launch_fa<128, 128, true>(tk, tk, tv, a, fgrid, st);
+    if (q.q_f16) e = q.D == 64 ? launch_fa<64, 64, true, false>(tk, tk, tv, a, fgrid, st) : launch_fa<128, 128, true, false>(tk, tk, tv, a, fgrid, st);
+    else e = q.D == 64 ? launch_fa<64, 64, true, true>(tk, tk, tv, a, fgrid, st) : launch_fa<128, 128, true, true>(tk, tk, tv, a, fgrid, st);
     if (e != cudaSuccess || Q.cut_tiles == 0) return e;
     const int rows = Q.cut_tiles * FA_ROWS;
     auto join = [&](auto kernel, int warps) {

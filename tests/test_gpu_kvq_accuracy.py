@@ -52,3 +52,23 @@ def test_queries_at_the_end_of_f32(cuda, T):
     q, k, v = inputs(1, T, 8, 2, 128, 300)
     for qq, scale in ((q.sign() * 3e38, 1e-39), (q / q.abs().max() * 3.4e38, 2e-39), (q * 1e-38, 1e37)):
         loose(run(qq, k, v, None, scale), qq, k, v, None, scale)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("q_f16", [False, True])
+@pytest.mark.parametrize("S,T,H,HK,D,KV", [
+    (1, 100, 4, 1, 128, 5),
+    (2, 60, 4, 2, 64, 9),
+    (1, 64, 8, 2, 128, 129),
+    (1, 200, 32, 8, 128, 1000),
+    (2, 130, 14, 2, 64, 700),        # a head a tile
+    (3, 17, 8, 2, 128, 2000),        # the keys of a tile over several CTAs
+    (1, 700, 64, 8, 128, 900),       # whole tiles, then cut ones
+    (1, 512, 8, 2, 128, 4096),
+])
+def test_prompts_keep_what_the_row_kernels_keep(cuda, S, T, H, HK, D, KV, q_f16, f16):
+    q, k, v = inputs(S, T, H, HK, D, KV, seed=3, q_f16=q_f16)
+    m = causal(S, T, KV) if T <= KV else None
+    for scale in (1 / 128, 1 / math.sqrt(D)):
+        check(run(q, k, v, m, scale, f16), q, k, v, m, scale)
+    check(run(q, k, v, None, -0.02, f16), q, k, v, None, -0.02)
