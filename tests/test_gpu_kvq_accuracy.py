@@ -72,3 +72,12 @@ def test_prompts_keep_what_the_row_kernels_keep(cuda, S, T, H, HK, D, KV, q_f16,
     for scale in (1 / 128, 1 / math.sqrt(D)):
         check(run(q, k, v, m, scale, f16), q, k, v, m, scale)
     check(run(q, k, v, None, -0.02, f16), q, k, v, None, -0.02)
+
+
+@pytest.mark.parametrize("T", [1, 70])
+@pytest.mark.parametrize("cap", [1e5, 1000.0, 30.0, 2.0])
+def test_softcap(cuda, T, cap):
+    """tanhf is within 2^-22 of its value, the cap far above the scores too."""
+    q, k, v = inputs(2, T, 8, 2, 128, 20, seed=4)
+    for scale in (1 / 128, 0.3):
+        check(run(q, k, v, None, scale, softcap=cap), q, k, v, None, scale, softcap=cap)
