@@ -62,7 +62,7 @@ struct FaArgs {
     FaUnits units;
     int dst_f16;
     float* part;               // [unit - whole][rows of a unit][DV] outputs not divided by their sums
-    float* stat;               // {max in log2 units, sum} of each of their rows
+    float* stat;               // {max in log2 units, sum, mask value it is relative to} of each of their rows
 };
 
 // True in one lane of a converged warp.
@@ -261,7 +261,8 @@ struct FaCfg {
     static constexpr int XCH_MAX = 2 * FA_SPLIT * 128 * 4;
     static constexpr int XCH_SUM = FA_SPLIT * 128 * 4;
     static constexpr int OFF_XCH = EXT ? OFF_K + RING * K_BYTES : OFF_V + 2 * V_BYTES;
-    static constexpr int OFF_BAR = OFF_XCH + 2 * XCH_MAX + 2 * XCH_SUM;
+    static constexpr int OFF_REF = OFF_XCH + 2 * XCH_MAX + 2 * XCH_SUM;   // EXT: mask references, like the maxima
+    static constexpr int OFF_BAR = OFF_REF + (EXT ? XCH_MAX : 0);
     static constexpr int SMEM = OFF_BAR + 256 + 1024;
     // TMEM columns: S0 [0,128) | S1 [128,256) | O [256, 256+DV) | P0 [384,448) | P1 [448,512)
     // (P is fp16, two keys per 32-bit column, read by the P.V MMA as its A operand)
@@ -636,6 +637,8 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
             if (lane == 0) mbar_arrive(q_full);
         }
         float m = -INFINITY;                             // running max (log2 units)
+        float mref = 0.0f;                               // EXT: of a score less this mask value
+        volatile float* xr = reinterpret_cast<volatile float*>(smem + C::OFF_REF);
         float l = 0.0f;                                  // this thread's partial row sum
         int i = 0;
         bool ok = true;
@@ -665,6 +668,23 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
             }
             const int k0 = j * FA_KB + pt * KPT;
             float bmax = -INFINITY;
+            float ref = 0.0f;                            // EXT: the largest mask value of this thread's keys
+            if (EXT && use_mask) {
+                ref = -INFINITY;
+#pragma unroll
+                for (int c0 = 0; c0 < KPT; c0 += 32) {
+                    uint4 mv[4];
+                    load_mask32(mrow, k0 + c0, args.KV, args.mask_vec, mv);
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const uint32_t w = (&mv[e >> 2].x)[e & 3];
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+                        if (k0 + c0 + 2 * e < args.KV) ref = fmaxf(ref, f.x);
+                        if (k0 + c0 + 2 * e + 1 < args.KV) ref = fmaxf(ref, f.y);
+                    }
+                }
+                ref = fabsf(ref) <= 65504.0f ? ref : 0.0f;   // all masked (or an infinite mask): nothing to gain
+            }
             if (!general) {
 #pragma unroll
                 for (int e = 0; e < KPT; e++) bmax = fmaxf(bmax, x[e]);
@@ -682,7 +702,7 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
                         if (use_mask) {
                             const uint32_t mw = (&mv[e >> 3].x)[(e & 7) >> 1];
                             const uint16_t mb = (uint16_t)((e & 1) ? (mw >> 16) : (mw & 0xFFFFu));
-                            sv = fmaf(__half2float(__ushort_as_half(mb)), LOG2E, sv);
+                            sv = fmaf(__half2float(__ushort_as_half(mb)) - ref, LOG2E, sv);
                             if (EXT && mb == 0xFC00u) sv = -INFINITY;
                         }
                         if (k0 + c0 + e >= args.KV) sv = -INFINITY;
@@ -693,15 +713,37 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
             }
             // the row max over all parts (double-buffered by block parity)
             float maxes[FA_SPLIT];
+            if (EXT && use_mask) xr[(i & 1) * (FA_SPLIT * 128) + pt * 128 + r] = ref;   // published with the maximum
             if (!together(exchange(xv + (i & 1) * (FA_SPLIT * 128), xs + (i & 1) * (FA_SPLIT * 128), bmax, i + 1, maxes))) {
                 ok = false;
                 break;
             }
+            float m_new, alpha, mu;
+            if constexpr (EXT) {
+                // The row's maximum as a pair (value, mask reference). Pairs are compared, and scores taken against
+                // the running one, through differences, which are exact for mask values also where a score plus its
+                // mask is not (fp16's lowest value on every key).
+                float b_ref = 0.0f;
+                bmax = maxes[0];
+                if (use_mask) b_ref = xr[(i & 1) * (FA_SPLIT * 128) + r];
 #pragma unroll
-            for (int k = 0; k < FA_SPLIT; k++) bmax = fmaxf(bmax, maxes[k]);
-            const bool grow = bmax > m + FA_RESCALE_LOG2;
-            const float m_new = grow ? bmax : m;
-            const float alpha = (grow && m != -INFINITY) ? ex2_approx(m - m_new) : 1.0f;
+                for (int k = 1; k < FA_SPLIT; k++) {
+                    const float k_ref = use_mask ? xr[(i & 1) * (FA_SPLIT * 128) + k * 128 + r] : 0.0f;
+                    if ((maxes[k] - bmax) + (k_ref - b_ref) * LOG2E > 0.0f) bmax = maxes[k], b_ref = k_ref;
+                }
+                const bool grow = (bmax - m) + (b_ref - mref) * LOG2E > FA_RESCALE_LOG2;
+                m_new = grow ? bmax : m;
+                alpha = (grow && m != -INFINITY) ? ex2_approx((m - m_new) + (mref - b_ref) * LOG2E) : 1.0f;
+                mref = grow ? b_ref : mref;
+                mu = (m_new == -INFINITY) ? 0.0f : m_new - (ref - mref) * LOG2E;
+            } else {
+#pragma unroll
+                for (int k = 0; k < FA_SPLIT; k++) bmax = fmaxf(bmax, maxes[k]);
+                const bool grow = bmax > m + FA_RESCALE_LOG2;
+                m_new = grow ? bmax : m;
+                alpha = (grow && m != -INFINITY) ? ex2_approx(m - m_new) : 1.0f;
+                mu = (m_new == -INFINITY) ? 0.0f : m_new;
+            }
             // O is rescaled in place only after the previous block's P.V has landed in it
             if (i > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
                 if (!wait_pv(i - 1)) { ok = false; break; }
@@ -721,7 +763,6 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
             }
             l *= alpha;
             m = m_new;
-            const float mu = (m == -INFINITY) ? 0.0f : m;
             if constexpr (EXT) {
                 uint32_t ph[KPT / 2], pl[KPT / 2];
 #pragma unroll
@@ -785,8 +826,9 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
                 const int64_t at = whole ? ((int64_t)str * args.T + t) * args.H + h : (int64_t)un.slot * FA_ROWS + r;
                 const float inv = whole ? 1.0f / l_tot : 1.0f;
                 if (!whole && pt == 0) {
-                    args.stat[2 * at] = m;
-                    args.stat[2 * at + 1] = l_tot;
+                    args.stat[3 * at] = m;
+                    args.stat[3 * at + 1] = l_tot;
+                    args.stat[3 * at + 2] = mref;
                 }
 #pragma unroll
                 for (int c0 = 0; c0 < OPT; c0 += 16) {
@@ -861,19 +903,26 @@ __global__ void __launch_bounds__(256) fa_join_kernel(const FaArgs args, int n_r
     constexpr int PER = D / 32;
     float acc[PER] = {}, l_all = 0.0f;
     if (in) {
-        float top = -INFINITY;
+        // maxima are compared as maximum plus mask reference; their differences are formed apart, where they are exact
+        constexpr float LOG2E = 1.4426950408889634f;
+        float top = -INFINITY, m_best = 0.0f, r_best = 0.0f;
         for (int k = lane; k < cut; k += 32) {
-            const float* st = args.stat + 2 * (first + (int64_t)k * FA_ROWS);
-            if (st[1] != 0.0f) top = fmaxf(top, st[0]);
+            const float* st = args.stat + 3 * (first + (int64_t)k * FA_ROWS);
+            const float v = st[0] + st[2] * LOG2E;
+            if (st[1] != 0.0f && v > top) top = v, m_best = st[0], r_best = st[2];
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (top == -INFINITY) top = 0.0f;
+        for (int o = 16; o > 0; o >>= 1) {
+            const float v = __shfl_xor_sync(0xffffffffu, top, o), mo = __shfl_xor_sync(0xffffffffu, m_best, o);
+            const float ro = __shfl_xor_sync(0xffffffffu, r_best, o);
+            if (v > top || (v == top && mo > m_best)) top = v, m_best = mo, r_best = ro;   // the same pair on every lane
+        }
 #pragma unroll 4
         for (int k = w; k < cut; k += W) {
             const int64_t at = first + (int64_t)k * FA_ROWS;
-            const float l = args.stat[2 * at + 1];
-            const float f = l == 0.0f ? 0.0f : ex2_approx(args.stat[2 * at] - top);   // l is 0 where no key is seen
+            const float l = args.stat[3 * at + 1];
+            // l is 0 where no key is seen
+            const float f = l == 0.0f ? 0.0f : ex2_approx((args.stat[3 * at] - m_best) + (args.stat[3 * at + 2] - r_best) * LOG2E);
             l_all = fmaf(l, f, l_all);
             const float* p = args.part + at * D + lane * PER;
 #pragma unroll
@@ -1190,7 +1239,7 @@ static FaQuantLayout fa_quant_layout(int64_t D, int64_t T, int64_t H, int64_t KV
     Q.k_off = take((size_t)(S * HK * KV * D) * 4);
     Q.v_off = take((size_t)(S * HK * KV * D) * 4);
     Q.part_off = take((size_t)(rows * D) * 4);
-    Q.stat_off = take((size_t)rows * 8);
+    Q.stat_off = take((size_t)rows * 12);
     Q.total = at;
     return Q;
 }

@@ -182,8 +182,8 @@ int    b200_kv_to_f16(int type, const void * src, int64_t D, int64_t KV, int64_t
  * largest value of a key's head), an F16 dst adds its own rounding alone. With at most 48 query rows a KV head
  * (T * H / HK), and with more where that is faster, the cache's codes enter the products as they are. Otherwise
  * the cache is brought to pairs of fp16 tiles in the workspace once, which hold its values exactly; there a key
- * with a block scale above 8188 (whose values may leave fp16's range) is no number to rows that see it, and a
- * score is rounded to fp32 after its mask value is added. The workspace (256-byte aligned,
+ * with a block scale above 8188 (whose values may leave fp16's range) is no number to rows that see it. The
+ * workspace (256-byte aligned,
  * b200_flash_attn_kvq_workspace_size bytes; the calling device's) holds that and the parts of rows whose
  * keys several CTAs share; calls sharing one must not overlap on the GPU.
  * No ALiBi, no sinks. */

@@ -81,3 +81,18 @@ def test_softcap(cuda, T, cap):
     q, k, v = inputs(2, T, 8, 2, 128, 20, seed=4)
     for scale in (1 / 128, 0.3):
         check(run(q, k, v, None, scale, softcap=cap), q, k, v, None, scale, softcap=cap)
+
+
+@pytest.mark.parametrize("T,KV", [(1, 700), (70, 700), (40, 9000)])
+def test_masks_far_from_zero(cuda, T, KV):
+    """Mask values whose sum with a score is no f32 number: a row's weights are those of the differences."""
+    import torch
+    q, k, v = inputs(1, T, 8, 2, 128, KV, seed=6)
+    m = torch.full((1, T, KV), -65504.0, dtype=torch.float16, device="cuda")
+    check(run(q, k, v, m, 0.05), q, k, v, m, 0.05)
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    m[:, :, ::3] = float("-inf")
+    m[:, 1::4, 100:300] = -65472.0                       # 32 above the lowest
+    m[:, 2::4] = -30000 - 16 * torch.randint(0, 3, (KV,), device="cuda", generator=gen).half()
+    m[:, 3::4, 400:] = 0
+    check(run(q, k, v, m, 0.05), q, k, v, m, 0.05)
