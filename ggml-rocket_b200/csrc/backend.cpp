@@ -141,8 +141,7 @@ int flash_attn_min_kv() {
 }
 // FLASH_ATTN_EXT over a quantized KV cache. Q4_0 K and V in device memory: read as they are stored, any
 // number of tokens and streams (b200_flash_attn_kvq). Otherwise Q8_0 / Q4_0 K or V converted to fp16
-// tiles, then the fp16 kernel (b200_kv_to_f16). Off by default: the reference declines these (F16 K / V
-// only).
+// tiles, then the fp16 kernel (b200_kv_to_f16). Off by default: the reference declines these (F16 K / V only).
 bool fa_quant_kv_on() {
     static const bool v = knob_on("B200_FA_QUANT_KV", false);
     return v;
@@ -1079,6 +1078,34 @@ static bool fa_kvq(const b200_tensor* op) {
                    (m->ne[3] == S || m->ne[3] == 1)));
 }
 
+// FLASH_ATTN_EXT by the fp16 kernel, a quantised cache converted to fp16 tiles first: one stream, above the floors.
+static bool fa_fp16(const b200_tensor* op) {
+    const b200_tensor* q = op->src[0];
+    const b200_tensor* k = op->src[1];
+    const b200_tensor* v = op->src[2];
+    const b200_tensor* m = op->src[3];
+    const float max_bias = op_param_f32(op, 1);
+    const int64_t D = q->ne[0], T = q->ne[1], H = q->ne[2], DV = v->ne[0];
+    const int64_t KV = k->ne[1], HK = k->ne[2];
+    auto aligned16 = [](const b200_tensor* t) {
+        return (t->nb[1] % 16 == 0) && (t->nb[2] % 16 == 0) && (t->on_device ? ((uintptr_t)t->data % 16 == 0) : true);
+    };
+    // a quantized cache: 32-value blocks along the head dimension, read as bytes, so no
+    // 16-byte alignment is needed of its view
+    auto kv_ok = [&](const b200_tensor* t) {
+        if (t->type == T_F16) return t->nb[0] == 2 && aligned16(t);
+        return fa_quant_kv_on() && (t->type == T_Q8_0 || t->type == T_Q4_0) && t->ne[0] % 32 == 0 &&
+               t->nb[0] == (size_t)(t->type == T_Q8_0 ? 34 : 18) && (t->on_device || is_contiguous(t));
+    };
+    return max_bias == 0.0f && q->type == T_F32 && kv_ok(k) && kv_ok(v) &&
+           (!m || (m->type == T_F16 && is_contiguous(m))) && op->type == T_F32 && is_contiguous(op) &&
+           q->ne[3] == 1 && k->ne[3] == 1 && v->ne[3] == 1 && k->ne[0] == D && op->ne[0] == DV &&
+           v->ne[1] == KV && v->ne[2] == HK && q->nb[0] == 4 &&
+           (D == 64 || D == 128) && (DV == 64 || DV == 128) && HK > 0 && H % HK == 0 &&
+           (!m || (m->ne[0] >= KV && m->ne[1] >= T)) &&
+           T >= flash_attn_min_t() && KV >= flash_attn_min_kv();
+}
+
 extern "C" bool ggml_backend_b200_supports_op(const b200_tensor* op) {
     if (!op) return false;
     if (!sources_readable(op)) return false;
@@ -1155,26 +1182,7 @@ extern "C" bool ggml_backend_b200_supports_op(const b200_tensor* op) {
             if (!m && !flash_attn_unmasked()) return false;
             if (op->src[4]) return false;   // attention sinks: a different softmax (ggml-rocket.cpp:7703-7721)
             if (fa_kvq(op)) return true;
-            const float max_bias = op_param_f32(op, 1);
-            const int64_t D = q->ne[0], T = q->ne[1], H = q->ne[2], DV = v->ne[0];
-            const int64_t KV = k->ne[1], HK = k->ne[2];
-            auto aligned16 = [](const b200_tensor* t) {
-                return (t->nb[1] % 16 == 0) && (t->nb[2] % 16 == 0) && (t->on_device ? ((uintptr_t)t->data % 16 == 0) : true);
-            };
-            // a quantized cache: 32-value blocks along the head dimension, read as bytes, so no
-            // 16-byte alignment is needed of its view
-            auto kv_ok = [&](const b200_tensor* t) {
-                if (t->type == T_F16) return t->nb[0] == 2 && aligned16(t);
-                return fa_quant_kv_on() && (t->type == T_Q8_0 || t->type == T_Q4_0) && t->ne[0] % 32 == 0 &&
-                       t->nb[0] == (size_t)(t->type == T_Q8_0 ? 34 : 18) && (t->on_device || is_contiguous(t));
-            };
-            return max_bias == 0.0f && q->type == T_F32 && kv_ok(k) && kv_ok(v) &&
-                   (!m || (m->type == T_F16 && is_contiguous(m))) && op->type == T_F32 && is_contiguous(op) &&
-                   q->ne[3] == 1 && k->ne[3] == 1 && v->ne[3] == 1 && k->ne[0] == D && op->ne[0] == DV &&
-                   v->ne[1] == KV && v->ne[2] == HK && q->nb[0] == 4 &&
-                   (D == 64 || D == 128) && (DV == 64 || DV == 128) && HK > 0 && H % HK == 0 &&
-                   (!m || (m->ne[0] >= KV && m->ne[1] >= T)) &&
-                   T >= flash_attn_min_t() && KV >= flash_attn_min_kv();
+            return fa_fp16(op);
         }
         case B200_OP_RMS_NORM:
         case B200_OP_ADD:
@@ -1656,7 +1664,11 @@ int do_rope_cpy(b200_backend* b, const b200_tensor* r, const b200_tensor* c) {
     return B200_OK;
 }
 
-int do_flash_attn_kvq(b200_backend* b, b200_tensor* op) {
+// Over a Q4_0 cache as it is stored. Long prompts bring it to fp16 tiles, 7 times its size: as many streams at a
+// time as FA_KVQ_WS holds, one at least; fewer where the device has no room. *room: false where it has none for one.
+constexpr size_t FA_KVQ_WS = (size_t)2 << 30;
+
+int do_flash_attn_kvq(b200_backend* b, b200_tensor* op, bool* room) {
     const b200_tensor* q = op->src[0];
     const b200_tensor* k = op->src[1];
     const b200_tensor* v = op->src[2];
@@ -1664,21 +1676,37 @@ int do_flash_attn_kvq(b200_backend* b, b200_tensor* op) {
     OpStaging stg;
     stg.ins = {q, k, v, m};
     stg.outs = {op};
-    const size_t need = b200_flash_attn_kvq_workspace_size(q->ne[0], q->ne[1], q->ne[2], k->ne[1], k->ne[2], q->ne[3]);
+    const int64_t S = q->ne[3];
+    auto size = [&](int64_t n) { return b200_flash_attn_kvq_workspace_size(q->ne[0], q->ne[1], q->ne[2], k->ne[1], k->ne[2], n); };
+    auto need = [&](int64_t n) { return std::max(size(n), S % n ? size(S % n) : 0); };   // the last ones may be fewer
+    int64_t per = S;
+    while (per > 1 && need(per) > FA_KVQ_WS) per = (per + 1) / 2;
+    while (!grow(&b->ws, &b->ws_bytes, need(per), b->stream)) {
+        cudaGetLastError();
+        if (per == 1) {
+            *room = false;
+            return B200_E_CUDA;
+        }
+        per = (per + 1) / 2;
+    }
     if (!op_reserve(b, stg)) return B200_E_CUDA;
-    if (!grow(&b->ws, &b->ws_bytes, need, b->stream)) return B200_E_CUDA;
     bool ok = true;
-    const void* qd = stage_in(b, q, &ok);
-    const void* kd = stage_in(b, k, &ok);
-    const void* vd = stage_in(b, v, &ok);
-    const void* md = m ? stage_in(b, m, &ok) : nullptr;
+    const char* qd = static_cast<const char*>(stage_in(b, q, &ok));
+    const char* kd = static_cast<const char*>(stage_in(b, k, &ok));
+    const char* vd = static_cast<const char*>(stage_in(b, v, &ok));
+    const char* md = m ? static_cast<const char*>(stage_in(b, m, &ok)) : nullptr;
     char* dd = stage_out(b, op, false, &ok);
     if (!ok || !op_inputs_ready(b)) return B200_E_CUDA;
     const size_t mnb[4] = {2, m ? m->nb[1] : 0, 0, m && m->ne[3] > 1 ? m->nb[3] : 0};
-    const int rc = b200_flash_attn_kvq(k->type, q->type, qd, q->ne, q->nb, kd, k->ne, k->nb, vd, v->ne, v->nb, md, mnb,
-                                       op->type, dd, op_param_f32(op, 0), op_param_f32(op, 2), b->ws, b->ws_bytes, b->dev_err,
-                                       b->stream);
-    if (rc != B200_OK) return rc;
+    for (int64_t s = 0; s < S; s += per) {
+        const int64_t n = std::min(per, S - s);
+        const int64_t qne[4] = {q->ne[0], q->ne[1], q->ne[2], n}, kne[4] = {k->ne[0], k->ne[1], k->ne[2], n};
+        const int rc = b200_flash_attn_kvq(k->type, q->type, qd + s * q->nb[3], qne, q->nb, kd + s * k->nb[3], kne, k->nb,
+                                           vd + s * v->nb[3], kne, v->nb, md ? md + s * mnb[3] : nullptr, mnb, op->type,
+                                           dd + s * op->nb[3], op_param_f32(op, 0), op_param_f32(op, 2), b->ws, b->ws_bytes,
+                                           b->dev_err, b->stream);
+        if (rc != B200_OK) return rc;
+    }
     if (!op_outputs_done(b, stg.outs, {dd})) return B200_E_CUDA;
     b->route_ops["fa"]++;
     b->route_ops["fa_kvq"]++;
@@ -1686,7 +1714,11 @@ int do_flash_attn_kvq(b200_backend* b, b200_tensor* op) {
 }
 
 int do_flash_attn(b200_backend* b, b200_tensor* op) {
-    if (fa_kvq(op)) return do_flash_attn_kvq(b, op);
+    if (fa_kvq(op)) {
+        bool room = true;
+        const int rc = do_flash_attn_kvq(b, op, &room);
+        if (room || !fa_fp16(op)) return rc;      // no room for its tiles: the fp16 kernel's take half of it
+    }
     const b200_tensor* q = op->src[0];
     const b200_tensor* k = op->src[1];
     const b200_tensor* v = op->src[2];

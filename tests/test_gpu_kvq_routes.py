@@ -1,0 +1,82 @@
+"""Which kernel graph_compute gives FLASH_ATTN_EXT over a Q4_0 cache in device memory, and what it holds meanwhile.
+
+Long prompts of one stream run, as over a Q8_0 cache, on the fp16 kernel over tiles made by b200_kv_to_f16, bit for
+bit; shorter ones on b200_flash_attn_kvq, and so do several streams, a few at a time where their tiles are large."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+from conftest import ROOT
+
+pytestmark = pytest.mark.gpu
+
+_CHILD = r"""
+import sys
+sys.path[:0] = [sys.argv[1], sys.argv[1] + "/ggml-rocket_b200", sys.argv[1] + "/tests"]
+import math
+import torch
+import ggml_b200 as g
+from test_gpu_flash_attn_kvq import causal, inputs, run
+
+be = g.Backend()
+def node(q, k, v, m, out, scale):
+    S, T, H, D = q.shape
+    KV, HK = k.shape[1:3]
+    row = HK * D // 32 * 18
+    tq = g.make_tensor(g.F32, [D, T, H, S], q.data_ptr(), nb=[4, 4 * H * D, 4 * D, 4 * T * H * D], on_device=True)
+    tk, tv = [g.make_tensor(g.Q4_0, [D, KV, HK, S], c.data_ptr(), nb=[18, row, D // 32 * 18, row * KV], on_device=True) for c in (k, v)]
+    tm = g.make_tensor(g.F16, [KV, T, 1, S], m.data_ptr(), on_device=True)
+    return g.make_tensor(g.F32, [D, H, T, S], out.data_ptr(), op=g.OP_FLASH_ATTN_EXT, srcs=[tq, tk, tv, tm],
+                         op_params=[scale, 0.0, 0.0, 10], on_device=True)
+def routes():
+    return [be.route_ops(r) for r in ("fa", "fa_kvq", "fa_quant_kv")]
+def graph(q, k, v, m, scale=0.09):
+    out = torch.full(q.shape, 3.0, device="cuda")
+    n = node(q, k, v, m, out, scale)
+    assert g.supports_op(n)
+    torch.cuda.synchronize()
+    before = routes()
+    assert be.graph_compute([n]) == g.STATUS_SUCCESS
+    torch.cuda.synchronize()
+    return out, [b - a for a, b in zip(before, routes())]
+def fp16(q, k, v, m, scale=0.09):
+    S, T, H, D = q.shape
+    KV, HK = k.shape[1:3]
+    t16 = torch.empty(2, HK, KV, D, dtype=torch.float16, device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    for i, c in enumerate((k, v)):
+        assert g.lib().b200_kv_to_f16(2, c.data_ptr(), D, KV, HK, HK * D // 32 * 18, D // 32 * 18, t16[i].data_ptr(), st) == 0
+    out, err = torch.empty_like(q), torch.zeros(1, dtype=torch.int32, device="cuda")
+    ws = torch.empty(g.flash_attn_workspace_size(D, D, T, H, KV, HK), dtype=torch.uint8, device="cuda")
+    g.flash_attn_ext(q, 4 * H * D, 4 * D, t16[0], 2 * D, 2 * KV * D, t16[1], 2 * D, 2 * KV * D, m, 2 * KV, out, D, D, T, H, KV,
+                     HK, scale, 0.0, ws, err)
+    torch.cuda.synchronize()
+    return out
+
+if True:
+    # sixteen streams whose tiles would take 4.4 GB
+    S, T, H, HK, D, KV = 16, 13, 32, 8, 128, 32768
+    q, k, v = inputs(S, T, H, HK, D, KV)
+    m = causal(S, T, KV, [KV - 1000 * s for s in range(S)])
+    torch.cuda.empty_cache()
+    free = torch.cuda.mem_get_info()[0]
+    out, by = graph(q, k, v, m)
+    held = free - torch.cuda.mem_get_info()[0]
+    assert by == [1, 1, 0] and held < (3 << 30), (by, held)
+    for s in (0, 7, 8, 15):
+        one = run(q[s:s + 1], k[s:s + 1], v[s:s + 1], m[s:s + 1], 0.09)
+        assert float((one - out[s:s + 1]).abs().max()) < 2e-5 * 4
+be.close()
+print("DONE")
+"""
+
+
+@pytest.mark.parametrize("what", ["memory"])
+def test_routes_and_memory(cuda, what):
+    env = {k: v for k, v in os.environ.items() if not k.startswith("B200_")}
+    env.update(B200_FA_QUANT_KV="1")
+    p = subprocess.run([sys.executable, "-c", _CHILD, ROOT, what], env=env, capture_output=True, text=True, timeout=600)
+    assert p.returncode == 0, p.stdout[-3000:] + p.stderr[-3000:]
+    assert "DONE" in p.stdout
