@@ -140,8 +140,9 @@ int flash_attn_min_kv() {
     return kv;
 }
 // FLASH_ATTN_EXT over a quantized KV cache. Q4_0 K and V in device memory: read as they are stored, any
-// number of tokens and streams (b200_flash_attn_kvq). Otherwise Q8_0 / Q4_0 K or V converted to fp16
-// tiles, then the fp16 kernel (b200_kv_to_f16). Off by default: the reference declines these (F16 K / V only).
+// number of tokens and streams (b200_flash_attn_kvq), but for long prompts of one stream (fa_fp16_faster).
+// Those, and Q8_0 / Q4_0 K or V otherwise, are converted to fp16 tiles, then the fp16 kernel
+// (b200_kv_to_f16). Off by default: the reference declines these (F16 K / V only).
 bool fa_quant_kv_on() {
     static const bool v = knob_on("B200_FA_QUANT_KV", false);
     return v;
@@ -1106,6 +1107,19 @@ static bool fa_fp16(const b200_tensor* op) {
            T >= flash_attn_min_t() && KV >= flash_attn_min_kv();
 }
 
+// Of the calls both routes take, those the fp16 one is faster at: with more query tiles (128 rows) than half the
+// SMs it does half the products or fewer and the other has no tiles left to cut (32 heads over 8, 128 values,
+// 512 tokens x 16384 keys: 226 against 314 us, 2048 tokens 727 against 1069; 256 tokens 221 against 187, 16
+// tokens 211 against 69); with few keys there is nothing to cut either (512 tokens x 1024 keys 33 against 40, 64
+// tokens 26 against 33; 14 heads over 2 of 64 and 64 tokens 26 against 24).
+static bool fa_fp16_faster(const b200_tensor* op) {
+    const int64_t T = op->src[0]->ne[1], H = op->src[0]->ne[2], G = H / op->src[1]->ne[2];
+    int64_t heads = 1;                            // of a tile
+    while (heads < 16 && G % (2 * heads) == 0) heads *= 2;
+    const int64_t tiles = H / heads * ((T * heads + 127) / 128);
+    return tiles > 74 || (tiles >= 8 && op->src[1]->ne[1] <= 1024);
+}
+
 extern "C" bool ggml_backend_b200_supports_op(const b200_tensor* op) {
     if (!op) return false;
     if (!sources_readable(op)) return false;
@@ -1714,7 +1728,7 @@ int do_flash_attn_kvq(b200_backend* b, b200_tensor* op, bool* room) {
 }
 
 int do_flash_attn(b200_backend* b, b200_tensor* op) {
-    if (fa_kvq(op)) {
+    if (fa_kvq(op) && !(fa_fp16(op) && fa_fp16_faster(op))) {
         bool room = true;
         const int rc = do_flash_attn_kvq(b, op, &room);
         if (room || !fa_fp16(op)) return rc;      // no room for its tiles: the fp16 kernel's take half of it

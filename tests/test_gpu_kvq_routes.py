@@ -55,7 +55,21 @@ def fp16(q, k, v, m, scale=0.09):
     torch.cuda.synchronize()
     return out
 
-if True:
+if sys.argv[2] == "routes":
+    for T, H, HK, D, KV in ((512, 32, 8, 128, 2048), (300, 32, 8, 128, 1024), (64, 32, 8, 128, 1000 + 24), (2048, 14, 2, 64, 2048)):
+        q, k, v = inputs(1, T, H, HK, D, KV)
+        m = causal(1, T, KV)
+        out, by = graph(q, k, v, m)
+        assert by == [1, 0, 1], (T, H, KV, by)
+        assert torch.equal(out, fp16(q, k, v, m))
+    for S, T, H, HK, D, KV in ((1, 1, 32, 8, 128, 300), (1, 40, 8, 2, 128, 1024), (1, 64, 32, 8, 128, 4096), (2, 600, 32, 8, 64, 1100),
+                               (1, 512, 32, 8, 128, 1023)):
+        q, k, v = inputs(S, T, H, HK, D, KV)
+        m = causal(S, T, KV)
+        out, by = graph(q, k, v, m)
+        assert by == [1, 1, 0], (S, T, H, KV, by)
+        assert torch.equal(out, run(q, k, v, m, 0.09))
+else:
     # sixteen streams whose tiles would take 4.4 GB
     S, T, H, HK, D, KV = 16, 13, 32, 8, 128, 32768
     q, k, v = inputs(S, T, H, HK, D, KV)
@@ -73,7 +87,7 @@ print("DONE")
 """
 
 
-@pytest.mark.parametrize("what", ["memory"])
+@pytest.mark.parametrize("what", ["routes", "memory"])
 def test_routes_and_memory(cuda, what):
     env = {k: v for k, v in os.environ.items() if not k.startswith("B200_")}
     env.update(B200_FA_QUANT_KV="1")
