@@ -35,6 +35,7 @@
 
 #include "ggml-b200-kernels.h"
 #include "ggml-b200.h"
+#include "internal.h"
 
 namespace {
 
@@ -1027,8 +1028,7 @@ static bool glue_supported(const b200_tensor* op) {
             // op: the cache tensor itself (its rows that no index names stay as they are, so it has to lie
             // in device memory); a: the new rows; b: their indices
             const size_t unit = op->type == T_F32 ? 4 : 2;
-            for (int i = 1; i < 4; i++)
-                if (op->ne[i] > 1 && op->nb[i] < row_bytes(op->type, op->ne[0])) return false;   // rows that lie in one another
+            if (!b200::rows_apart(op->ne, op->nb, row_bytes(op->type, op->ne[0]))) return false;   // rows that lie in one another
             return b && op->on_device && a->type == T_F32 && (b->type == T_I64 || b->type == T_I32) &&
                    (op->type == T_F32 || op->type == T_F16 || kv_block_type(op)) && op->nb[0] == type_size(op->type) &&
                    (op->nb[1] | op->nb[2] | op->nb[3]) % unit == 0 && (uintptr_t)op->data % unit == 0 && a->nb[0] == 4 &&

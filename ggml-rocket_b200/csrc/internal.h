@@ -48,6 +48,22 @@ inline cudaError_t launch_pdl_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 
     return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// Whether no two rows (of `row` bytes, dims 1 to 3) share bytes: sorted by stride, each dim steps over all that
+// the ones below it reach.
+inline bool rows_apart(const int64_t ne[4], const size_t nb[4], size_t row) {
+    bool used[4] = {true, ne[1] <= 1, ne[2] <= 1, ne[3] <= 1};
+    double reach = (double)row;                  // exact below 2^53, which no memory passes
+    for (int n = 0; n < 3; n++) {
+        int at = 0;
+        for (int i = 1; i < 4; i++)
+            if (!used[i] && (at == 0 || nb[i] < nb[at])) at = i;
+        if (at == 0) break;
+        if ((double)nb[at] < reach) return false;
+        reach += (double)nb[at] * (double)(ne[at] - 1);
+        used[at] = true;
+    }
+    return true;
+}
 int device_sm_count();
 // The give-up limit of waits on another GPU's flags (b200_set_peer_wait_limit_ns), nanoseconds.
 uint64_t peer_wait_limit_ns();

@@ -430,8 +430,7 @@ int b200_set_rows(const float* src, const int64_t sne[4], const size_t snb[4], i
     if (sne[0] > (1ll << 36) || sne[1] > INT32_MAX || sne[2] > INT32_MAX || sne[3] > INT32_MAX) return B200_E_UNSUPPORTED;
     // rows of dst that lie in one another would take values from several rows of src
     const size_t row = (size_t)(quant ? dne[0] / 32 : dne[0]) * cell;
-    for (int i = 1; i < 4; i++)
-        if (dne[i] > 1 && dnb[i] < row) return B200_E_INVALID;
+    if (!rows_apart(dne, dnb, row)) return B200_E_INVALID;
     if (snb[0] != 4 || ((snb[1] | snb[2] | snb[3]) & 3) || (reinterpret_cast<uintptr_t>(src) & 3u) ||
         ((inb[0] | inb[1] | inb[2]) & (isz - 1)) || (reinterpret_cast<uintptr_t>(idx) & (isz - 1)) ||
         dnb[0] != cell || ((dnb[1] | dnb[2] | dnb[3]) & (unit - 1)) || (reinterpret_cast<uintptr_t>(dst) & (unit - 1)))

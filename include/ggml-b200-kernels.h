@@ -292,7 +292,7 @@ int b200_get_rows(int src_type, const void * src, const int64_t sne[4], const si
                   const int64_t ine[4], const size_t inb[4], float * dst, int * dev_err, void * stream);
 /* SET_ROWS, a KV cache's write: dst[:, idx[i, j % ine[1], k % ine[2]], j, k] = src[:, i, j, k], src F32
  * [n, n_rows, ..], idx I32 (26) or I64 (27) [n_rows, ..], dst a view of F32 (0), F16 (1), Q4_0 (2) or
- * Q8_0 (8) rows with any strides (multiples of 2 bytes, 4 for F32; rows at least a row's bytes apart),
+ * Q8_0 (8) rows with any strides (multiples of 2 bytes, 4 for F32) that let no two rows share bytes,
  * quantised as ggml's reference encoders do, bit for bit (n a multiple of 32 for those). Rows that no
  * index names stay as they are; of several source rows for one destination row the last stays, as if
  * written in order. An index outside dst's rows records a device error and its row is not written. A

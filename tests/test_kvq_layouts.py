@@ -1,0 +1,44 @@
+"""Cache layouts of SET_ROWS: rows that share bytes are refused whichever dims share them, others are not, checked
+before any CUDA call."""
+import ctypes
+
+import pytest
+
+import ggml_b200 as g
+
+P = ctypes.c_void_p(1 << 20)
+
+
+def call(dne, dnb):
+    """SET_ROWS of Q4_0 rows of 64 values; a call that is not refused fails at its launch, here without a GPU."""
+    ne = (ctypes.c_int64 * 4)
+    nb = (ctypes.c_size_t * 4)
+    n2, n3 = dne[2], dne[3]
+    return g.lib().b200_set_rows(P, ne(64, 5, n2, n3), nb(4, 256, 1280, 1280 * n2), 27, P, ne(5, 1, 1, 1), nb(8, 40, 40, 40),
+                                 2, P, ne(*dne), nb(*dnb), P, None)
+
+
+@pytest.mark.parametrize("dne,dnb", [
+    ((64, 9, 2, 1), (18, 36, 36, 72)),                # a slice begins at the other's second row
+    ((64, 9, 2, 1), (18, 36, 288, 576)),              # at its last
+    ((64, 9, 2, 1), (18, 70, 36, 72)),                # rows of two slices in turn, two bytes short
+    ((64, 9, 2, 3), (18, 72, 36, 72)),                # the streams at each other's rows
+    ((64, 9, 1, 2), (18, 36, 0, 0)),
+    ((64, 9, 1, 2), (18, 36, 324, 323)),
+])
+def test_rows_that_share_bytes_are_refused(dne, dnb):
+    assert call(dne, dnb) == g.B200_E_INVALID
+
+
+@pytest.mark.parametrize("dne,dnb", [
+    ((64, 9, 2, 1), (18, 36, 324, 648)),              # slice behind slice
+    ((64, 9, 2, 1), (18, 72, 36, 648)),               # the slices' rows in turn
+    ((64, 9, 2, 3), (18, 216, 36, 72)),               # those of the streams too
+    ((64, 9, 1, 1), (18, 36, 0, 0)),                  # strides of dims of one mean nothing
+    ((64, 1, 2, 1), (18, 0, 36, 72)),
+])
+def test_rows_apart_are_taken(dne, dnb):
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("the call would launch, on made-up addresses")
+    assert call(dne, dnb) == -3                          # B200_E_CUDA
