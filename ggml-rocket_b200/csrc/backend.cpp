@@ -1858,8 +1858,10 @@ int do_glue(b200_backend* b, const b200_tensor* op) {
                                c->nb, df, b->dev_err, st);
             break;
         case B200_OP_SET_ROWS:
-            rc = b200_set_rows(reinterpret_cast<const float*>(sa), a->ne, a->nb, c->type, sc, c->ne, c->nb, op->type, d,
-                               op->ne, op->nb, b->dev_err, st);
+            if (const size_t need = b200_set_rows_workspace_size(c->ne, op->ne))
+                if (!grow(&b->ws, &b->ws_bytes, need, st)) return B200_E_CUDA;
+            rc = b200_set_rows_ws(reinterpret_cast<const float*>(sa), a->ne, a->nb, c->type, sc, c->ne, c->nb, op->type, d,
+                                  op->ne, op->nb, b->ws, b->ws_bytes, b->dev_err, st);
             break;
         case B200_OP_CPY:
             rc = b200_cpy(a->type == T_F16 ? 1 : 0, sa, a->ne, a->nb, op->type == T_F16 ? 1 : 0, d, op->ne, op->nb, st);

@@ -16,7 +16,7 @@
 //
 // Q8_0 rows of 1024 values: 12345 read back in 9.7 us (6.6 TB/s, as fast as a copy), 1999 written at scattered
 // places in 9.9 us (1.1 TB/s: every CTA scans the indices behind its own for a later row of the same place,
-// after which the work is short); 512 rows of Q4_0 written in 4.3 us, 4096 read back in 4.6 us, a single
+// after which the work is short; more rows find their last writers in a workspace, in linear time); 512 rows of Q4_0 written in 4.3 us, 4096 read back in 4.6 us, a single
 // token's in 2.5 us each: launches.
 #include <algorithm>
 #include <cstdint>
@@ -130,15 +130,34 @@ __device__ __forceinline__ void put_q8_0(const float (&x)[4], uint8_t* out) {
     if (q == 0) o16[0] = bad ? 0x7e00u : __half_as_ushort(__float2half_rn(d));
 }
 
+// The last source row of every destination row that a slice of the indices names, in two passes: -1 into each
+// of them, then the largest row. owner: [slices of idx][destination rows].
+template <bool CLEAR>
+__global__ void __launch_bounds__(KV_THREADS) set_rows_owner_kernel(const char* __restrict__ idx, Dims4 si, int idx64,
+                                                                   int64_t dst_rows, int* __restrict__ owner) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const int64_t n = si.ne[0], slice = blockIdx.y;
+    const char* ip = idx + (slice % si.ne[1]) * si.nb[1] + (slice / si.ne[1]) * si.nb[2];
+    int* own = owner + slice * dst_rows;
+    for (int64_t r = (int64_t)blockIdx.x * KV_THREADS + threadIdx.x; r < n; r += (int64_t)gridDim.x * KV_THREADS) {
+        const int64_t at = load_index(ip + r * si.nb[0], idx64);
+        if (at < 0 || at >= dst_rows) continue;
+        if constexpr (CLEAR) own[at] = -1;
+        else atomicMax(own + at, (int)r);
+    }
+}
+
 // Unit u of a slice: 128 values from 128 * (u % cpr) of source row u / cpr. A CTA takes 8 * upw
 // consecutive units of slice blockIdx.y; its rows' indices are read once, and a row that a later row
-// of the slice writes again is left to that one (the result of writing the rows in order): the CTA
-// scans the indices behind its first row once for all its rows.
+// of the slice writes again is left to that one (the result of writing the rows in order): as `owner`
+// says, or where that is null the CTA scans the indices behind its first row once for all its rows,
+// which takes time by the square of their number (2.1 ms for 131072).
 template <int TYPE, bool VEC>
 __global__ void __launch_bounds__(KV_THREADS) set_rows_kernel(const char* __restrict__ src, Dims4 ss,
                                                              const char* __restrict__ idx, Dims4 si, int idx64,
                                                              char* __restrict__ dst, Dims4 sd, int upw, int cpr,
-                                                             int* err) {
+                                                             const int* __restrict__ owner, int* err) {
     grid_dep_wait();
     grid_dep_launch();
     __shared__ int64_t row_at[KV_MAX_ROWS + 1];
@@ -153,7 +172,12 @@ __global__ void __launch_bounds__(KV_THREADS) set_rows_kernel(const char* __rest
     for (int slice = blockIdx.y; slice < slices; slice += gridDim.y) {
         const int i2 = slices == 1 ? 0 : slice % n2, i3 = slices == 1 ? 0 : slice / n2;
         const char* ip = idx;
-        if (slices > 1) ip += (i2 % (int)si.ne[1]) * si.nb[1] + (i3 % (int)si.ne[2]) * si.nb[2];
+        const int* own = owner;
+        if (slices > 1) {
+            const int j1 = i2 % (int)si.ne[1], j2 = i3 % (int)si.ne[2];
+            ip += j1 * si.nb[1] + j2 * si.nb[2];
+            if (owner) own += (j1 + j2 * si.ne[1]) * sd.ne[1];
+        }
         const char* sp = src + i2 * ss.nb[2] + i3 * ss.nb[3];
         char* dp = dst + i2 * sd.nb[2] + i3 * sd.nb[3];
         // the warp's 128 values of its units k .. k + KV_AHEAD - 1, all under way together
@@ -186,11 +210,11 @@ __global__ void __launch_bounds__(KV_THREADS) set_rows_kernel(const char* __rest
             const bool in = at >= 0 && at < sd.ne[1];
             if (!in) atomicCAS(err, 0, ERR_BAD_INDEX);
             row_at[r] = at;
-            live[r] = in ? 1 : 0;
+            live[r] = in && (!own || own[at] == r0 + r) ? 1 : 0;
         }
         __syncthreads();
         constexpr int SCAN = 4;          // indices a thread has in flight
-        for (int64_t j0 = r0 + 1 + threadIdx.x; j0 < n_rows; j0 += KV_THREADS * SCAN) {
+        for (int64_t j0 = r0 + 1 + threadIdx.x; !own && j0 < n_rows; j0 += KV_THREADS * SCAN) {
             int64_t at[SCAN];
 #pragma unroll
             for (int n = 0; n < SCAN; n++) {
@@ -369,6 +393,11 @@ __global__ void __launch_bounds__(KV_THREADS) get_rows_q_wide_kernel(const char*
     }
 }
 
+constexpr int64_t SCAN_ROWS = 131072;                  // the most rows the scan takes
+constexpr int64_t OWNER_ROWS = 2048;                   // rows from which owners are quicker (1024 values: 1999 rows 10.5
+                                                       // by the scan, 11.0 us, 4096 rows 20.2, 16.7; single values: 8192
+                                                       // rows 24, 7.3, 524288 rows 31.8 ms, 108 us)
+
 int launched(cudaError_t e) { return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? B200_OK : B200_E_CUDA; }
 
 }  // namespace
@@ -411,9 +440,22 @@ int get_rows_quant_impl(int src_type, const void* src, const int64_t sne[4], con
 
 extern "C" {
 
+size_t b200_set_rows_workspace_size(const int64_t ine[4], const int64_t dne[4]) {
+    using namespace b200;
+    if (!ine || !dne || ine[0] < OWNER_ROWS || ine[1] <= 0 || ine[2] <= 0 || dne[1] <= 0) return 0;
+    if ((double)ine[1] * (double)ine[2] * (double)dne[1] > 1e18) return 0;
+    return (size_t)(ine[1] * ine[2] * dne[1]) * 4;
+}
+
 int b200_set_rows(const float* src, const int64_t sne[4], const size_t snb[4], int idx_type, const void* idx,
                   const int64_t ine[4], const size_t inb[4], int dst_type, void* dst, const int64_t dne[4],
                   const size_t dnb[4], int* dev_err, void* stream) {
+    return b200_set_rows_ws(src, sne, snb, idx_type, idx, ine, inb, dst_type, dst, dne, dnb, nullptr, 0, dev_err, stream);
+}
+
+int b200_set_rows_ws(const float* src, const int64_t sne[4], const size_t snb[4], int idx_type, const void* idx,
+                     const int64_t ine[4], const size_t inb[4], int dst_type, void* dst, const int64_t dne[4],
+                     const size_t dnb[4], void* workspace, size_t workspace_bytes, int* dev_err, void* stream) {
     using namespace b200;
     if (!src || !idx || !dst || !dev_err || !dims_ok(sne, snb) || !dims_ok(ine, inb) || !dims_ok(dne, dnb))
         return B200_E_INVALID;
@@ -443,12 +485,30 @@ int b200_set_rows(const float* src, const int64_t sne[4], const size_t snb[4], i
     while (upw < KV_MAX_UNITS && n_units / (KV_WARPS * upw) > (int64_t)device_sm_count() * 4) upw *= 2;
     const int64_t gx = (n_units + (int64_t)KV_WARPS * upw - 1) / ((int64_t)KV_WARPS * upw);
     if (n_units > INT32_MAX - 1024 || sne[2] * sne[3] > INT32_MAX) return B200_E_UNSUPPORTED;
+    const size_t need = b200_set_rows_workspace_size(ine, dne);
+    int* owner = nullptr;
+    if (workspace && need > 0 && ine[1] * ine[2] <= 65535) {
+        if (workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3u)) return B200_E_WORKSPACE;
+        owner = static_cast<int*>(workspace);
+    } else if (sne[1] > SCAN_ROWS) {
+        return workspace ? B200_E_UNSUPPORTED : B200_E_WORKSPACE;
+    }
     const dim3 grid((unsigned)gx, (unsigned)std::min<int64_t>(sne[2] * sne[3], 65535)), block(KV_THREADS);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (owner) {
+        const dim3 og((unsigned)std::min<int64_t>((sne[1] + KV_THREADS - 1) / KV_THREADS, (int64_t)device_sm_count() * 16),
+                      (unsigned)(ine[1] * ine[2]));
+        const char* ix = static_cast<const char*>(idx);
+        const int idx64 = idx_type == KT_I64 ? 1 : 0;
+        int rc = launched(launch_pdl(set_rows_owner_kernel<true>, og, block, 0, st, ix, dims_of(ine, inb), idx64, dne[1], owner));
+        if (rc == B200_OK)
+            rc = launched(launch_pdl(set_rows_owner_kernel<false>, og, block, 0, st, ix, dims_of(ine, inb), idx64, dne[1], owner));
+        if (rc != B200_OK) return rc;
+    }
     auto go = [&](auto kernel) {
         return launched(launch_pdl(kernel, grid, block, 0, st, reinterpret_cast<const char*>(src), dims_of(sne, snb),
                                    static_cast<const char*>(idx), dims_of(ine, inb), idx_type == KT_I64 ? 1 : 0,
-                                   static_cast<char*>(dst), dims_of(dne, dnb), upw, cpr, dev_err));
+                                   static_cast<char*>(dst), dims_of(dne, dnb), upw, cpr, (const int*)owner, dev_err));
     };
     switch (dst_type) {
         case KT_Q4_0: return vec ? go(set_rows_kernel<KT_Q4_0, true>) : go(set_rows_kernel<KT_Q4_0, false>);

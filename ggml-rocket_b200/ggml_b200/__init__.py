@@ -334,6 +334,8 @@ _SIGS.update({
 _SIGS.update({
     "b200_rope_multi": (_int, [_int, _vp, _vp, _vp, _vp, _int, _int, _vp, _f, _f, _f, _vp, _vp]),
     "b200_set_rows": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp]),
+    "b200_set_rows_workspace_size": (_sz, [_vp, _vp]),
+    "b200_set_rows_ws": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _sz, _vp, _vp]),
     "b200_flash_attn_kvq_workspace_size": (_sz, [_i64] * 6),
     "b200_flash_attn_kvq": (_int, [_int, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _vp, _f,
                                    _f, _vp, _sz, _vp, _vp]),
@@ -689,10 +691,16 @@ def rope_multi(x, pos, dst, n_dims, mode, sections, freq_base=10000.0, freq_scal
     return dst
 
 
-def set_rows(src, idx, dst, dst_type, dev_err, stream=None):
+def set_rows_workspace_size(idx, dst):
+    """Bytes of workspace for `set_rows` of these: 0 where it uses none."""
+    return lib().b200_set_rows_workspace_size(_ne4(*_dims(idx)[0]), _ne4(*_dims(dst)[0]))
+
+
+def set_rows(src, idx, dst, dst_type, dev_err, stream=None, workspace=None):
     """dst[.., idx[i], :] = src[.., i, :] (b200_set_rows): src f32, idx int32 / int64 [.., n_rows], dst f32, f16 or,
-    for Q4_0 / Q8_0, a uint8 tensor whose last dim holds a row's blocks; quantised as they are written."""
-    dev = _on("set_rows", src, idx, dst, dev_err)
+    for Q4_0 / Q8_0, a uint8 tensor whose last dim holds a row's blocks; quantised as they are written. Thousands of
+    rows are quicker with a workspace of set_rows_workspace_size bytes, more than 131072 need one."""
+    dev = _on("set_rows", src, idx, dst, dev_err, workspace)
     if _type_of(src, "set_rows") != F32:
         raise B200Error("set_rows: src is f32")
     sne, snb = _dims(src)
@@ -703,9 +711,10 @@ def set_rows(src, idx, dst, dst_type, dev_err, stream=None):
         dne, dnb = _dims(dst)
     else:
         dne, dnb = _dims_q(dst, dst_type, "set_rows")
-    rc = lib().b200_set_rows(src.data_ptr(), _ne4(*sne), _ne4(*snb), _type_of(idx, "set_rows"), idx.data_ptr(), _ne4(*ine),
-                             _ne4(*inb), dst_type, dst.data_ptr(), _ne4(*dne), _ne4(*dnb), _err_of(dev_err, "set_rows"),
-                             _stream_of(stream, dev))
+    ws, wsb = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    rc = lib().b200_set_rows_ws(src.data_ptr(), _ne4(*sne), _ne4(*snb), _type_of(idx, "set_rows"), idx.data_ptr(),
+                                _ne4(*ine), _ne4(*inb), dst_type, dst.data_ptr(), _ne4(*dne), _ne4(*dnb), ws, wsb,
+                                _err_of(dev_err, "set_rows"), _stream_of(stream, dev))
     if rc:
         check(rc, "set_rows")
     return dst

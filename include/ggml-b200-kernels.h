@@ -300,6 +300,13 @@ int b200_get_rows(int src_type, const void * src, const int64_t sne[4], const si
 int b200_set_rows(const float * src, const int64_t sne[4], const size_t snb[4], int idx_type, const void * idx,
                   const int64_t ine[4], const size_t inb[4], int dst_type, void * dst, const int64_t dne[4],
                   const size_t dnb[4], int * dev_err, void * stream);
+/* The same with a workspace (4-byte aligned, b200_set_rows_workspace_size bytes: an int for every row of dst and
+ * slice of idx; 0 where there are so few indices that none is used). Finding the last of equal indices takes time
+ * by the square of n_rows without one; more than 131072 rows then return B200_E_WORKSPACE. */
+size_t b200_set_rows_workspace_size(const int64_t ine[4], const int64_t dne[4]);
+int b200_set_rows_ws(const float * src, const int64_t sne[4], const size_t snb[4], int idx_type, const void * idx,
+                     const int64_t ine[4], const size_t inb[4], int dst_type, void * dst, const int64_t dne[4],
+                     const size_t dnb[4], void * workspace, size_t workspace_bytes, int * dev_err, void * stream);
 /* element k of src (ne[0] fastest) to element k of dst, converting between f32 (0) and f16 (1)
  * (round to nearest even); dst has src's shape (any strides) or is contiguous */
 int b200_cpy(int src_type, const void * src, const int64_t sne[4], const size_t snb[4], int dst_type, void * dst,

@@ -42,3 +42,19 @@ def test_rows_apart_are_taken(dne, dnb):
     if torch.cuda.is_available():
         pytest.skip("the call would launch, on made-up addresses")
     assert call(dne, dnb) == -3                          # B200_E_CUDA
+
+
+def test_many_rows_need_a_workspace():
+    """Without one the time grows by the square of the rows."""
+    ne, nb = (ctypes.c_int64 * 4), (ctypes.c_size_t * 4)
+
+    def many(rows, ws=None, wsb=0):
+        return g.lib().b200_set_rows_ws(P, ne(64, rows, 1, 1), nb(4, 256, 256 * rows, 256 * rows), 27, P, ne(rows, 1, 1, 1),
+                                        nb(8, 0, 0, 0), 2, P, ne(64, 1 << 20, 1, 1), nb(18, 36, 0, 0), ws, wsb, P, None)
+
+    size = g.lib().b200_set_rows_workspace_size
+    assert size(ne(2047, 1, 1, 1), ne(64, 9, 1, 1)) == 0 and size(ne(2048, 3, 2, 1), ne(64, 9, 6, 2)) == 9 * 6 * 4
+    assert many(131073) == g.B200_E_WORKSPACE
+    assert many(131073, P, (1 << 22) - 1) == g.B200_E_WORKSPACE and many(5000, ctypes.c_void_p((1 << 20) + 2), 1 << 22) == g.B200_E_WORKSPACE
+    assert g.lib().b200_set_rows(P, ne(64, 1 << 20, 1, 1), nb(4, 256, 1 << 28, 1 << 28), 27, P, ne(1 << 20, 1, 1, 1),
+                                 nb(8, 0, 0, 0), 2, P, ne(64, 1 << 20, 1, 1), nb(18, 36, 0, 0), P, None) == g.B200_E_WORKSPACE
