@@ -6,7 +6,8 @@
 //         code = min(15, trunc(x * id + 8.5)), id = 1 / d in f32 (0 when d is 0); element j < 16 is
 //         the low nibble of byte j, element j + 16 its high nibble; a code c stands for (c - 8) d.
 //         The product and sum are not rounded before the truncation: one FMA rounded toward zero
-//         truncates to the same integer as the exact value.
+//         truncates to the same integer as the exact value. ggml rounds both to f32, so that about one
+//         code in two million, next to a border, differs by one; the exact one is the nearer to x.
 //   Q8_0  d = amax / 127, code = roundf(x * id), the product rounded to f32; it stands for code * d.
 //
 // Both are bound by HBM (4 bytes a value on the f32 side, 0.5625 / 1.0625 on the other; no reuse).

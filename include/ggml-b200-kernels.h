@@ -293,7 +293,9 @@ int b200_get_rows(int src_type, const void * src, const int64_t sne[4], const si
 /* SET_ROWS, a KV cache's write: dst[:, idx[i, j % ine[1], k % ine[2]], j, k] = src[:, i, j, k], src F32
  * [n, n_rows, ..], idx I32 (26) or I64 (27) [n_rows, ..], dst a view of F32 (0), F16 (1), Q4_0 (2) or
  * Q8_0 (8) rows with any strides (multiples of 2 bytes, 4 for F32) that let no two rows share bytes,
- * quantised as ggml's reference encoders do, bit for bit (n a multiple of 32 for those). Rows that no
+ * quantised by the steps of ggml's reference encoders (n a multiple of 32 for those): Q8_0 bit for bit; a Q4_0
+ * code is that of the exact x / d + 8.5 with 1 / d rounded to f32, where ggml rounds the product and the sum
+ * to f32 too, which next to a border (about one code in two million) gives the code beside it. Rows that no
  * index names stay as they are; of several source rows for one destination row the last stays, as if
  * written in order. An index outside dst's rows records a device error and its row is not written. A
  * block that holds a NaN or an infinity is stored with a NaN scale (ggml leaves it undefined). */
