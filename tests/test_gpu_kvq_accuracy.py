@@ -96,3 +96,40 @@ def test_masks_far_from_zero(cuda, T, KV):
     m[:, 2::4] = -30000 - 16 * torch.randint(0, 3, (KV,), device="cuda", generator=gen).half()
     m[:, 3::4, 400:] = 0
     check(run(q, k, v, m, 0.05), q, k, v, m, 0.05)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("S,T,H,HK,D,KV", [
+    (1, 1, 40, 1, 128, 777),
+    (1, 33, 1, 1, 64, 33),
+    (2, 1, 33, 1, 64, 5),
+    (1, 17, 2, 1, 128, 1),
+    (1, 12, 8, 2, 128, 700),         # 48 rows a KV head, the last size whatever the group
+    (2, 16, 14, 2, 64, 900),         # 112 of them in groups of seven
+    (1, 5, 56, 8, 128, 3000),
+    (1, 13, 8, 2, 128, 700),         # 52: the prompt kernel
+    (3, 1, 32, 8, 128, 2500),
+    (1, 3, 24, 3, 64, 5003),
+])
+def test_either_side_of_the_row_kernels_last_size(cuda, S, T, H, HK, D, KV, f16):
+    """One bound for both kernels, whichever takes the call."""
+    import torch
+    q, k, v = inputs(S, T, H, HK, D, KV, seed=5, q_f16=f16)
+    gen = torch.Generator(device="cuda").manual_seed(S + T + KV)
+    m = torch.randn(S, T, KV, device="cuda", generator=gen).half()
+    m[torch.rand(S, T, KV, device="cuda", generator=gen) < 0.5] = float("-inf")
+    m[:, 1:, -1] = 0.0
+    m[:, 0] = float("-inf")
+    for mask in (m, None):
+        check(run(q, k, v, mask, 1 / math.sqrt(D), f16), q, k, v, mask, 1 / math.sqrt(D))
+
+
+def test_streams_inside_keys(cuda):
+    """A cache whose streams lie side by side in a key's row: the stride of a stream below that of a key."""
+    S, T, H, HK, D, KV = 3, 1, 8, 2, 128, 300
+    q, k, v = inputs(S, T, H, HK, D, KV)
+    kk, vv = (c.transpose(0, 1).contiguous().transpose(0, 1) for c in (k, v))
+    assert kk.stride(0) < kk.stride(1)
+    check(run(q, kk, vv, None, 0.1), q, k, v, None, 0.1)
+    q, _, _ = inputs(S, 70, H, HK, D, KV)
+    check(run(q, kk, vv, None, 0.1), q, k, v, None, 0.1)
