@@ -657,6 +657,8 @@ def _dims(t):
     es = t.element_size()
     ne = list(t.shape)[::-1]
     nb = [x * es for x in t.stride()][::-1]
+    if len(ne) > 4:
+        raise B200Error(f"a tensor of {len(ne)} dims: ggml's have four at most")
     while len(ne) < 4:
         nb.append(nb[-1] * ne[-1] if nb else es)
         ne.append(1)
@@ -675,6 +677,13 @@ def _dims_q(t, kind, what):
     return ne, nb
 
 
+def _sections(s):
+    s = tuple(s)
+    if len(s) != 4:
+        raise B200Error(f"rope_multi: four sections (pairs of each axis, 0 where there is none), not {len(s)}")
+    return _sec4(*s)
+
+
 def rope_multi(x, pos, dst, n_dims, mode, sections, freq_base=10000.0, freq_scale=1.0, attn_factor=1.0, stream=None):
     """ROPE with several position axes (b200_rope_multi): x f32 / f16 [.., n_tokens, n_head, head_dim] with any
     strides, pos int32 [4, n_tokens], dst contiguous of x's shape and type (x itself when contiguous)."""
@@ -684,7 +693,7 @@ def rope_multi(x, pos, dst, n_dims, mode, sections, freq_base=10000.0, freq_scal
     if dst.dtype != x.dtype or dst.shape != x.shape or not dst.is_contiguous() or _type_of(pos, "rope_multi") != I32 or \
             not pos.is_contiguous() or pos.shape != (4, ne[2]):
         raise B200Error("rope_multi: dst is contiguous and of x's shape and type, pos contiguous int32 [4, n_tokens]")
-    rc = lib().b200_rope_multi(ty, x.data_ptr(), _ne4(*ne), _ne4(*nb), pos.data_ptr(), n_dims, mode, _sec4(*sections),
+    rc = lib().b200_rope_multi(ty, x.data_ptr(), _ne4(*ne), _ne4(*nb), pos.data_ptr(), n_dims, mode, _sections(sections),
                                freq_base, freq_scale, attn_factor, dst.data_ptr(), _stream_of(stream, dev))
     if rc:
         check(rc, "rope_multi")
@@ -750,6 +759,8 @@ def flash_attn_kvq(kv_type, q, k, v, mask, dst, scale, workspace, dev_err, softc
     [S, KV, HK, D / 32 * 18] (Q4_0 blocks), mask f16 [S or 1, T, KV] or None, dst contiguous f32 / f16 [S, T, H, D];
     strides of q, k, v and mask are theirs."""
     dev = _on("flash_attn_kvq", q, k, v, mask, dst, workspace, dev_err)
+    if q.dim() != 4:
+        raise B200Error("flash_attn_kvq: q is [S, T, H, D]")
     S, T, H, D = q.shape
     es = q.element_size()
     qs, qt, qh, qd = q.stride()

@@ -58,3 +58,13 @@ def test_many_rows_need_a_workspace():
     assert many(131073, P, (1 << 22) - 1) == g.B200_E_WORKSPACE and many(5000, ctypes.c_void_p((1 << 20) + 2), 1 << 22) == g.B200_E_WORKSPACE
     assert g.lib().b200_set_rows(P, ne(64, 1 << 20, 1, 1), nb(4, 256, 1 << 28, 1 << 28), 27, P, ne(1 << 20, 1, 1, 1),
                                  nb(8, 0, 0, 0), 2, P, ne(64, 1 << 20, 1, 1), nb(18, 36, 0, 0), P, None) == g.B200_E_WORKSPACE
+
+
+def test_wrappers_name_shapes_they_do_not_take():
+    """As B200Error, before any CUDA call."""
+    import torch
+    with pytest.raises(g.B200Error, match="5 dims"):
+        g._dims(torch.zeros(1, 1, 1, 1, 1))
+    with pytest.raises(g.B200Error, match="four sections"):
+        g._sections([16, 24, 24])
+    assert g._sections([16, 24, 24, 0]) == b"".join(v.to_bytes(4, "little") for v in (16, 24, 24, 0))
