@@ -1766,7 +1766,8 @@ int do_flash_attn(b200_backend* b, b200_tensor* op) {
             kd = base, k_nb1 = (int64_t)D * 2, k_nb2 = (int64_t)KV * D * 2;
         }
         if (v->type != T_F16) {
-            const int rc = b200_kv_to_f16(v->type, vd, DV, KV, HK, v_nb1, v_nb2, base + kb, b->stream);
+            const int rc = b200::kv_to_f16_impl(v->type, vd, DV, KV, HK, v_nb1, v_nb2, base + kb, k->type != T_F16 ? base : nullptr,
+                                                D, b->stream);
             if (rc != B200_OK) return rc;
             vd = base + kb, v_nb1 = (int64_t)DV * 2, v_nb2 = (int64_t)KV * DV * 2;
         }

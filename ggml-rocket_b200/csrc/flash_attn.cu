@@ -703,7 +703,7 @@ fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUten
                             const uint32_t mw = (&mv[e >> 3].x)[(e & 7) >> 1];
                             const uint16_t mb = (uint16_t)((e & 1) ? (mw >> 16) : (mw & 0xFFFFu));
                             sv = fmaf(__half2float(__ushort_as_half(mb)) - ref, LOG2E, sv);
-                            if (EXT && mb == 0xFC00u) sv = -INFINITY;
+                            if (mb == 0xFC00u) sv = -INFINITY;   // whatever its score is
                         }
                         if (k0 + c0 + e >= args.KV) sv = -INFINITY;
                         x[c0 + e] = sv;
@@ -1343,9 +1343,12 @@ namespace b200 {
 // One thread per 32-value block of a [HK][KV][D] view (rows nb1 bytes apart, heads nb2): ggml's
 // dequantize_row_q8_0 / _q4_0 (y = q * d, resp. (nibble - 8) * d, in f32), then fp16 (nearest
 // even), written contiguous [HK][KV][D]. Blocks are 2-byte aligned only: byte loads.
+// keys (the fp16 keys of these values, k_dim a key; or null): a block with values that are no finite fp16 numbers is
+// written as zeros and its key's first value as a NaN, so that rows that see the key still become NaN, through their
+// scores, and rows whose mask hides it stay clear of it (in the product of weights and values 0 * NaN is NaN).
 template <int TYPE>
 __global__ void kv_to_f16_kernel(const uint8_t* __restrict__ src, int64_t D, int64_t KV, int64_t HK, int64_t nb1,
-                                 int64_t nb2, __half* __restrict__ dst) {
+                                 int64_t nb2, __half* __restrict__ dst, __half* __restrict__ keys, int64_t k_dim) {
     grid_dep_wait();
     grid_dep_launch();
     const int64_t per_row = D / 32, total = HK * KV * per_row;
@@ -1371,10 +1374,37 @@ __global__ void kv_to_f16_kernel(const uint8_t* __restrict__ src, int64_t D, int
             w[e / 2] = (uint32_t)__half_as_ushort(__float2half_rn(v0)) |
                        ((uint32_t)__half_as_ushort(__float2half_rn(v1)) << 16);
         }
+        if (keys) {
+            bool bad = false;
+#pragma unroll
+            for (int e = 0; e < 16; e++) bad |= (w[e] & 0x7c00u) == 0x7c00u || (w[e] & 0x7c000000u) == 0x7c000000u;
+            if (bad) {
+                keys[(h * KV + r) * k_dim] = __ushort_as_half((unsigned short)0x7e00);
+#pragma unroll
+                for (int e = 0; e < 16; e++) w[e] = 0u;
+            }
+        }
         uint4* o = reinterpret_cast<uint4*>(dst + (h * KV + r) * D + 32 * c);
 #pragma unroll
         for (int q = 0; q < 4; q++) o[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
     }
+}
+
+int kv_to_f16_impl(int type, const void* src, int64_t D, int64_t KV, int64_t HK, int64_t nb1, int64_t nb2, void* dst,
+                   void* keys, int64_t k_dim, cudaStream_t st) {
+    if (!src || !dst || D <= 0 || KV <= 0 || HK <= 0 || nb1 <= 0 || nb2 <= 0) return B200_E_INVALID;
+    if ((type != 8 && type != 2) || D % 32 != 0 || (reinterpret_cast<uintptr_t>(dst) & 15u) != 0)
+        return B200_E_UNSUPPORTED;
+    const int64_t total = HK * KV * (D / 32);
+    const int threads = 256;
+    const int64_t want = (total + threads - 1) / threads;
+    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(want, (int64_t)device_sm_count() * 16));
+    auto go = [&](auto kernel) {
+        return launch_pdl(kernel, dim3(grid), dim3(threads), 0, st, static_cast<const uint8_t*>(src), D, KV, HK, nb1, nb2,
+                          static_cast<__half*>(dst), static_cast<__half*>(keys), k_dim);
+    };
+    const cudaError_t e = type == 8 ? go(kv_to_f16_kernel<8>) : go(kv_to_f16_kernel<2>);
+    return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? B200_OK : B200_E_CUDA;
 }
 
 }  // namespace b200
@@ -1383,23 +1413,8 @@ extern "C" {
 
 int b200_kv_to_f16(int type, const void* src, int64_t D, int64_t KV, int64_t HK, int64_t nb1, int64_t nb2, void* dst,
                    void* stream) {
-    using namespace b200;
-    if (!src || !dst || D <= 0 || KV <= 0 || HK <= 0 || nb1 <= 0 || nb2 <= 0) return B200_E_INVALID;
-    if ((type != 8 && type != 2) || D % 32 != 0 || (reinterpret_cast<uintptr_t>(dst) & 15u) != 0)
-        return B200_E_UNSUPPORTED;
-    const int64_t total = HK * KV * (D / 32);
-    const int threads = 256;
-    const int64_t want = (total + threads - 1) / threads;
-    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(want, (int64_t)device_sm_count() * 16));
-    const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const cudaError_t e =
-        type == 8 ? launch_pdl(kv_to_f16_kernel<8>, dim3(grid), dim3(threads), 0, st,
-                               static_cast<const uint8_t*>(src), D, KV, HK, nb1, nb2, static_cast<__half*>(dst))
-                  : launch_pdl(kv_to_f16_kernel<2>, dim3(grid), dim3(threads), 0, st,
-                               static_cast<const uint8_t*>(src), D, KV, HK, nb1, nb2, static_cast<__half*>(dst));
-    return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? B200_OK : B200_E_CUDA;
+    return b200::kv_to_f16_impl(type, src, D, KV, HK, nb1, nb2, dst, nullptr, 0, static_cast<cudaStream_t>(stream));
 }
-
 
 size_t b200_flash_attn_workspace_size(int D, int DV, int T, int H, int KV, int HK) {
     (void)DV;

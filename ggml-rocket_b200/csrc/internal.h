@@ -110,6 +110,9 @@ struct FaQuantArgs {
 int64_t fa_quant_tiles(int64_t T, int64_t H, int64_t HK);
 size_t fa_quant_workspace(int64_t D, int64_t T, int64_t H, int64_t KV, int64_t HK, int64_t S);
 cudaError_t fa_quant_run(const FaQuantArgs& q, char* ws, cudaStream_t st);
+// b200_kv_to_f16; keys, not null: the fp16 keys (k_dim values each) of the values being converted, see flash_attn.cu.
+int kv_to_f16_impl(int type, const void* src, int64_t D, int64_t KV, int64_t HK, int64_t nb1, int64_t nb2, void* dst,
+                   void* keys, int64_t k_dim, cudaStream_t st);
 // b200_get_rows over a Q4_0 (2) / Q8_0 (8) table (kv_cache.cu); pointers, shapes and idx checked before.
 int get_rows_quant_impl(int src_type, const void* src, const int64_t sne[4], const size_t snb[4], const int32_t* idx,
                         const int64_t ine[4], const size_t inb[4], float* dst, int* dev_err, cudaStream_t st);

@@ -69,6 +69,23 @@ if sys.argv[2] == "routes":
         out, by = graph(q, k, v, m)
         assert by == [1, 1, 0], (S, T, H, KV, by)
         assert torch.equal(out, run(q, k, v, m, 0.09))
+elif sys.argv[2] == "garbage":
+    # cells no row sees, and one the last token alone does, of bytes that decode to NaN and infinity
+    T, H, HK, D, KV = 512, 32, 8, 128, 2048
+    q, k, v = inputs(1, T, H, HK, D, KV)
+    m = causal(1, T, KV, [1500])
+    clean, by = graph(q, k, v, m)
+    assert by == [1, 0, 1]
+    k[:, 1500:], v[:, 1500:] = 0xff, 0xff
+    k[:, 1600:1700, :, 1::18], v[:, 1600:1700, :, 1::18] = 0x7c, 0x7c
+    v[:, 1700:1800, :, 1::18] = 0x7a               # scales of fp16's largest size: code * scale is past its range
+    assert torch.equal(graph(q, k, v, m)[0], clean)
+    v[0, 1499, 2, 0], v[0, 1499, 2, 1] = 0xff, 0x7f
+    got = graph(q, k, v, m)[0]
+    assert torch.equal(got[:, :T - 1], clean[:, :T - 1])
+    assert bool(torch.isnan(got[0, T - 1, 8:12]).all())
+    got[0, T - 1, 8:12] = clean[0, T - 1, 8:12]
+    assert torch.equal(got, clean)
 else:
     # sixteen streams whose tiles would take 4.4 GB
     S, T, H, HK, D, KV = 16, 13, 32, 8, 128, 32768
@@ -87,7 +104,7 @@ print("DONE")
 """
 
 
-@pytest.mark.parametrize("what", ["routes", "memory"])
+@pytest.mark.parametrize("what", ["routes", "garbage", "memory"])
 def test_routes_and_memory(cuda, what):
     env = {k: v for k, v in os.environ.items() if not k.startswith("B200_")}
     env.update(B200_FA_QUANT_KV="1")
