@@ -31,16 +31,18 @@
 // the rows are never fetched: the CTA reads its mask range first. Caches TMA cannot address (heads not
 // side by side, bases or strides off 16 bytes, a number of heads that does not divide) take the same
 // arithmetic with cp.async copies of 8 (4) bytes, of which an SM moves about one a cycle (32 streams x 16384
-// keys: 498 us so, 175 by TMA when that came).
+// keys: 498 us so, 175 by TMA when that came). One KV head of 128 or two of 64 go that way: 32 streams, 38 us with
+// one head of 128 (29 a head with two).
 //
 // With few rows the keys are split over CTAs, whose parts are joined through the shared memory of a cluster
 // or by a second kernel. Calls with more rows go to the tcgen05 kernel of flash_attn.cu (see by_rows below).
 //
 // Bound by the issue of instructions, not by HBM: about 30 a key and KV head (decoding the codes, their
-// fragments, the softmax). 64 streams x 32000 keys, 8 KV heads of 128: 554 us, 3.2 TB/s of cache, 0.49 of
-// the measured copy bandwidth, 63 % of the issue slots; 32 streams of 8192 to 16384 keys 178 us (2.6 TB/s; 164
-// with softmax weights of fp16, which an fp16 result showed).
-// A single stream is latency: 16384 keys 17.2 us, 512 keys 7.4 us, of which some 4 are launch, mask and q.
+// fragments, the softmax). 64 streams of 16000 to 32000 keys, 8 KV heads of 128: 616 us, 2.9 TB/s of cache, 0.44
+// of the measured copy bandwidth, 64 % of the issue slots; 32 streams of 8192 to 16384 keys 181 us (2.5 TB/s; 166
+// with softmax weights of fp16, which an fp16 result showed). Some 15 % of that is SMs done before the others.
+// A single stream: 16384 keys 17.6 us, 512 keys 7.6 us, of which some 4 are launch, mask and q; where the other ten
+// of the long one go has not been taken apart (three tiles a CTA, a join in the cluster, a join of 11 parts).
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -936,11 +938,13 @@ cudaError_t launch_kvq(const CUtensorMap& tk, const CUtensorMap& tv, const KvqAr
                       (const float*)a.part, (const float*)a.stat, parts, a.dst_f16, a.dst);
 }
 
-// Whether the row kernels take the call, or the tcgen05 kernel over fp16 tiles of the cache. With 32 heads of
-// 128 over 8 KV heads and 16384 keys the row kernels take 15 us and 0.9 us for every 8 rows of a KV head; the
-// other 50 us to make the tiles and 1.25 us for every query tile it has (128 rows, of several heads where
-// a power of two of them shares a KV head). 12 tokens: 56 against 63 us, 16: 69 against 64; 5 tokens of 56
-// heads 55 against 121. 4096 keys cross at the same place (12 tokens 23.5 against 26.7, 24: 35 against 28).
+// Whether the row kernels take the call, or the tcgen05 kernel over fp16 tiles of the cache. The row kernels take
+// some 15 us and 0.95 for every 8 rows of a KV head, the other the time to make the tiles and 0.6 for every query
+// tile it has (128 rows, of several heads where a power of two of them shares a KV head). In us, rows / tiles, f16:
+// 32 heads of 128 over 8, 16384 keys: 12 tokens 61 / 66, 16 88 / 67; 4096 keys: 12 tokens 25 / 30, 16 30 / 30, 24
+// 38 / 31, four streams of them 61 / 67, 88 / 67, 118 / 67; 56 heads over 8, 4096 keys: 16 tokens 44 / 51, 24 53 /
+// 51; 14 heads of 64 over 2, 4096 keys: 16 tokens 16 / 21, 32 21 / 22. The number of keys does not enter, so that
+// with 1024 the tiles come too early (32 heads over 8: 16 tokens 16 / 25, 48 tokens 23 / 28, 64 31 / 28).
 bool by_rows(int64_t T, int64_t H, int64_t HK) {
     const int64_t row_tiles = HK * ((T * (H / HK) + KR_ROWS - 1) / KR_ROWS);
     return 5 * row_tiles <= 25 * HK + 7 * fa_quant_tiles(T, H, HK);

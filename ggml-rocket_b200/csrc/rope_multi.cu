@@ -15,7 +15,8 @@
 // a thread per (token, pair) computes the cosine and sine into shared memory for every head of the
 // token, so that the 64-bit work hides behind the loads. 4096 tokens x 32 heads x 128 f32 (134 MB): 23.5 us,
 // 5.7 TB/s, 0.87 of the measured copy bandwidth (30.3 us with two items in flight and a 64-bit exp2 a pair).
-// A picture's 27.5 MB take 9.0 us (3.1 TB/s: a wave and a half), a few tokens 2.9 us, a launch.
+// A picture's 27.5 MB take 9.0 us (3.1 TB/s: 445 CTAs, three quarters of one wave, which load together and
+// store together), a few tokens 2.9 us, a launch.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>

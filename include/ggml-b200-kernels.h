@@ -178,12 +178,14 @@ int    b200_kv_to_f16(int type, const void * src, int64_t D, int64_t KV, int64_t
  *   dst[:, h, t, s] = sum_j softmax_j(S[j]) v[:, j, h / (H / HK), s],
  *   S[j] = softcap * tanh(scale * q.k / softcap) (scale * q.k when softcap == 0) + mask[s][t][j]
  * A key whose mask is -inf takes no part, whatever its bytes hold; a row with no other key is zeros. D in
- * {64, 128}, H % HK == 0, KV <= 2^30, dst 16-byte aligned. An F32 dst has fp32's accuracy (relative to the
- * largest value of a key's head), an F16 dst adds its own rounding alone. With at most 48 query rows a KV head
- * (T * H / HK), and with more where that is faster, the cache's codes enter the products as they are. Otherwise
- * the cache is brought to pairs of fp16 tiles in the workspace once, which hold its values exactly; there a key
- * with a block scale above 8188 (whose values may leave fp16's range) is no number to rows that see it. The
- * workspace (256-byte aligned,
+ * {64, 128}, H % HK == 0, KV <= 2^30, dst 16-byte aligned and apart from the inputs. Every operand enters the
+ * products to 22 bits at least and sums are fp32 (a value's error is relative to the largest of its key's head);
+ * an F16 dst adds its own rounding. With at most 48 query rows a KV head (T * H / HK), and with more where that is
+ * faster, the cache's codes enter as they are: an F32 dst is off by 3e-7 of its size. Otherwise the cache is
+ * brought to pairs of fp16 tiles in the workspace once, which hold its values exactly, and the sums of all keys
+ * are formed in the tensor core, which truncates: off by 4e-6 over 1024 keys, 1.5e-5 over 32768; there a key with
+ * a block scale above 8188 (whose values may leave fp16's range) is no number to rows that see it. The workspace
+ * (256-byte aligned,
  * b200_flash_attn_kvq_workspace_size bytes; the calling device's) holds that and the parts of rows whose
  * keys several CTAs share; calls sharing one must not overlap on the GPU.
  * No ALiBi, no sinks. */
