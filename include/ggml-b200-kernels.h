@@ -306,7 +306,8 @@ int b200_set_rows(const float * src, const int64_t sne[4], const size_t snb[4], 
                   const size_t dnb[4], int * dev_err, void * stream);
 /* The same with a workspace (4-byte aligned, b200_set_rows_workspace_size bytes: an int for every row of dst and
  * slice of idx; 0 where there are so few indices that none is used). Finding the last of equal indices takes time
- * by the square of n_rows without one; more than 131072 rows then return B200_E_WORKSPACE. */
+ * by the square of n_rows without one; more than 131072 rows then return B200_E_WORKSPACE. Calls sharing a workspace
+ * must not overlap on the GPU. */
 size_t b200_set_rows_workspace_size(const int64_t ine[4], const int64_t dne[4]);
 int b200_set_rows_ws(const float * src, const int64_t sne[4], const size_t snb[4], int idx_type, const void * idx,
                      const int64_t ine[4], const size_t inb[4], int dst_type, void * dst, const int64_t dne[4],

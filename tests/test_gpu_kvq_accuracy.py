@@ -133,3 +133,30 @@ def test_streams_inside_keys(cuda):
     check(run(q, kk, vv, None, 0.1), q, k, v, None, 0.1)
     q, _, _ = inputs(S, 70, H, HK, D, KV)
     check(run(q, kk, vv, None, 0.1), q, k, v, None, 0.1)
+
+
+@pytest.mark.parametrize("S,T,H,HK,D,KV", [(1, 70, 8, 2, 128, 3000), (2, 300, 32, 8, 64, 700)])
+def test_prompts_repeat_exactly_and_replay(cuda, S, T, H, HK, D, KV):
+    """Whole tiles, and tiles whose keys CTAs share; nothing is expected of the workspace's bytes."""
+    import torch
+    import ggml_b200 as g
+    from test_gpu_flash_attn_kvq import workspace
+    q, k, v = inputs(S, T, H, HK, D, KV)
+    m = causal(S, T, KV)
+    want = run(q, k, v, m, 0.1)
+    assert all(torch.equal(run(q, k, v, m, 0.1), want) for _ in range(3))
+    out, ws = torch.empty_like(q), workspace(D, T, H, KV, HK, S)
+    ws.fill_(0xff)
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        g.flash_attn_kvq(2, q, k, v, m, out, 0.1, ws, err)
+    for seed in (5, 6):
+        for a, b in zip((q, k, v), inputs(S, T, H, HK, D, KV, seed=seed)):
+            a.copy_(b)
+        m.copy_(causal(S, T, KV, [KV - 100 * s - seed for s in range(S)]))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(err.item()) == 0 and torch.equal(out, run(q, k, v, m, 0.1))
+        check(out, q, k, v, m, 0.1)
